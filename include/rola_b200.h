@@ -367,6 +367,90 @@ int rola_b200_pipeline_forward(rola_pipeline* pl, const void* x_host, const void
 int rola_b200_pipeline_wait(rola_pipeline* pl, rola_stream_t stream);
 int rola_b200_pipeline_destroy(rola_pipeline* pl);
 
+/* --------------------------------------------------------------------------
+ * The cross-attention sublayer of a DiT block: norm with the residual's
+ * addition, e4m3 product with a scale per block of 128, attention to an
+ * encoder's states.  `*_fp32` flags: 1 = the tensor is fp32, 0 = bf16.
+ * -------------------------------------------------------------------------- */
+
+/* h = x + res in res's type; y = h (mean_k h^2 + eps)^-1/2 w, rounded once to
+ * bf16.  x, res: [M, K] rows with strides x_ld, res_ld (elements, 16-byte
+ * rows); res and h both NULL: h = x.  w [K]; h, y [M, K] dense; rstd [M] fp32
+ * (the row factor, for the backward) or NULL.  K % 8 == 0, K <= 16384.
+ * The reference's WanRMSNorm (sparkdiffusion/networks/wan2pt1.py:188-206)
+ * rounds the unit row to x's type before the weight; here the product is
+ * rounded once. */
+int rola_b200_add_rms_norm(const void* x, int x_fp32, int64_t x_ld, const void* res, int res_fp32, int64_t res_ld,
+                           const void* w, int w_fp32, int64_t M, int64_t K, float eps, void* h, void* y, float* rstd,
+                           rola_stream_t stream);
+
+/* The same with y in e4m3: yq = e4m3(y / scale), scale = max|y| / 448 + 1e-12
+ * (fp32, from the unrounded y) over each 128 columns (block == 128; scale of
+ * row m and block c at scale + m*scale_sM + c*scale_sK) or over the row
+ * (block == 0; scale [M], for rola_b200_qkv_gemm_fp8).  yq [M, K] bytes. */
+int rola_b200_add_rms_norm_e4m3(const void* x, int x_fp32, int64_t x_ld, const void* res, int res_fp32, int64_t res_ld,
+                                const void* w, int w_fp32, int64_t M, int64_t K, float eps, void* h, void* yq,
+                                float* scale, int64_t scale_sM, int64_t scale_sK, int block, rola_stream_t stream);
+
+/* Backward of rola_b200_add_rms_norm: dx = dres = dh + rstd (g - u mean(g u)),
+ * g = dy w, u = h rstd, each in its own type (dres NULL: not written; dh NULL:
+ * zero); dw = sum_m dy u in w's type (NULL: skipped), summed in a fixed order.
+ * dy bf16; h, dy, dh with row strides; dx, dres dense.  workspace (for dw):
+ * rola_b200_add_rms_norm_bwd_workspace bytes, 16-byte aligned. */
+size_t rola_b200_add_rms_norm_bwd_workspace(int64_t M, int64_t K);
+int rola_b200_add_rms_norm_bwd(const void* h, int h_fp32, int64_t h_ld, const void* w, int w_fp32, const float* rstd,
+                               const void* dy, int64_t dy_ld, const void* dh, int dh_fp32, int64_t dh_ld, int64_t M,
+                               int64_t K, void* dx, int dx_fp32, void* dres, int dres_fp32, void* dw, void* workspace,
+                               size_t workspace_bytes, rola_stream_t stream);
+
+/* e4m3 quantisation of activations [M, K] with a scale per row and 128 columns
+ * (as rola_b200_add_rms_norm_e4m3 with block == 128, without the norm) and of a
+ * weight [N, K] with a scale per 128 x 128 block, scale
+ * [ceil(N/128), ceil(K/128)]. */
+int rola_b200_quantize_blocks_e4m3(const void* x, int x_fp32, int64_t x_ld, int64_t M, int64_t K, void* xq,
+                                   float* scale, int64_t scale_sM, int64_t scale_sK, rola_stream_t stream);
+int rola_b200_quantize_tiles_e4m3(const void* w, int w_fp32, int64_t ld, int64_t N, int64_t K, void* wq, float* scale,
+                                  rola_stream_t stream);
+
+/* out[M, N] = bf16(sum_kb x_scale[m, kb] w_scale[n/128, kb] (xq . wq^T over the
+ * 128 columns of block kb) + bias[n]), fp32 sums.  xq [M, K], wq [N, K] e4m3,
+ * dense; x_scale of row m and block kb at m*xs_sM + kb*xs_sK; w_scale
+ * [ceil(N/128), ceil(K/128)]; bias bf16 [N] or NULL.  N % 8 == 0, K % 16 == 0. */
+int rola_b200_gemm_fp8_block(const void* xq, const float* x_scale, int64_t xs_sM, int64_t xs_sK, const void* wq,
+                             const float* w_scale, const void* bias, void* out, int64_t M, int64_t N, int64_t K,
+                             rola_stream_t stream);
+
+/* Attention of q [B, H, Lq, 128] to k, v [B, Hkv, Lk, 128] (bf16; element
+ * (b, h, t, d) at p + sB*b + sH*h + sT*t + d, positive strides, multiples of 8;
+ * H % Hkv == 0, query head h reads key head h / (H / Hkv)), softmax of
+ * q.k 128^-1/2 over the keys j < kv_lens[b] (int32 [B] on the device, clamped
+ * to [0, Lk]; NULL: Lk).  What k and v hold past kv_lens[b] has no effect.  A
+ * row without keys is 0.  lse (NULL to skip): fp32 [B*H, 128*ceil(Lq/128)],
+ * base-2 log-sum-exp in units of 128^-1/2 log2(e), +inf on padding rows and
+ * rows without keys.  workspace: rola_b200_cross_attn_workspace bytes (0 when
+ * the keys are not cut), 16-byte aligned; calls that may overlap on the GPU
+ * need their own.  The reference's cross-attention calls its attention op
+ * (sparkdiffusion/utils/attention.py:122-186). */
+size_t rola_b200_cross_attn_workspace(int B, int H, int Hkv, int Lq, int Lk);
+int rola_b200_cross_attn(const void* q, int64_t q_sB, int64_t q_sH, int64_t q_sT, const void* k, int64_t k_sB,
+                         int64_t k_sH, int64_t k_sT, const void* v, int64_t v_sB, int64_t v_sH, int64_t v_sT,
+                         const int32_t* kv_lens, int B, int H, int Hkv, int Lq, int Lk, void* out, int64_t o_sB,
+                         int64_t o_sH, int64_t o_sT, float* lse, void* workspace, size_t workspace_bytes,
+                         rola_stream_t stream);
+
+/* Its backward: dq [B, H, Lq, 128], dk and dv [B, Hkv, Lk, 128] (shared
+ * strides; summed over the query heads of a key head; 0 past kv_lens[b]) from
+ * the forward's out and lse and from dout.  No atomics: the same inputs give the
+ * same bits.  workspace: rola_b200_cross_attn_bwd_workspace bytes. */
+size_t rola_b200_cross_attn_bwd_workspace(int B, int H, int Hkv, int Lq, int Lk);
+int rola_b200_cross_attn_bwd(const void* q, int64_t q_sB, int64_t q_sH, int64_t q_sT, const void* k, int64_t k_sB,
+                             int64_t k_sH, int64_t k_sT, const void* v, int64_t v_sB, int64_t v_sH, int64_t v_sT,
+                             const void* out, int64_t o_sB, int64_t o_sH, int64_t o_sT, const void* dout, int64_t do_sB,
+                             int64_t do_sH, int64_t do_sT, const int32_t* kv_lens, const float* lse, int B, int H,
+                             int Hkv, int Lq, int Lk, void* dq, int64_t dq_sB, int64_t dq_sH, int64_t dq_sT, void* dk,
+                             void* dv, int64_t dkv_sB, int64_t dkv_sH, int64_t dkv_sT, void* workspace,
+                             size_t workspace_bytes, rola_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

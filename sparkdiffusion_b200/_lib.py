@@ -68,6 +68,20 @@ SIGNATURES = {
     "rola_b200_sparse_attn_bwd_workspace": [_I, _I, _I, _I],
     "rola_b200_sparse_attn_bwd": [_P, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _L, _L, _L, _P, _P, _P, _I, _I, _I,
                                   _I, _I, _P, _P, _P, _L, _L, _L, _P, _Z, _P],
+    "rola_b200_add_rms_norm": [_P, _I, _L, _P, _I, _L, _P, _I, _L, _L, _F, _P, _P, _P, _P],
+    "rola_b200_add_rms_norm_e4m3": [_P, _I, _L, _P, _I, _L, _P, _I, _L, _L, _F, _P, _P, _P, _L, _L, _I, _P],
+    "rola_b200_add_rms_norm_bwd_workspace": [_L, _L],
+    "rola_b200_add_rms_norm_bwd": [_P, _I, _L, _P, _I, _P, _P, _L, _P, _I, _L, _L, _L, _P, _I, _P, _I, _P, _P, _Z,
+                                   _P],
+    "rola_b200_quantize_blocks_e4m3": [_P, _I, _L, _L, _L, _P, _P, _L, _L, _P],
+    "rola_b200_quantize_tiles_e4m3": [_P, _I, _L, _L, _L, _P, _P, _P],
+    "rola_b200_gemm_fp8_block": [_P, _P, _L, _L, _P, _P, _P, _P, _L, _L, _L, _P],
+    "rola_b200_cross_attn_workspace": [_I, _I, _I, _I, _I],
+    "rola_b200_cross_attn": [_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _I, _I, _I, _I, _I, _P, _L, _L, _L,
+                             _P, _P, _Z, _P],
+    "rola_b200_cross_attn_bwd_workspace": [_I, _I, _I, _I, _I],
+    "rola_b200_cross_attn_bwd": [_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P,
+                                 _P, _I, _I, _I, _I, _I, _P, _L, _L, _L, _P, _P, _L, _L, _L, _P, _Z, _P],
     "rola_b200_peer_alloc": [_Z, ctypes.POINTER(_P), _P],
     "rola_b200_peer_open": [_P, ctypes.POINTER(_P)],
     "rola_b200_peer_close": [_P],
@@ -87,6 +101,9 @@ _RESTYPES = {
     "rola_b200_last_error": ctypes.c_char_p,
     "rola_b200_forward_workspace_bytes": _Z,
     "rola_b200_sparse_attn_bwd_workspace": _Z,
+    "rola_b200_add_rms_norm_bwd_workspace": _Z,
+    "rola_b200_cross_attn_workspace": _Z,
+    "rola_b200_cross_attn_bwd_workspace": _Z,
 }
 
 MAX_RANKS = 8

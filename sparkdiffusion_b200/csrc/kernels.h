@@ -176,4 +176,97 @@ int launch_lut_invert(const int32_t* lut, int BH, int NBq, int NBk, int topk, in
 int launch_attn_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
                     const AttnBwdParams& p, cudaStream_t s);
 
+// norm.cu -----------------------------------------------------------------
+struct AddRmsNormParams {
+  const void* x;    // [M, K], row stride x_ld (elements), bf16 or fp32
+  const void* res;  // [M, K], row stride res_ld, or nullptr
+  const void* w;    // [K]
+  void* h;          // [M, K] in res's type (with res)
+  void* y;          // bf16 [M, K], or nullptr: e4m3 output
+  void* yq;         // e4m3 [M, K]
+  float* scale;     // (m, block) at m * scale_sM + block * scale_sK; scale_row: [M]
+  float* rstd;      // [M] or nullptr
+  int64_t x_ld, res_ld, M, scale_sM, scale_sK;
+  int K;
+  bool x_fp32, res_fp32, w_fp32, scale_row;
+  bool norm;        // false: quantise x as it is
+  float eps;
+};
+int launch_add_rms_norm(const AddRmsNormParams& p, cudaStream_t s);
+struct AddRmsNormBwdParams {
+  const void* h;      // [M, K], row stride h_ld
+  const void* w;      // [K]
+  const float* rstd;  // [M]
+  const void* dy;     // bf16 [M, K], row stride dy_ld
+  const void* dh;     // [M, K], row stride dh_ld, or nullptr
+  void* dx;           // [M, K]
+  void* dres;         // [M, K] or nullptr
+  float* dw_part;     // [add_rms_norm_bwd_parts, K] or nullptr (no dw)
+  void* dw;           // [K] in w's type
+  int64_t h_ld, dy_ld, dh_ld, M;
+  int K;
+  bool h_fp32, w_fp32, dh_fp32, dx_fp32, dres_fp32;
+};
+int add_rms_norm_bwd_parts(int64_t M, int K);  // rows of dw_part
+int launch_add_rms_norm_bwd(const AddRmsNormBwdParams& p, cudaStream_t s);
+// weight [N, K] (row stride ld) -> wq [N, K], scale [ceil(N/128), scale_ld]
+int launch_quantize_tiles_e4m3(const void* w, bool w_fp32, int64_t ld, int N, int K, uint8_t* wq, float* scale,
+                               int64_t scale_ld, cudaStream_t s);
+
+// gemm_block.cu -----------------------------------------------------------
+struct GemmBlockParams {
+  const uint8_t* xq;  // [M, K]
+  const uint8_t* wq;  // [N, K]
+  const float* xs;    // (m, kb) at m * xs_sM + kb * xs_sK
+  const float* ws;    // [ceil(N/128), ws_ld]
+  const __nv_bfloat16* bias;  // [N] or nullptr
+  __nv_bfloat16* out;         // [M, N]
+  int64_t xs_sM, xs_sK, ws_ld;
+  int M, N, K;
+};
+// rows of the W box the launch for these sizes loads (the map of W is made with it)
+int gemm_block_w_rows(int M, int N, int K);
+int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, cudaStream_t s);
+
+// cross_attn.cu -----------------------------------------------------------
+struct CrossAttnPlan {
+  bool pack;     // the G query heads of a key head share one tile (G * Lq <= 128)
+  int nqt, nqp;  // 128-row query tiles and pairs of them, per (b, head of the grid)
+  int nsplit;    // slices of the keys
+};
+CrossAttnPlan cross_attn_plan(int B, int H, int Hkv, int Lq, int Lk);
+struct CrossAttnParams {
+  const int32_t* kv_lens;  // [B] or nullptr (all Lk)
+  __nv_bfloat16* out;      // element (b, h, t, d) at out + b*o_sB + h*o_sH + t*o_sT + d
+  int64_t o_sB, o_sH, o_sT;
+  float* lse;              // [B*H, lse_ld] base-2 log-sum-exp (+inf: padding, rows without keys), or nullptr
+  float* part_o;           // nsplit > 1: [nsplit, B*H, Lq, 128] and [nsplit, B*H, Lq]
+  float* part_lse;
+  int64_t items;           // nqp * nsplit * B * Hgrid
+  int B, H, Hkv, G, Lq, Lk;
+  int Hgrid;               // Hkv when packed, else H
+  int pack, nqt, nqp, nsplit, lse_ld;
+  uint32_t q_bytes;        // bytes of one Q tile load
+  float qk_scale;          // D^-1/2 * log2(e)
+};
+int launch_cross_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CrossAttnParams& p,
+                      cudaStream_t s);
+
+// cross_attn_bwd.cu -------------------------------------------------------
+struct CrossBwdParams {
+  const int32_t* kv_lens;
+  const float* lse;    // [B*H, Lpad]
+  const float* delta;  // [B*H, Lpad]
+  __nv_bfloat16* dq;
+  __nv_bfloat16* dk;
+  __nv_bfloat16* dv;
+  int64_t dq_sB, dq_sH, dq_sT, dkv_sB, dkv_sH, dkv_sT;
+  float* part;         // nsplit > 1: [2 (dv, dk), nsplit, B*Hkv, 128 * NKT, 128]
+  int B, H, Hkv, G, Lq, Lk, Lpad, NQT, NKT, nsplit;
+  float qk_scale;
+};
+int cross_bwd_splits(int B, int H, int Hkv, int Lq, int Lk);
+int launch_cross_attn_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
+                          const CrossBwdParams& p, cudaStream_t s);
+
 }  // namespace rola

@@ -5,9 +5,14 @@
 #include "select.cu"
 #include "lowrank.cu"
 #include "gemm.cu"
+#include "norm.cu"
+#include "gemm_block.cu"
 #include "attn.cu"
 #include "attn_bwd.cu"
+#include "cross_attn.cu"
+#include "cross_attn_bwd.cu"
 #include "capi.cu"
+#include "capi_cross.cu"
 #include "peer.cu"
 #include "pipeline.cu"
 #include "noalloc.cu"

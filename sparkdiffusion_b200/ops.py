@@ -688,3 +688,315 @@ def sparse_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
               _ptr(lse), B, L, H, blk, topk, _ptr(dq), _ptr(dk), _ptr(dv), *dq.stride()[:3], _ptr(ws), ws_bytes,
               _stream())
     return dq, dk, dv
+
+
+# ---------------------------------------------------------------------------
+# cross-attention sublayer: norm with the residual's addition, block-scaled e4m3
+# product, attention to an encoder's states
+# ---------------------------------------------------------------------------
+SCALE_BLOCK = 128  # values that share a scale
+E4M3 = torch.float8_e4m3fn
+
+
+def _one_device(what: str, *ts: torch.Tensor | None) -> torch.device:
+    """The CUDA device all of ``ts`` live on (the launch goes to it, on its current stream)."""
+    dev = None
+    for t in ts:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{what}: CUDA tensors required (no CPU fallback)")
+        if dev is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+        dev = t.device
+    return dev
+
+
+def _call_on(dev: torch.device, name: str, *args) -> None:
+    """``_lib.call`` on ``dev`` with its current stream as the last argument."""
+    with torch.cuda.device(dev):
+        _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _rows(t: torch.Tensor, K: int, what: str, dtypes=(BF16, torch.float32)) -> tuple[torch.Tensor, int]:
+    """``t [..., K]`` as ``([M, K]`` with unit column stride and 16-byte rows, its row stride)``; copies what is not."""
+    if t.dtype not in dtypes:
+        raise ValueError(f"{what}: {' or '.join(str(d) for d in dtypes)} required, got {t.dtype}")
+    if t.dim() < 1 or t.shape[-1] != K:
+        raise ValueError(f"{what}: last dimension must be {K}, got shape {tuple(t.shape)}")
+    t2 = t.reshape(-1, K)
+    el = t.element_size()
+    if (t2.stride(1) != 1 or t2.data_ptr() % 16 or (t2.shape[0] > 1 and (t2.stride(0) < K or t2.stride(0) * el % 16))):
+        t2 = t2.clone(memory_format=torch.contiguous_format)
+    return t2, (t2.stride(0) if t2.shape[0] > 1 else K)
+
+
+def _fp32(t: torch.Tensor | None) -> int:
+    return int(t is not None and t.dtype == torch.float32)
+
+
+def _norm_args(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None, what: str):
+    dev = _one_device(what, x, weight, residual)
+    if x.dim() < 1:
+        raise ValueError(f"{what}: x must have a last dimension")
+    K = x.shape[-1]
+    if K == 0 or K % 8 or K > 16384:
+        raise ValueError(f"{what}: the last dimension must be a multiple of 8, at most 16384, got {K}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"{what}: residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
+    x2, x_ld = _rows(x, K, f"{what}: x")
+    r2, r_ld = (None, 0) if residual is None else _rows(residual, K, f"{what}: residual")
+    if weight.numel() != K or weight.dtype not in (BF16, torch.float32):
+        raise ValueError(f"{what}: weight must have {K} bf16 or fp32 elements")
+    w = weight.reshape(-1).contiguous()
+    if w.data_ptr() % 16:
+        w = w.clone()
+    h = None if residual is None else torch.empty(x.shape, device=dev, dtype=residual.dtype)
+    head = (_ptr(x2), _fp32(x2), x_ld, _ptr(r2), _fp32(r2), r_ld, _ptr(w), _fp32(w), x2.shape[0], K)
+    return dev, head, (x2, r2, w), h
+
+
+def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
+                 rstd: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(y, h)``: ``h = x + residual`` (in the residual's type; ``x`` itself
+    without one) and ``y = h * rsqrt(mean(h^2) + eps) * weight`` over the last
+    dimension, rounded once to bf16.  ``x`` and ``residual`` are bf16 or fp32 of
+    one shape, ``weight`` bf16 or fp32.  ``rstd`` (fp32, one per row) receives
+    the row factors.  Beside ``train.rms_norm``; differentiable as
+    ``train.add_rms_norm``."""
+    dev, head, keep, h = _norm_args(x, weight, residual, "add_rms_norm")
+    y = torch.empty(x.shape, device=dev, dtype=BF16)
+    M = head[8]
+    if rstd is not None and (rstd.device != dev or rstd.dtype != torch.float32 or rstd.numel() != M
+                             or not rstd.is_contiguous()):
+        raise ValueError("add_rms_norm: rstd must be a contiguous fp32 tensor of one value per row")
+    if M:
+        _call_on(dev, "rola_b200_add_rms_norm", *head, eps, _ptr(h), _ptr(y), _ptr(rstd))
+    return y, (x if h is None else h)
+
+
+def _block_scales(M: int, K: int, dev) -> torch.Tensor:
+    """``[M, ceil(K/128)]`` fp32 scales, stored one block's column after the other (what the product reads)."""
+    return torch.empty((K + SCALE_BLOCK - 1) // SCALE_BLOCK, M, device=dev, dtype=torch.float32).t()
+
+
+def add_rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
+                      block: int | None = SCALE_BLOCK) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """``(yq, scale, h)``: ``add_rms_norm`` with ``y ~= yq * scale`` in e4m3,
+    quantised from the unrounded norm.  ``block=128``: one scale per 128 columns,
+    ``scale [..., ceil(K/128)]``, for ``gemm_fp8_block``; ``block=None``: one per
+    row, ``scale [...]``, for ``qkv_gemm_fp8``.  Scales are ``max|y|/448 + 1e-12``."""
+    if block not in (SCALE_BLOCK, None):
+        raise ValueError("add_rms_norm_e4m3: block must be 128, or None for one scale per row")
+    dev, head, keep, h = _norm_args(x, weight, residual, "add_rms_norm_e4m3")
+    M, K = head[8], head[9]
+    yq = torch.empty(x.shape, device=dev, dtype=E4M3)
+    scale = torch.empty(M, device=dev, dtype=torch.float32) if block is None else _block_scales(M, K, dev)
+    sM, sK = (1, 0) if block is None else scale.stride()
+    if M:
+        _call_on(dev, "rola_b200_add_rms_norm_e4m3", *head, eps, _ptr(h), _ptr(yq), _ptr(scale), sM, sK, block or 0)
+    lead = x.shape[:-1]
+    if block is None:
+        scale = scale.view(lead)
+    elif len(lead) != 1:
+        scale = scale.unflatten(0, lead) if lead else scale[0]
+    return yq, scale, (x if h is None else h)
+
+
+def add_rms_norm_bwd(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, dy: torch.Tensor,
+                     dh: torch.Tensor | None, x_dtype: torch.dtype, res_dtype: torch.dtype | None,
+                     need_dw: bool = True) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """Gradients ``(dx, dresidual, dweight)`` of ``add_rms_norm`` from its ``h``
+    and row factors: ``dy`` is the gradient of y, ``dh`` of h (None: zero).  dx
+    and dresidual share one tensor where their types agree."""
+    what = "add_rms_norm_bwd"
+    dev = _one_device(what, h, weight, rstd, dy, dh)
+    K = h.shape[-1]
+    if dy.shape != h.shape or (dh is not None and dh.shape != h.shape):
+        raise ValueError(f"{what}: dy and dh must have the shape of h")
+    for d in (x_dtype, res_dtype):
+        if d not in (BF16, torch.float32, None):
+            raise ValueError(f"{what}: bf16 or fp32 gradients only")
+    h2, h_ld = _rows(h, K, f"{what}: h")
+    dy2, dy_ld = _rows(dy.to(BF16), K, f"{what}: dy")
+    dh2, dh_ld = (None, 0) if dh is None else _rows(dh, K, f"{what}: dh")
+    M = h2.shape[0]
+    if rstd.dtype != torch.float32 or rstd.numel() != M or not rstd.is_contiguous():
+        raise ValueError(f"{what}: rstd must be add_rms_norm's row factors")
+    if weight.numel() != K or weight.dtype not in (BF16, torch.float32):
+        raise ValueError(f"{what}: weight must have {K} bf16 or fp32 elements")
+    w = weight.reshape(-1).contiguous()
+    if w.data_ptr() % 16:
+        w = w.clone()
+    dx = torch.empty(h.shape, device=dev, dtype=x_dtype)
+    dres = None if res_dtype is None else dx if res_dtype == x_dtype else torch.empty_like(dx, dtype=res_dtype)
+    dw = torch.zeros_like(w) if need_dw and M == 0 else torch.empty_like(w) if need_dw else None
+    if M:
+        nb = _lib.lib().rola_b200_add_rms_norm_bwd_workspace(M, K) if need_dw else 0
+        with torch.cuda.device(dev):
+            ws = torch.empty(nb, device=dev, dtype=torch.uint8) if nb else None
+        _call_on(dev, "rola_b200_add_rms_norm_bwd", _ptr(h2), _fp32(h2), h_ld, _ptr(w), _fp32(w), _ptr(rstd),
+                 _ptr(dy2), dy_ld, _ptr(dh2), _fp32(dh2), dh_ld, M, K, _ptr(dx), _fp32(dx),
+                 _ptr(None if dres is dx else dres), _fp32(dres), _ptr(dw), _ptr(ws), nb)
+    return dx, dres, None if dw is None else dw.view(weight.shape)
+
+
+def quantize_blocks_e4m3(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Activations ``x [M, K]`` (bf16 or fp32) -> ``(xq float8_e4m3fn [M, K],
+    scale fp32 [M, ceil(K/128)])``, one scale per row and 128 columns: the
+    operand of ``gemm_fp8_block`` where no norm precedes the product."""
+    what = "quantize_blocks_e4m3"
+    dev = _one_device(what, x)
+    if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] % 8 or x.shape[1] > 16384:
+        raise ValueError(f"{what}: [M, K] with K a multiple of 8, at most 16384, required")
+    M, K = x.shape
+    x2, ld = _rows(x, K, f"{what}: x")
+    xq = torch.empty(M, K, device=dev, dtype=E4M3)
+    scale = _block_scales(M, K, dev)
+    if M:
+        _call_on(dev, "rola_b200_quantize_blocks_e4m3", _ptr(x2), _fp32(x2), ld, M, K, _ptr(xq), _ptr(scale),
+                 *scale.stride())
+    return xq, scale
+
+
+def quantize_tiles_e4m3(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Weight ``w [N, K]`` (bf16 or fp32) -> ``(wq float8_e4m3fn [N, K], scale
+    fp32 [ceil(N/128), ceil(K/128)])``, one scale per 128 x 128 block; done once
+    per weight."""
+    what = "quantize_tiles_e4m3"
+    dev = _one_device(what, w)
+    if w.dim() != 2 or w.shape[1] == 0 or w.shape[1] % 8 or max(w.shape) > 65536 or w.shape[0] == 0:
+        raise ValueError(f"{what}: [N, K] with K a multiple of 8, both at most 65536, required")
+    N, K = w.shape
+    w2, ld = _rows(w, K, f"{what}: w")
+    wq = torch.empty(N, K, device=dev, dtype=E4M3)
+    scale = torch.empty((N + 127) // 128, (K + 127) // 128, device=dev, dtype=torch.float32)
+    _call_on(dev, "rola_b200_quantize_tiles_e4m3", _ptr(w2), _fp32(w2), ld, N, K, _ptr(wq), _ptr(scale))
+    return wq, scale
+
+
+def gemm_fp8_block(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
+                   bias: torch.Tensor | None = None) -> torch.Tensor:
+    """``out [M, N] = bf16(sum over blocks of 128 columns of x_scale[m, kb] *
+    w_scale[n // 128, kb] * (xq . wq^T) + bias)`` on e4m3 operands ``xq [M, K]``,
+    ``wq [N, K]`` (``add_rms_norm_e4m3`` or ``quantize_blocks_e4m3``, and
+    ``quantize_tiles_e4m3``), fp32 sums.  Beside ``qkv_gemm_fp8``, whose scales
+    are one per row.  N % 8 == 0, K % 16 == 0."""
+    what = "gemm_fp8_block"
+    dev = _one_device(what, xq, x_scale, wq, w_scale, bias)
+    if xq.dtype != E4M3 or wq.dtype != E4M3:
+        raise ValueError(f"{what}: float8_e4m3fn operands required")
+    if xq.dim() != 2 or wq.dim() != 2 or xq.shape[1] != wq.shape[1]:
+        raise ValueError(f"{what}: weight {tuple(wq.shape)} does not match x {tuple(xq.shape)}")
+    (M, K), N = xq.shape, wq.shape[0]
+    nk = (K + SCALE_BLOCK - 1) // SCALE_BLOCK
+    if K == 0 or N == 0 or K % 16 or N % 8 or max(N, K) > 65536:
+        raise ValueError(f"{what}: K must be a multiple of 16 and N of 8, both at most 65536, got K={K}, N={N}")
+    if x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (M, nk):
+        raise ValueError(f"{what}: x_scale must be fp32 {(M, nk)}, got {tuple(x_scale.shape)}")
+    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != ((N + 127) // 128, nk):
+        raise ValueError(f"{what}: w_scale must be fp32 {((N + 127) // 128, nk)}, got {tuple(w_scale.shape)}")
+    if bias is not None and bias.numel() != N:
+        raise ValueError(f"{what}: bias must have {N} elements")
+    b = None if bias is None else bias.reshape(-1).to(BF16).contiguous()
+    xq, wq, b = (t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0)
+                 else t.clone(memory_format=torch.contiguous_format) for t in (xq, wq, b))
+    w_scale = w_scale.contiguous()
+    out = torch.empty(M, N, device=dev, dtype=BF16)
+    if M:
+        _call_on(dev, "rola_b200_gemm_fp8_block", _ptr(xq), _ptr(x_scale), *x_scale.stride(), _ptr(wq), _ptr(w_scale),
+                 _ptr(b), _ptr(out), M, N, K)
+    return out
+
+
+def _head_view(t: torch.Tensor) -> torch.Tensor:
+    """``t [B, H, L, 128]`` as the kernels can map it: unit last stride, positive
+    strides of 16-byte multiples, 16-byte base (a broadcast or unaligned view is copied)."""
+    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(
+            n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride()[:3])):
+        return t
+    return _token_major(t)
+
+
+def _head_strides(t: torch.Tensor) -> tuple[int, int, int]:
+    """(b, h, t) strides; those of dimensions of size 1 carry no meaning and get one the maps accept."""
+    return tuple(s if n > 1 else max(HEAD_DIM, 8 * (abs(s) // 8)) for n, s in zip(t.shape[:3], t.stride()[:3]))
+
+
+def _cross_args(what: str, q, k, v, kv_lens):
+    dev = _one_device(what, q, k, v, kv_lens)
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        if t.dtype != BF16:
+            raise ValueError(f"{what}: bf16 {n} required, got {t.dtype}")
+        if t.dim() != 4 or t.shape[3] != HEAD_DIM:
+            raise ValueError(f"{what}: {n} must be [B, H, L, 128], got {tuple(t.shape)}")
+    B, H, Lq, _ = q.shape
+    Hkv, Lk = k.shape[1], k.shape[2]
+    if v.shape != k.shape or k.shape[0] != B:
+        raise ValueError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} must share a shape with q's batch {B}")
+    if Hkv == 0 or H % Hkv:
+        raise ValueError(f"{what}: {H} query heads are not a multiple of {Hkv} key heads")
+    if kv_lens is not None and (kv_lens.dtype != torch.int32 or tuple(kv_lens.shape) != (B,)):
+        raise ValueError(f"{what}: kv_lens must be int32 [{B}]")
+    return dev, (B, H, Hkv, Lq, Lk), None if kv_lens is None else kv_lens.contiguous()
+
+
+def cross_attention_fwd_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: torch.Tensor | None = None,
+                            need_lse: bool = True) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """``cross_attention`` and the rows' base-2 log-sum-exp ``[B*H, lse_rows(Lq)]``
+    (fp32; +inf on padding rows and rows without keys), which
+    ``cross_attention_bwd`` reads."""
+    what = "cross_attention"
+    dev, (B, H, Hkv, Lq, Lk), lens = _cross_args(what, q, k, v, kv_lens)
+    o = torch.empty(B, Lq, H, HEAD_DIM, device=dev, dtype=BF16).transpose(1, 2)
+    lse = torch.empty(B * H, lse_rows(Lq), device=dev, dtype=torch.float32) if need_lse else None
+    if o.numel() == 0:
+        return o, lse
+    if Lk == 0:
+        return o.zero_(), None if lse is None else lse.fill_(float("inf"))
+    q, k, v = _head_view(q), _head_view(k), _head_view(v)
+    nb = _lib.lib().rola_b200_cross_attn_workspace(B, H, Hkv, Lq, Lk)
+    ws = torch.empty(nb, device=dev, dtype=torch.uint8) if nb else None
+    _call_on(dev, "rola_b200_cross_attn", _ptr(q), *_head_strides(q), _ptr(k), *_head_strides(k), _ptr(v),
+             *_head_strides(v), _ptr(lens), B, H, Hkv, Lq, Lk, _ptr(o), *_head_strides(o), _ptr(lse), _ptr(ws), nb)
+    return o, lse
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                    kv_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """Softmax attention of ``q [B, H, Lq, 128]`` to the states ``k, v [B, Hkv,
+    Lk, 128]`` of another sequence (bf16, any head view) -> ``o [B, H, Lq, 128]``,
+    a view of a token-major tensor.  Query head ``h`` reads key head ``h // (H //
+    Hkv)``.  ``kv_lens`` (int32 ``[B]`` on the device, clamped to ``[0, Lk]``):
+    only the first ``kv_lens[b]`` states count, whatever the others hold; a row
+    without states is 0.  Lq may be 1 (the keys are then cut over the SMs).
+    Beside ``dense_attention``, which takes one length."""
+    return cross_attention_fwd_lse(q, k, v, kv_lens, need_lse=False)[0]
+
+
+def cross_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: torch.Tensor, do: torch.Tensor,
+                        lse: torch.Tensor, kv_lens: torch.Tensor | None = None
+                        ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Gradients ``(dq, dk, dv)`` (bf16) of ``cross_attention`` given its ``o``,
+    ``lse`` and ``do = dL/do``; dk and dv sum over the query heads of a key head.
+    The same inputs give the same bits."""
+    what = "cross_attention_bwd"
+    dev, (B, H, Hkv, Lq, Lk), lens = _cross_args(what, q, k, v, kv_lens)
+    _one_device(what, q, o, do, lse)
+    if o.shape != q.shape or do.shape != q.shape or o.dtype != BF16:
+        raise ValueError(f"{what}: o and do must have q's shape, o in bf16")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (B * H, lse_rows(Lq)) or not lse.is_contiguous():
+        raise ValueError(f"{what}: lse must be the forward's")
+    dq = torch.empty(B, Lq, H, HEAD_DIM, device=dev, dtype=BF16).transpose(1, 2)
+    dk, dv = torch.empty(2, B, Lk, Hkv, HEAD_DIM, device=dev, dtype=BF16).transpose(2, 3)
+    if q.numel() == 0 or k.numel() == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    q, k, v, o, do = (_head_view(t) for t in (q, k, v, o, do.to(BF16)))
+    nb = _lib.lib().rola_b200_cross_attn_bwd_workspace(B, H, Hkv, Lq, Lk)
+    if nb == 0:
+        raise ValueError(f"{what}: bad sizes")
+    ws = torch.empty(nb, device=dev, dtype=torch.uint8)
+    _call_on(dev, "rola_b200_cross_attn_bwd", _ptr(q), *_head_strides(q), _ptr(k), *_head_strides(k), _ptr(v),
+             *_head_strides(v), _ptr(o), *_head_strides(o), _ptr(do), *_head_strides(do), _ptr(lens), _ptr(lse), B, H,
+             Hkv, Lq, Lk, _ptr(dq), *_head_strides(dq), _ptr(dk), _ptr(dv), *_head_strides(dk), _ptr(ws), nb)
+    return dq, dk, dv

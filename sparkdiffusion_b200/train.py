@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import _lib, ops
 
@@ -177,3 +178,62 @@ def dense_training_forward(layer, x: torch.Tensor, freqs: torch.Tensor) -> torch
     v = layer.v(x).view(b, s, n, d)
     o = dense_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
     return layer.o(o.transpose(1, 2).reshape(b, s, n * d))
+
+
+class AddRMSNorm(torch.autograd.Function):
+    """``ops.add_rms_norm`` with its backward kernel; saves h and the row factors."""
+
+    @staticmethod
+    def forward(ctx, x, weight, eps: float, residual):
+        rstd = torch.empty(x.numel() // max(1, x.shape[-1]), device=x.device, dtype=torch.float32)
+        y, h = ops.add_rms_norm(x, weight, eps, residual, rstd=rstd)
+        ctx.save_for_backward(h, weight, rstd)
+        ctx.x_dtype, ctx.res_dtype = x.dtype, None if residual is None else residual.dtype
+        ctx.set_materialize_grads(False)
+        return (y, h) if residual is not None else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        if dy is None:
+            dy = torch.zeros(h.shape, device=h.device, dtype=torch.bfloat16)
+        dx, dres, dw = ops.add_rms_norm_bwd(h, weight, rstd, dy, dh, ctx.x_dtype, ctx.res_dtype,
+                                            need_dw=ctx.needs_input_grad[1])
+        return dx, dw, None, dres
+
+
+def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None):
+    """Differentiable ``ops.add_rms_norm``: ``(y, h)``, gradients to ``x``,
+    ``residual`` and ``weight``, one kernel each way."""
+    if not x.is_cuda:
+        raise RuntimeError("the B200 training path runs on CUDA tensors only")
+    out = AddRMSNorm.apply(x, weight, eps, residual)
+    return out if residual is not None else (out, x)
+
+
+class CrossAttention(torch.autograd.Function):
+    """``ops.cross_attention`` with its backward kernels."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, kv_lens):
+        o, lse = ops.cross_attention_fwd_lse(q, k, v, kv_lens)
+        ctx.save_for_backward(q, k, v, o, lse, kv_lens)
+        return o
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, do):
+        q, k, v, o, lse, kv_lens = ctx.saved_tensors
+        return (*ops.cross_attention_bwd(q, k, v, o, do, lse, kv_lens), None)
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                    kv_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """Differentiable attention of ``q [B, H, Lq, 128]`` to the states ``k, v
+    [B, Hkv, Lk, 128]`` (``ops.cross_attention``), in the input dtype; beside
+    ``dense_attention``, which takes one length."""
+    if not q.is_cuda:
+        raise RuntimeError("the B200 training path runs on CUDA tensors only")
+    dt = q.dtype
+    return CrossAttention.apply(*(t.to(torch.bfloat16) for t in (q, k, v)), kv_lens).to(dt)
