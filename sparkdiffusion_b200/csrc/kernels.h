@@ -187,7 +187,7 @@ struct AddRmsNormParams {
   float* scale;     // (m, block) at m * scale_sM + block * scale_sK; scale_row: [M]
   float* rstd;      // [M] or nullptr
   int64_t x_ld, res_ld, M, scale_sM, scale_sK;
-  int K;
+  int K, ring;      // ring: rows on their way per CTA (set by the launch)
   bool x_fp32, res_fp32, w_fp32, scale_row;
   bool norm;        // false: quantise x as it is
   float eps;
@@ -204,7 +204,7 @@ struct AddRmsNormBwdParams {
   float* dw_part;     // [add_rms_norm_bwd_parts, K] or nullptr (no dw)
   void* dw;           // [K] in w's type
   int64_t h_ld, dy_ld, dh_ld, M;
-  int K;
+  int K, ring;
   bool h_fp32, w_fp32, dh_fp32, dx_fp32, dres_fp32;
 };
 int add_rms_norm_bwd_parts(int64_t M, int K);  // rows of dw_part

@@ -24,6 +24,8 @@ namespace rola {
 namespace norm {
 constexpr int kQBlock = 128;     // columns that share a scale
 constexpr float kE4M3Max = 448.f;
+constexpr int kRing = 3, kRingBwd = 2;  // rows on their way per CTA, where shared memory holds them
+constexpr size_t kRingBytes = 220 * 1024;
 }  // namespace norm
 
 // 8 consecutive columns as fp32
@@ -93,97 +95,161 @@ __device__ __forceinline__ float row_reduce(float v, float* slot, Op op, float z
 
 enum : int { kOutBf16 = 0, kOutE4M3Block = 1, kOutE4M3Row = 2 };
 
-template <int NV, bool kWarpRow, int kOut>
-__global__ void __launch_bounds__(kWarpRow ? 128 : 512) add_rms_norm_kernel(const AddRmsNormParams p) {
-  __shared__ float s_red[2][2][32];
+// Everything after a row's loads: v holds x (and r the residual's values) of
+// NV vectors, 0 past the row.  `slots`: two arrays for this row's reductions;
+// `rows_read` runs once every thread of the row has its values in registers.
+template <int NV, bool kWarpRow, int kOut, typename Read>
+__device__ __forceinline__ void norm_row(const AddRmsNormParams& p, int64_t m, float (&v)[NV][8], float (*slots)[32],
+                                         Read rows_read) {
   const int lane_in_row = kWarpRow ? (threadIdx.x & 31) : threadIdx.x;
   const int row_threads = kWarpRow ? 32 : blockDim.x;
-  const int rows_per_cta = kWarpRow ? (blockDim.x >> 5) : 1;
-  const int64_t first = (int64_t)blockIdx.x * rows_per_cta + (kWarpRow ? (threadIdx.x >> 5) : 0);
-  const int64_t step = (int64_t)gridDim.x * rows_per_cta;
   const int nvec = p.K >> 3;
-  const float inv_k = 1.0f / (float)p.K;
-  int parity = 0;
-  for (int64_t m = first; m < p.M; m += step, parity ^= 1) {
-    float v[NV][8];
+  if (p.norm) {
     float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(v[i][e], v[i][e], ss);
+    ss = row_reduce<kWarpRow>(ss, slots[0], AddOp(), 0.f);
+    rows_read();
+    const float r = rsqrtf(ss * (1.0f / (float)p.K) + p.eps);
+    if (p.rstd && lane_in_row == 0) p.rstd[m] = r;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int c = lane_in_row + i * row_threads;
+      if (c < nvec) {
+        float w[8];
+        load8(p.w, p.w_fp32, 8 * c, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * r * w[e];
+      }
+    }
+  } else {
+    if (!kWarpRow) __syncthreads();
+    rows_read();
+  }
+  if (kOut == kOutBf16) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = lane_in_row + i * row_threads;
+      if (c < nvec) store8(p.y, false, m * p.K + 8 * c, v[i]);
+    }
+  } else {
+    float amax[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      amax[i] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax[i] = max_nan(amax[i], fabsf(v[i][e]));
+    }
+    if (kOut == kOutE4M3Row) {
+      float a = 0.f;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) a = max_nan(a, amax[i]);
+      a = row_reduce<kWarpRow>(a, slots[1], MaxOp(), 0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) amax[i] = a;
+    } else {
+      // 16 neighbouring threads hold the 128 columns of a scale
+#pragma unroll
+      for (int i = 0; i < NV; ++i) amax[i] = lanes_reduce<16>(amax[i], MaxOp());
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = lane_in_row + i * row_threads;
+      if (c < nvec) {
+        const float s = e4m3_scale(amax[i]);
+        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.yq) + m * p.K + 8 * c) = pack8_e4m3(v[i], 1.0f / s);
+        if (kOut == kOutE4M3Row) {
+          if (c == 0) p.scale[m] = s;
+        } else if ((c & 15) == 0) {
+          p.scale[m * p.scale_sM + (c >> 4) * p.scale_sK] = s;
+        }
+      }
+    }
+  }
+}
+
+// v (x) += residual in the stream's type, stored as h
+__device__ __forceinline__ void add_residual(const AddRmsNormParams& p, int64_t m, int c, const void* res, int64_t off,
+                                             float (&v)[8]) {
+  float r[8];
+  load8(res, p.res_fp32, off, r);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] += r[e];
+  if (!p.res_fp32) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) rbf2(v[e], v[e + 1]);
+  }
+  store8(p.h, p.res_fp32, m * p.K + 8 * c, v);
+}
+
+// rows of up to 1024 columns: one warp each
+template <int NV, int kOut>
+__global__ void __launch_bounds__(128) add_rms_norm_warp_kernel(const AddRmsNormParams p) {
+  const int lane = threadIdx.x & 31, nvec = p.K >> 3;
+  const int64_t step = (int64_t)gridDim.x * 4;
+  for (int64_t m = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); m < p.M; m += step) {
+    float v[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int c = lane + i * 32;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
       if (c < nvec) {
         load8(p.x, p.x_fp32, m * p.x_ld + 8 * c, v[i]);
-        if (p.res) {
-          float r[8];
-          load8(p.res, p.res_fp32, m * p.res_ld + 8 * c, r);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[i][e] += r[e];
-          if (!p.res_fp32) {
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) rbf2(v[i][e], v[i][e + 1]);
-          }
-          store8(p.h, p.res_fp32, m * p.K + 8 * c, v[i]);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(v[i][e], v[i][e], ss);
+        if (p.res) add_residual(p, m, c, p.res, m * p.res_ld + 8 * c, v[i]);
       }
     }
-    if (p.norm) {
-      ss = row_reduce<kWarpRow>(ss, s_red[parity][0], AddOp(), 0.f);
-      const float r = rsqrtf(ss * inv_k + p.eps);
-      if (p.rstd && lane_in_row == 0) p.rstd[m] = r;
+    norm_row<NV, true, kOut>(p, m, v, nullptr, [] {});
+  }
+}
+
+// Longer rows: a CTA each, the next rows on their way.  Thread 0 fetches whole
+// rows of x and res by bulk copies into a ring of kRing shared-memory stages (fewer where rows are too long);
+// the barrier of the row's reduction also says that its stage is free.
+template <int NV, int kOut>
+__global__ void __launch_bounds__(512) add_rms_norm_ring_kernel(const AddRmsNormParams p) {
+  extern __shared__ __align__(128) uint8_t smem_ring[];
+  __shared__ float s_red[2][2][32];
+  __shared__ uint64_t s_bar[norm::kRing];
+  const int nvec = p.K >> 3;
+  const uint32_t xb = (uint32_t)p.K * (p.x_fp32 ? 4 : 2), rb = p.res ? (uint32_t)p.K * (p.res_fp32 ? 4 : 2) : 0u;
+  const uint32_t stage = xb + rb;
+  auto fetch = [&](int64_t m, int s) {
+    const uint32_t dst = smem_u32(smem_ring) + s * stage, bar = smem_u32(&s_bar[s]);
+    mbar_expect_tx(bar, stage);
+    bulk_load(dst, static_cast<const uint8_t*>(p.x) + m * p.x_ld * (p.x_fp32 ? 4 : 2), xb, bar);
+    if (rb) bulk_load(dst + xb, static_cast<const uint8_t*>(p.res) + m * p.res_ld * (p.res_fp32 ? 4 : 2), rb, bar);
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.ring; ++s) mbar_init(smem_u32(&s_bar[s]), 1);
+    fence_barrier_init();
+    for (int s = 0; s < p.ring; ++s)
+      if (blockIdx.x + (int64_t)s * gridDim.x < p.M) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
+  }
+  __syncthreads();
+  int n = 0;
+  bool ok = true;
+  for (int64_t m = blockIdx.x; m < p.M; m += gridDim.x, ++n) {
+    const int s = n % p.ring;
+    if (ok) ok = mbar_wait_until(smem_u32(&s_bar[s]), (n / p.ring) & 1, globaltimer_ns() + kWaitLimitNs);
+    const uint8_t* xs = smem_ring + s * stage;
+    float v[NV][8];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = lane_in_row + i * row_threads;
-        if (c < nvec) {
-          float w[8];
-          load8(p.w, p.w_fp32, 8 * c, w);
+    for (int i = 0; i < NV; ++i) {
+      const int c = threadIdx.x + i * blockDim.x;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * r * w[e];
-        }
+      for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+      if (c < nvec) {
+        load8(xs, p.x_fp32, 8 * c, v[i]);
+        if (rb) add_residual(p, m, c, xs + xb, 8 * c, v[i]);
       }
     }
-    if (kOut == kOutBf16) {
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = lane_in_row + i * row_threads;
-        if (c < nvec) store8(p.y, false, m * p.K + 8 * c, v[i]);
-      }
-    } else {
-      float amax[NV];
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        amax[i] = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) amax[i] = max_nan(amax[i], fabsf(v[i][e]));
-      }
-      if (kOut == kOutE4M3Row) {
-        float a = 0.f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) a = max_nan(a, amax[i]);
-        a = row_reduce<kWarpRow>(a, s_red[parity][1], MaxOp(), 0.f);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) amax[i] = a;
-      } else {
-        // 16 neighbouring threads hold the 128 columns of a scale
-#pragma unroll
-        for (int i = 0; i < NV; ++i) amax[i] = lanes_reduce<16>(amax[i], MaxOp());
-      }
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int c = lane_in_row + i * row_threads;
-        if (c < nvec) {
-          const float s = e4m3_scale(amax[i]);
-          *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.yq) + m * p.K + 8 * c) = pack8_e4m3(v[i], 1.0f / s);
-          if (kOut == kOutE4M3Row) {
-            if (c == 0) p.scale[m] = s;
-          } else if ((c & 15) == 0) {
-            p.scale[m * p.scale_sM + (c >> 4) * p.scale_sK] = s;
-          }
-        }
-      }
-    }
+    norm_row<NV, false, kOut>(p, m, v, s_red[n & 1], [&] {
+      const int64_t next = m + (int64_t)p.ring * gridDim.x;
+      if (threadIdx.x == 0 && next < p.M) fetch(next, s);
+    });
   }
 }
 
@@ -192,70 +258,105 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : 512) add_rms_norm_kernel(cons
 //   dw = sum_m dy u: every CTA sums its own rows in registers (fixed order) and
 //   leaves one fp32 row of partials; dw_reduce_kernel adds them in order, so the
 //   result does not depend on timing.
-template <int NV, bool kWarpRow>
-__global__ void __launch_bounds__(kWarpRow ? 128 : 512) add_rms_norm_bwd_kernel(const AddRmsNormBwdParams p) {
-  __shared__ float s_red[2][32];
+template <int NV, bool kWarpRow, typename Read>
+__device__ __forceinline__ void norm_bwd_row(const AddRmsNormBwdParams& p, int64_t m, const void* h, int64_t h_off,
+                                             const void* dy, int64_t dy_off, const void* dh, int64_t dh_off,
+                                             float (&dw)[NV][8], float* slot, Read rows_read) {
   const int lane_in_row = kWarpRow ? (threadIdx.x & 31) : threadIdx.x;
   const int row_threads = kWarpRow ? 32 : blockDim.x;
-  const int rows_per_cta = kWarpRow ? (blockDim.x >> 5) : 1;
-  const int64_t first = (int64_t)blockIdx.x * rows_per_cta + (kWarpRow ? (threadIdx.x >> 5) : 0);
-  const int64_t step = (int64_t)gridDim.x * rows_per_cta;
   const int nvec = p.K >> 3;
-  const float inv_k = 1.0f / (float)p.K;
-  float dw[NV][8];
+  const float r = p.rstd[m];
+  float u[NV][8], g[NV][8], d[NV][8];
+  float gu = 0.f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
+  for (int i = 0; i < NV; ++i) {
+    const int c = lane_in_row + i * row_threads;
+    if (c < nvec) {
+      float w[8];
+      load8(h, p.h_fp32, h_off + 8 * c, u[i]);
+      load8(dy, false, dy_off + 8 * c, g[i]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) dw[i][e] = 0.f;
-  int parity = 0;
-  for (int64_t m = first; m < p.M; m += step, parity ^= 1) {
-    const float r = p.rstd[m];
-    float u[NV][8], g[NV][8];
-    float gu = 0.f;
+      for (int e = 0; e < 8; ++e) d[i][e] = 0.f;
+      if (dh) load8(dh, p.dh_fp32, dh_off + 8 * c, d[i]);
+      load8(p.w, p.w_fp32, 8 * c, w);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = lane_in_row + i * row_threads;
-      if (c < nvec) {
-        float w[8];
-        load8(p.h, p.h_fp32, m * p.h_ld + 8 * c, u[i]);
-        load8(p.dy, false, m * p.dy_ld + 8 * c, g[i]);
-        load8(p.w, p.w_fp32, 8 * c, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          u[i][e] *= r;
-          dw[i][e] = fmaf(g[i][e], u[i][e], dw[i][e]);
-          g[i][e] *= w[e];
-          gu = fmaf(g[i][e], u[i][e], gu);
-        }
-      }
-    }
-    gu = row_reduce<kWarpRow>(gu, s_red[parity], AddOp(), 0.f) * inv_k;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = lane_in_row + i * row_threads;
-      if (c < nvec) {
-        float d[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) d[e] = r * (g[i][e] - u[i][e] * gu);
-        if (p.dh) {
-          float in[8];
-          load8(p.dh, p.dh_fp32, m * p.dh_ld + 8 * c, in);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) d[e] += in[e];
-        }
-        store8(p.dx, p.dx_fp32, m * p.K + 8 * c, d);
-        if (p.dres) store8(p.dres, p.dres_fp32, m * p.K + 8 * c, d);
+      for (int e = 0; e < 8; ++e) {
+        u[i][e] *= r;
+        dw[i][e] = fmaf(g[i][e], u[i][e], dw[i][e]);
+        g[i][e] *= w[e];
+        gu = fmaf(g[i][e], u[i][e], gu);
       }
     }
   }
-  if (p.dw_part) {
-    const int64_t prow = kWarpRow ? first : (int64_t)blockIdx.x;  // one row of partials per warp or CTA
+  gu = row_reduce<kWarpRow>(gu, slot, AddOp(), 0.f) * (1.0f / (float)p.K);
+  rows_read();
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int c = lane_in_row + i * row_threads;
-      if (c < nvec) store8(p.dw_part, true, prow * p.K + 8 * c, dw[i]);
+  for (int i = 0; i < NV; ++i) {
+    const int c = lane_in_row + i * row_threads;
+    if (c < nvec) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) d[i][e] = fmaf(r, g[i][e] - u[i][e] * gu, d[i][e]);
+      store8(p.dx, p.dx_fp32, m * p.K + 8 * c, d[i]);
+      if (p.dres) store8(p.dres, p.dres_fp32, m * p.K + 8 * c, d[i]);
     }
   }
+}
+
+template <int NV>
+__device__ __forceinline__ void store_dw_part(const AddRmsNormBwdParams& p, int64_t prow, int lane_in_row,
+                                              int row_threads, const float (&dw)[NV][8]) {
+  if (p.dw_part == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int c = lane_in_row + i * row_threads;
+    if (c < (p.K >> 3)) store8(p.dw_part, true, prow * p.K + 8 * c, dw[i]);
+  }
+}
+
+template <int NV>
+__global__ void __launch_bounds__(128) add_rms_norm_bwd_warp_kernel(const AddRmsNormBwdParams p) {
+  const int64_t first = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5), step = (int64_t)gridDim.x * 4;
+  float dw[NV][8] = {};
+  for (int64_t m = first; m < p.M; m += step)
+    norm_bwd_row<NV, true>(p, m, p.h, m * p.h_ld, p.dy, m * p.dy_ld, p.dh, m * p.dh_ld, dw, nullptr, [] {});
+  store_dw_part<NV>(p, first, threadIdx.x & 31, 32, dw);  // one row of partials per warp
+}
+
+// rows h, dy and dh through a ring, as add_rms_norm_ring_kernel
+template <int NV>
+__global__ void __launch_bounds__(512) add_rms_norm_bwd_ring_kernel(const AddRmsNormBwdParams p) {
+  extern __shared__ __align__(128) uint8_t smem_ring[];
+  __shared__ float s_red[2][32];
+  __shared__ uint64_t s_bar[norm::kRingBwd];
+  const uint32_t hb = (uint32_t)p.K * (p.h_fp32 ? 4 : 2), yb = (uint32_t)p.K * 2;
+  const uint32_t db = p.dh ? (uint32_t)p.K * (p.dh_fp32 ? 4 : 2) : 0u, stage = hb + yb + db;
+  auto fetch = [&](int64_t m, int s) {
+    const uint32_t dst = smem_u32(smem_ring) + s * stage, bar = smem_u32(&s_bar[s]);
+    mbar_expect_tx(bar, stage);
+    bulk_load(dst, static_cast<const uint8_t*>(p.h) + m * p.h_ld * (p.h_fp32 ? 4 : 2), hb, bar);
+    bulk_load(dst + hb, static_cast<const uint8_t*>(p.dy) + m * p.dy_ld * 2, yb, bar);
+    if (db) bulk_load(dst + hb + yb, static_cast<const uint8_t*>(p.dh) + m * p.dh_ld * (p.dh_fp32 ? 4 : 2), db, bar);
+  };
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.ring; ++s) mbar_init(smem_u32(&s_bar[s]), 1);
+    fence_barrier_init();
+    for (int s = 0; s < p.ring; ++s)
+      if (blockIdx.x + (int64_t)s * gridDim.x < p.M) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
+  }
+  __syncthreads();
+  float dw[NV][8] = {};
+  int n = 0;
+  bool ok = true;
+  for (int64_t m = blockIdx.x; m < p.M; m += gridDim.x, ++n) {
+    const int s = n % p.ring;
+    if (ok) ok = mbar_wait_until(smem_u32(&s_bar[s]), (n / p.ring) & 1, globaltimer_ns() + kWaitLimitNs);
+    const uint8_t* hs = smem_ring + s * stage;
+    norm_bwd_row<NV, false>(p, m, hs, 0, hs + hb, 0, db ? hs + hb + yb : nullptr, 0, dw, s_red[n & 1], [&] {
+      const int64_t next = m + (int64_t)p.ring * gridDim.x;
+      if (threadIdx.x == 0 && next < p.M) fetch(next, s);
+    });
+  }
+  store_dw_part<NV>(p, blockIdx.x, threadIdx.x, blockDim.x, dw);
 }
 
 // dw[k] = sum_g part[g, k] in order of g: 8 warps take every 8th row of 32 columns, then add up
@@ -322,7 +423,7 @@ struct NormShape {
 static NormShape norm_shape(int K) {
   const int nvec = K / 8;
   if (nvec <= 128) return {nvec <= 32 ? 1 : nvec <= 64 ? 2 : 4, 128, true};
-  const int nv = nvec <= 512 ? 2 : 4;
+  const int nv = nvec <= 1024 ? 2 : 4;
   return {nv, ((nvec + nv - 1) / nv + 31) / 32 * 32, false};
 }
 
@@ -334,51 +435,91 @@ static int device_sms() {
   return sms;
 }
 
-// CTAs that walk M rows: all at once when they are few, else a whole number per SM
-static int64_t norm_ctas(int64_t M, const NormShape& s, int per_sm) {
+// CTAs that walk M rows: all at once when they are few, else as many as the
+// SMs hold at `bytes` of shared memory a CTA
+static int64_t norm_ctas(int64_t M, const NormShape& s, size_t bytes, int most) {
   const int64_t need = s.warp_row ? (M + 3) / 4 : M;
+  int per_sm = most;
+  if (!s.warp_row) {
+    per_sm = (int)(norm::kRingBytes / bytes);
+    if (per_sm > most) per_sm = most;
+    if (per_sm < 1) per_sm = 1;
+  }
   const int64_t cap = (int64_t)device_sms() * per_sm;
   return need < cap ? need : cap;
 }
 
+static int ring_depth(size_t stage, int most) {
+  const int fit = (int)(norm::kRingBytes / stage);
+  return fit < most ? (fit < 1 ? 1 : fit) : most;
+}
+
+template <int NV, int kOut>
+static cudaError_t launch_norm_ring(const AddRmsNormParams& p, const NormShape& s, unsigned grid, size_t smem,
+                                    cudaStream_t st) {
+  const cudaError_t e = cudaFuncSetAttribute(add_rms_norm_ring_kernel<NV, kOut>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+  if (e == cudaSuccess) add_rms_norm_ring_kernel<NV, kOut><<<grid, s.threads, smem, st>>>(p);
+  return e;
+}
+
 template <int kOut>
-static void launch_norm_out(const AddRmsNormParams& p, const NormShape& s, unsigned grid, cudaStream_t st) {
-  if (s.warp_row) {
-    if (s.nv == 1) add_rms_norm_kernel<1, true, kOut><<<grid, s.threads, 0, st>>>(p);
-    else if (s.nv == 2) add_rms_norm_kernel<2, true, kOut><<<grid, s.threads, 0, st>>>(p);
-    else add_rms_norm_kernel<4, true, kOut><<<grid, s.threads, 0, st>>>(p);
-  } else {
-    if (s.nv == 2) add_rms_norm_kernel<2, false, kOut><<<grid, s.threads, 0, st>>>(p);
-    else add_rms_norm_kernel<4, false, kOut><<<grid, s.threads, 0, st>>>(p);
-  }
+static cudaError_t launch_norm_out(AddRmsNormParams p, cudaStream_t st) {
+  const NormShape s = norm_shape(p.K);
+  const size_t stage = (size_t)p.K * ((p.x_fp32 ? 4 : 2) + (p.res ? (p.res_fp32 ? 4 : 2) : 0));
+  p.ring = ring_depth(stage, norm::kRing);
+  const size_t smem = p.ring * stage;
+  const unsigned grid = (unsigned)norm_ctas(p.M, s, smem + 1024, s.warp_row ? 16 : 2048 / s.threads);
+  if (!s.warp_row)
+    return s.nv == 2 ? launch_norm_ring<2, kOut>(p, s, grid, smem, st) : launch_norm_ring<4, kOut>(p, s, grid, smem, st);
+  if (s.nv == 1) add_rms_norm_warp_kernel<1, kOut><<<grid, s.threads, 0, st>>>(p);
+  else if (s.nv == 2) add_rms_norm_warp_kernel<2, kOut><<<grid, s.threads, 0, st>>>(p);
+  else add_rms_norm_warp_kernel<4, kOut><<<grid, s.threads, 0, st>>>(p);
+  return cudaSuccess;
 }
 
 int launch_add_rms_norm(const AddRmsNormParams& p, cudaStream_t s) {
-  const NormShape sh = norm_shape(p.K);
-  const unsigned grid = (unsigned)norm_ctas(p.M, sh, 16);
-  if (p.y) launch_norm_out<kOutBf16>(p, sh, grid, s);
-  else if (p.scale_row) launch_norm_out<kOutE4M3Row>(p, sh, grid, s);
-  else launch_norm_out<kOutE4M3Block>(p, sh, grid, s);
-  return (int)cudaGetLastError();
+  const cudaError_t e = p.y ? launch_norm_out<kOutBf16>(p, s)
+                            : p.scale_row ? launch_norm_out<kOutE4M3Row>(p, s) : launch_norm_out<kOutE4M3Block>(p, s);
+  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+}
+
+// the grid, and with it the order of dw's sums, follows from M, K and the
+// widest row (fp32 h and dh), not from the types at hand
+static int64_t norm_bwd_ctas(int64_t M, int K) {
+  const NormShape s = norm_shape(K);
+  return norm_ctas(M, s, (size_t)ring_depth((size_t)K * 10, norm::kRingBwd) * K * 10 + 1024, s.warp_row ? 4 : 2);
 }
 
 int add_rms_norm_bwd_parts(int64_t M, int K) {
-  const NormShape s = norm_shape(K);
-  return (int)(norm_ctas(M, s, 2) * (s.warp_row ? 4 : 1));
+  return (int)(norm_bwd_ctas(M, K) * (norm_shape(K).warp_row ? 4 : 1));
+}
+
+template <int NV>
+static cudaError_t launch_norm_bwd_ring(AddRmsNormBwdParams p, int threads, unsigned grid, cudaStream_t st) {
+  const cudaError_t e = cudaFuncSetAttribute(add_rms_norm_bwd_ring_kernel<NV>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+  const size_t stage = (size_t)p.K * ((p.h_fp32 ? 4 : 2) + 2 + (p.dh ? (p.dh_fp32 ? 4 : 2) : 0));
+  p.ring = ring_depth((size_t)p.K * 10, norm::kRingBwd);
+  const size_t smem = p.ring * stage;
+  if (e == cudaSuccess) add_rms_norm_bwd_ring_kernel<NV><<<grid, threads, smem, st>>>(p);
+  return e;
 }
 
 int launch_add_rms_norm_bwd(const AddRmsNormBwdParams& p, cudaStream_t st) {
   const NormShape s = norm_shape(p.K);
-  const unsigned grid = (unsigned)norm_ctas(p.M, s, 2);
-  if (s.warp_row) {
-    if (s.nv == 1) add_rms_norm_bwd_kernel<1, true><<<grid, s.threads, 0, st>>>(p);
-    else if (s.nv == 2) add_rms_norm_bwd_kernel<2, true><<<grid, s.threads, 0, st>>>(p);
-    else add_rms_norm_bwd_kernel<4, true><<<grid, s.threads, 0, st>>>(p);
+  const unsigned grid = (unsigned)norm_bwd_ctas(p.M, p.K);
+  cudaError_t e = cudaSuccess;
+  if (!s.warp_row) {
+    e = s.nv == 2 ? launch_norm_bwd_ring<2>(p, s.threads, grid, st) : launch_norm_bwd_ring<4>(p, s.threads, grid, st);
+  } else if (s.nv == 1) {
+    add_rms_norm_bwd_warp_kernel<1><<<grid, s.threads, 0, st>>>(p);
+  } else if (s.nv == 2) {
+    add_rms_norm_bwd_warp_kernel<2><<<grid, s.threads, 0, st>>>(p);
   } else {
-    if (s.nv == 2) add_rms_norm_bwd_kernel<2, false><<<grid, s.threads, 0, st>>>(p);
-    else add_rms_norm_bwd_kernel<4, false><<<grid, s.threads, 0, st>>>(p);
+    add_rms_norm_bwd_warp_kernel<4><<<grid, s.threads, 0, st>>>(p);
   }
-  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
   if (p.dw) {
     const int parts = add_rms_norm_bwd_parts(p.M, p.K);

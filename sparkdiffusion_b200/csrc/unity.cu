@@ -5,10 +5,10 @@
 #include "select.cu"
 #include "lowrank.cu"
 #include "gemm.cu"
-#include "norm.cu"
-#include "gemm_block.cu"
 #include "attn.cu"
 #include "attn_bwd.cu"
+#include "norm.cu"
+#include "gemm_block.cu"
 #include "cross_attn.cu"
 #include "cross_attn_bwd.cu"
 #include "capi.cu"
