@@ -13,33 +13,20 @@
 
 namespace rola {
 
-namespace gemmb {
-constexpr int BM = 128, BK = 128;   // one 128-byte row of e4m3 per K block
-constexpr int GROUP_M = 16;         // M tiles per raster group (A and W tiles in flight share L2)
-template <int BN>
-struct Cfg {
-  static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK;
-  static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int STAGES = BN >= 128 ? 6 : 8;
-  static constexpr int NBUF = 4;                   // block accumulators in TMEM
-  static constexpr int COLS = NBUF * BN;
-  static constexpr int OFF_BAR = STAGES * STAGE;
-  static constexpr int SMEM = OFF_BAR + 512 + 1024;
-};
-}  // namespace gemmb
-
-// acc[0 .. 31] += v * s for 32 columns, two at a time
-__device__ __forceinline__ void scaled_add32(uint64_t (&acc)[16], const uint32_t (&v)[32], uint64_t s2) {
+// acc += v * s for 2 n columns, two at a time
+template <int n>
+__device__ __forceinline__ void scaled_add(uint64_t (&acc)[n], const uint32_t (&v)[2 * n], uint64_t s2) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
+  for (int i = 0; i < n; ++i)
     acc[i] = fma_f32x2(f2_pack(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), s2, acc[i]);
 }
 
-// 32 finished columns of one row: bias, rounding, 16-byte stores of 8 columns
-__device__ __forceinline__ void store_row32(const uint64_t (&acc)[16], const __nv_bfloat16* bias, __nv_bfloat16* row,
-                                            int col, int N) {
+// 2 n finished columns of one row: bias, rounding, 16-byte stores of 8 columns
+template <int n>
+__device__ __forceinline__ void store_row(const uint64_t (&acc)[n], const __nv_bfloat16* bias, __nv_bfloat16* row,
+                                          int col, int N) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < n / 4; ++i) {
     const int c = col + 8 * i;
     if (c < N) {
       float f[8];
@@ -62,10 +49,53 @@ __device__ __forceinline__ void store_row32(const uint64_t (&acc)[16], const __n
   }
 }
 
+// ---------------------------------------------------------------------------
+// 128 x BN tiles (BN 256 or 128), persistent CTAs, one per SM.  Every K block is
+// a hand-off from the MMA issuer to the epilogue and back, and what is in flight
+// is bounded by the 512 columns of tensor memory, so the accumulators are small
+// units with a hand-off each: 128 columns, four of them.  BN = 256 has two
+// streams (column halves) of two, and a warpgroup of the epilogue each (128 sums
+// a thread; the registers of the producer's warpgroup go to them by setmaxnreg);
+// BN = 128 one stream of four that both warpgroups share, 64 columns each.
+// Measured at 32760 x 15360 x 5120 (TFLOP/s): BN = 256 1780, with neither
+// hand-off nor epilogue 2860 (operands from L2), hand-offs alone 2270; SM pairs
+// (256 x 256 tiles, whose hand-offs cross SMs) 1340 with the hand-offs alone.
+// A warp of its own copies the scales of the next kScales blocks into shared
+// memory (4-byte cp.async, so any strides): loaded by the epilogue itself, even
+// four blocks ahead, they held it to one L2 access per block (1260 TFLOP/s).
+// ---------------------------------------------------------------------------
+namespace gemmb {
+constexpr int BM = 128, BK = 128;             // one 128-byte row of e4m3 per K block
+constexpr int GROUP_M = 16;                   // M tiles per raster group (operands in flight share L2)
+constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
+constexpr int LAUNCH_REGS = 168, REGS_LOAD = 56, REGS_EPI = 224;  // 65536 / 384, in steps of 8
+static_assert(128 * REGS_LOAD + 32 * EPI_WARPS * REGS_EPI <= THREADS * LAUNCH_REGS, "register split");
+constexpr int kScales = 8;                    // blocks whose scales are on their way
 template <int BN>
-__global__ void __launch_bounds__(192, 1)
+struct Cfg {
+  static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE = A_BYTES + B_BYTES;
+  static constexpr int STAGES = BN == 256 ? 4 : 6;
+  static constexpr int STREAMS = BN / 128, NBUF = 4 / STREAMS;
+  static constexpr int CW = BN / 2;           // columns of one epilogue warp
+  static constexpr int SC_FLOATS = 132;       // 128 row scales, W scales of the streams
+  static constexpr int OFF_SC = STAGES * STAGE;
+  static constexpr int OFF_BAR = (OFF_SC + kScales * SC_FLOATS * 4 + 15) / 16 * 16;
+  static constexpr int SMEM = OFF_BAR + 512 + 1024;
+};
+}  // namespace gemmb
+
+// 4-byte asynchronous copy to shared memory; the arrival on `bar` once every earlier copy of this thread landed
+__device__ __forceinline__ void cp_async4(uint32_t dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
+template <int BN>
+__global__ void __launch_bounds__(gemmb::THREADS, 1)
     gemm_block_tcgen05(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
-                       const GemmBlockParams p) {
+                            const GemmBlockParams p) {
   using namespace gemmb;
   using C = Cfg<BN>;
   extern __shared__ uint8_t smem_raw[];
@@ -75,11 +105,14 @@ __global__ void __launch_bounds__(192, 1)
   const uint32_t bar0 = base + C::OFF_BAR;
   auto full = [&](int s) { return bar0 + 8u * s; };
   auto empty = [&](int s) { return bar0 + 8u * (C::STAGES + s); };
-  auto acc_full = [&](int a) { return bar0 + 8u * (2 * C::STAGES + a); };
-  auto acc_empty = [&](int a) { return bar0 + 8u * (2 * C::STAGES + C::NBUF + a); };
-  const uint32_t drain = bar0 + 8u * (2 * C::STAGES + 2 * C::NBUF);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + C::OFF_BAR + 256);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + C::OFF_BAR + 264);
+  auto acc_full = [&](int h, int a) { return bar0 + 8u * (2 * C::STAGES + C::NBUF * h + a); };
+  auto acc_empty = [&](int h, int a) { return bar0 + 8u * (2 * C::STAGES + 4 + C::NBUF * h + a); };
+  auto sc_full = [&](int s) { return bar0 + 8u * (2 * C::STAGES + 8 + s); };
+  auto sc_empty = [&](int s) { return bar0 + 8u * (2 * C::STAGES + 8 + kScales + s); };
+  const uint32_t drain = bar0 + 8u * (2 * C::STAGES + 8 + 2 * kScales);
+  static_assert(8 * (2 * C::STAGES + 9 + 2 * kScales) <= 320, "barrier region");
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(gbase + C::OFF_BAR + 320);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + C::OFF_BAR + 328);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int num_m = (p.M + BM - 1) / BM, num_n = (p.N + BN - 1) / BN;
@@ -100,9 +133,14 @@ __global__ void __launch_bounds__(192, 1)
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
     }
-    for (int a = 0; a < C::NBUF; ++a) {
-      mbar_init(acc_full(a), 1);
-      mbar_init(acc_empty(a), 4);  // one arrival per epilogue warp
+    for (int h = 0; h < C::STREAMS; ++h)
+      for (int a = 0; a < C::NBUF; ++a) {
+        mbar_init(acc_full(h, a), 1);
+        mbar_init(acc_empty(h, a), EPI_WARPS / C::STREAMS);
+      }
+    for (int c = 0; c < kScales; ++c) {
+      mbar_init(sc_full(c), 32);
+      mbar_init(sc_empty(c), EPI_WARPS);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -111,14 +149,15 @@ __global__ void __launch_bounds__(192, 1)
     prefetch_tmap(&tb);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), C::COLS);
+    tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = *tmem_slot;  // stream h, buffer a: columns [128 (NBUF h + a), + 128)
 
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_LOAD));
   if (warp == 0) {
     if (elect_one()) {
       int it = 0;
@@ -135,7 +174,9 @@ __global__ void __launch_bounds__(192, 1)
           const uint32_t sa = base + s * C::STAGE;
           mbar_expect_tx(full(s), C::STAGE);
           tma_load_2d(sa, &ta, full(s), kb * BK, m0);
-          tma_load_2d(sa + C::A_BYTES, &tb, full(s), kb * BK, n0);
+#pragma unroll
+          for (int h = 0; h < C::STREAMS; ++h)
+            tma_load_2d(sa + C::A_BYTES + h * 128 * BK, &tb, full(s), kb * BK, n0 + 128 * h);
         }
       }
       // no load is still writing shared memory when the CTA exits
@@ -146,29 +187,58 @@ __global__ void __launch_bounds__(192, 1)
     }
   } else if (warp == 1) {
     if (elect_one()) {
-      constexpr uint32_t idesc = idesc_e4m3_f32(BM, BN);
+      constexpr uint32_t idesc = idesc_e4m3_f32(BM, 128);
       const int total = my_tiles * nk;
-      for (int it = 0; it < total; ++it) {
+      bool ok = true;
+      for (int it = 0; it < total && ok; ++it) {
         const int a = it % C::NBUF, s = it % C::STAGES;
-        // the epilogue has read this accumulator (block it - NBUF)
-        if (!mbar_wait(acc_empty(a), ((it / C::NBUF) & 1) ^ 1, abort_flag, kDevTimeoutSoftmax)) break;
-        if (!mbar_wait(full(s), (it / C::STAGES) & 1, abort_flag, kDevTimeoutLoad)) break;
-        tc_fence_after();
+        ok = mbar_wait(full(s), (it / C::STAGES) & 1, abort_flag, kDevTimeoutLoad);
         const uint32_t sa = base + s * C::STAGE, sb = sa + C::A_BYTES;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          mma_f8_ss(tmem + a * BN, sdesc_sw128(sa + kk * 32, 16, 1024), sdesc_sw128(sb + kk * 32, 16, 1024), idesc,
-                    kk > 0 ? 1u : 0u);
-        mma_commit(empty(s));
-        mma_commit(acc_full(a));
+        for (int h = 0; h < C::STREAMS; ++h) {
+          // the epilogue has read this accumulator (block it - NBUF)
+          ok = ok && mbar_wait(acc_empty(h, a), ((it / C::NBUF) & 1) ^ 1, abort_flag, kDevTimeoutSoftmax);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f8_ss(tmem + 128 * (C::NBUF * h + a), sdesc_sw128(sa + kk * 32, 16, 1024),
+                      sdesc_sw128(sb + h * 128 * BK + kk * 32, 16, 1024), idesc, kk > 0 ? 1u : 0u);
+          mma_commit(acc_full(h, a));
+        }
+        if (ok) mma_commit(empty(s));
       }
       // every MMA issued has completed before TMEM is freed, also on the abort path
       mma_commit(drain);
       mbar_wait_until(drain, 0, globaltimer_ns() + kWaitLimitNs);
     }
-  } else {
-    // epilogue warps 2..5: TMEM lane quadrant = warp % 4, thread = row of the tile
-    const int q = warp & 3;
+  } else if (warp == 2) {
+    // scales: slot c holds xs of the tile's 128 rows, then ws of its streams
+    int it = 0;
+    bool ok = true;
+    for (int lt = 0; lt < my_tiles && ok; ++lt) {
+      int m0, n0;
+      tile_coords(lt, m0, n0);
+      const float* ws = p.ws + (int64_t)min((n0 >> 7) + lane % C::STREAMS, (p.N - 1) >> 7) * p.ws_ld;
+      for (int kb = 0; kb < nk; ++kb, ++it) {
+        const int c = it % kScales;
+        ok = __all_sync(0xffffffffu, mbar_wait(sc_empty(c), ((it / kScales) & 1) ^ 1, abort_flag, kDevTimeoutSoftmax));
+        if (!ok) break;
+        const uint32_t dst = base + C::OFF_SC + c * C::SC_FLOATS * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t m = min(m0 + 32 * i + lane, p.M - 1);
+          cp_async4(dst + 4 * (32 * i + lane), p.xs + m * p.xs_sM + kb * p.xs_sK);
+        }
+        if (lane < C::STREAMS) cp_async4(dst + 4 * (128 + lane), ws + kb);
+        cp_async_arrive(sc_full(c));
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");  // no copy outlives the CTA
+  } else if (warp >= 4) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_EPI));
+    // warps 4-7: columns [0, CW) of the tile, warps 8-11: [CW, BN); TMEM lane quadrant = warp % 4
+    const int q = warp & 3, group = (warp - 4) >> 2, h = C::STREAMS == 2 ? group : 0;
     const int row = q * 32 + lane;
     int it = 0;
     bool ok = true;
@@ -176,43 +246,44 @@ __global__ void __launch_bounds__(192, 1)
       int m0, n0;
       tile_coords(lt, m0, n0);
       const int64_t m = m0 + row;
-      const float* xs = p.xs + (m < p.M ? m : 0) * p.xs_sM;
-      const float* ws = p.ws + (int64_t)(n0 / 128) * p.ws_ld;
-      uint64_t acc[BN / 32][16];
+      const int col = n0 + C::CW * group;
+      uint64_t acc[C::CW / 32][16];
 #pragma unroll
-      for (int c = 0; c < BN / 32; ++c)
+      for (int c = 0; c < C::CW / 32; ++c)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[c][i] = 0ull;
-      float s_next = __ldg(xs) * __ldg(ws);
       for (int kb = 0; kb < nk; ++kb, ++it) {
-        const int a = it % C::NBUF;
-        const float s = s_next;
-        if (kb + 1 < nk) s_next = __ldg(xs + (kb + 1) * p.xs_sK) * __ldg(ws + kb + 1);
-        ok = __all_sync(0xffffffffu, mbar_wait(acc_full(a), (it / C::NBUF) & 1, abort_flag, kDevTimeoutMma));
+        const int a = it % C::NBUF, c = it % kScales;
+        ok = __all_sync(0xffffffffu, mbar_wait(sc_full(c), (it / kScales) & 1, abort_flag, kDevTimeoutLoad));
         if (!ok) break;
-        tc_fence_after();
-        const uint32_t t = tmem + a * BN + ((uint32_t)(q * 32) << 16);
+        const float* sc = reinterpret_cast<const float*>(gbase + C::OFF_SC) + c * C::SC_FLOATS;
+        const float s = sc[row] * sc[128 + h];
         const uint64_t s2 = f2_pack(s, s);
+        ok = __all_sync(0xffffffffu, mbar_wait(acc_full(h, a), (it / C::NBUF) & 1, abort_flag, kDevTimeoutMma));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(sc_empty(c));
+        tc_fence_after();
+        const uint32_t t = tmem + 128 * (C::NBUF * h + a) + (C::CW * group) % 128 + ((uint32_t)(q * 32) << 16);
         uint32_t v[2][32];
         tmem_ld32(t, v[0]);
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) {
+        for (int c = 0; c < C::CW / 32; ++c) {
           tmem_ld_wait();
-          if (c + 1 < BN / 32) {
+          if (c + 1 < C::CW / 32) {
             tmem_ld32(t + 32 * (c + 1), v[(c + 1) & 1]);
           } else {
-            // the whole accumulator is in registers: the next block may overwrite it
+            // the warp's part is in registers: the block NBUF further may overwrite it
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty(a));
+            if (lane == 0) mbar_arrive(acc_empty(h, a));
           }
-          scaled_add32(acc[c], v[c & 1], s2);
+          scaled_add(acc[c], v[c & 1], s2);
         }
       }
       if (ok && m < p.M) {
         __nv_bfloat16* out = p.out + m * p.N;
 #pragma unroll
-        for (int c = 0; c < BN / 32; ++c) store_row32(acc[c], p.bias, out, n0 + 32 * c, p.N);
+        for (int c = 0; c < C::CW / 32; ++c) store_row(acc[c], p.bias, out, col + 32 * c, p.N);
       }
     }
   }
@@ -221,25 +292,36 @@ __global__ void __launch_bounds__(192, 1)
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, C::COLS);
+    tmem_dealloc(tmem, 512);
   }
 }
 
 template <int BN>
-static int launch_gemm_block_1sm(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, int sms,
-                                 cudaStream_t s) {
+static int launch_gemm_block_bn(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, int sms,
+                                cudaStream_t s) {
   using C = gemmb::Cfg<BN>;
-  cudaError_t e = cudaFuncSetAttribute(gemm_block_tcgen05<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  // setmaxnreg redistributes the block's launch registers; an increase beyond them would wait
+  cudaFuncAttributes fa;
+  cudaError_t e = cudaFuncGetAttributes(&fa, gemm_block_tcgen05<BN>);
+  if (e != cudaSuccess) return (int)e;
+  if (fa.numRegs < gemmb::LAUNCH_REGS) return -1;
+  e = cudaFuncSetAttribute(gemm_block_tcgen05<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   if (e != cudaSuccess) return (int)e;
   const int64_t tiles = (int64_t)((p.M + 127) / 128) * ((p.N + BN - 1) / BN);
-  gemm_block_tcgen05<BN><<<(unsigned)(tiles < sms ? tiles : sms), 192, C::SMEM, s>>>(ta, tb, p);
+  gemm_block_tcgen05<BN><<<(unsigned)(tiles < sms ? tiles : sms), gemmb::THREADS, C::SMEM, s>>>(ta, tb, p);
   return (int)cudaGetLastError();
 }
 
 int gemm_block_w_rows(int, int, int) { return 128; }
 
+// The wider tile unless its last wave of CTAs is so empty that the narrower one,
+// at 0.57 of its time a tile (measured), finishes first
 int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, cudaStream_t s) {
-  return launch_gemm_block_1sm<128>(ta, tb, p, device_sms(), s);
+  const int sms = device_sms();
+  const int64_t num_m = (p.M + 127) / 128;
+  const int64_t wide = (num_m * ((p.N + 255) / 256) + sms - 1) / sms, narrow = (num_m * ((p.N + 127) / 128) + sms - 1) / sms;
+  return narrow * 57 < wide * 100 ? launch_gemm_block_bn<128>(ta, tb, p, sms, s)
+                                  : launch_gemm_block_bn<256>(ta, tb, p, sms, s);
 }
 
 }  // namespace rola
