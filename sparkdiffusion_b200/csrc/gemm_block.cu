@@ -312,11 +312,100 @@ static int launch_gemm_block_bn(const CUtensorMap& ta, const CUtensorMap& tb, co
   return (int)cudaGetLastError();
 }
 
+// ---------------------------------------------------------------------------
+// Few rows (M <= 8 NT): the weight is read once and little else matters, so the
+// work is cut along N and K for bytes in flight: a CTA per 16 rows of wq, its 8
+// warps take the K blocks in turn, and the partial sums meet in shared memory
+// in warp order.  m16n8k32 MMAs with W as the row operand: a lane loads 16
+// consecutive bytes of its W rows and of its token and uses them as the operand
+// words of two MMAs; the order of k within a block is the same for both, which
+// is all a sum over the block needs.
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ void mma_m16n8k32_e4m3(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                  uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int NT>
+__global__ void __launch_bounds__(256) gemm_block_few_rows_kernel(const GemmBlockParams p) {
+  __shared__ float s_part[8][16][8 * NT + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16;
+  const int nk = (p.K + 127) / 128;
+  const uint8_t* w_lo = p.wq + (int64_t)(n0 + g) * p.K;
+  const bool lo = n0 + g < p.N, hi = n0 + g + 8 < p.N;
+  const float* ws = p.ws + (int64_t)(n0 / 128) * p.ws_ld;
+  float acc[NT][4] = {};
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll(NT == 1 ? 2 : 1)
+  for (int kb = warp; kb < nk; kb += 8) {
+    uint4 wl[2], wh[2], xv[NT][2];
+    float sx[NT][2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int k = kb * 128 + 64 * c + 16 * t;
+      const bool in = k < p.K;
+      wl[c] = in && lo ? __ldcs(reinterpret_cast<const uint4*>(w_lo + k)) : zero;
+      wh[c] = in && hi ? __ldcs(reinterpret_cast<const uint4*>(w_lo + 8ll * p.K + k)) : zero;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+        xv[j][c] = in && 8 * j + g < p.M ? __ldg(reinterpret_cast<const uint4*>(p.xq + (int64_t)(8 * j + g) * p.K + k)) : zero;
+    }
+    const float sw = __ldg(ws + kb);
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        sx[j][e] = __ldg(p.xs + (int64_t)min(8 * j + 2 * t + e, p.M - 1) * p.xs_sM + kb * p.xs_sK) * sw;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        mma_m16n8k32_e4m3(d, wl[c].x, wh[c].x, wl[c].y, wh[c].y, xv[j][c].x, xv[j][c].y);
+        mma_m16n8k32_e4m3(d, wl[c].z, wh[c].z, wl[c].w, wh[c].w, xv[j][c].z, xv[j][c].w);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] = fmaf(d[e], sx[j][e & 1], acc[j][e]);
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s_part[warp][g + 8 * (e >> 1)][8 * j + 2 * t + (e & 1)] = acc[j][e];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * p.M; i += 256) {
+    const int r = i & 15, m = i >> 4;
+    if (n0 + r < p.N) {
+      float v = 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v += s_part[u][r][m];
+      if (p.bias) v += bf2f(p.bias[n0 + r]);
+      p.out[(int64_t)m * p.N + n0 + r] = f2bf(v);
+    }
+  }
+}
+
+template <int NT>
+static int launch_gemm_block_few_rows(const GemmBlockParams& p, cudaStream_t s) {
+  gemm_block_few_rows_kernel<NT><<<(p.N + 15) / 16, 256, 0, s>>>(p);
+  return (int)cudaGetLastError();
+}
+
 int gemm_block_w_rows(int, int, int) { return 128; }
 
 // The wider tile unless its last wave of CTAs is so empty that the narrower one,
 // at 0.57 of its time a tile (measured), finishes first
 int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, cudaStream_t s) {
+  // Up to 8 rows the weight's bytes decide (M = 8, us, few rows | tiles: N x K =
+  // 15360 x 5120 18.9 | 19.5, 5120 x 5120 9.1 | 17, 1536 x 1536 3.7 | 7.8); from 9
+  // to 16 the second token tile costs, and only narrow outputs gain (M = 16: 29 |
+  // 19.5, 15.5 | 17, 4.0 | 7.8).
+  if (p.M <= 8) return launch_gemm_block_few_rows<1>(p, s);
+  if (p.M <= 16 && p.N <= 8192) return launch_gemm_block_few_rows<2>(p, s);
   const int sms = device_sms();
   const int64_t num_m = (p.M + 127) / 128;
   const int64_t wide = (num_m * ((p.N + 255) / 256) + sms - 1) / sms, narrow = (num_m * ((p.N + 127) / 128) + sms - 1) / sms;
