@@ -564,13 +564,10 @@ CrossAttnPlan cross_attn_plan(int B, int H, int Hkv, int Lq, int Lk) {
 int launch_cross_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CrossAttnParams& p,
                       cudaStream_t s) {
   using namespace xattn;
-  // setmaxnreg redistributes the block's launch registers; an increase beyond them would wait
-  cudaFuncAttributes fa;
-  cudaError_t e = cudaFuncGetAttributes(&fa, cross_attn_tcgen05);
-  if (e != cudaSuccess) return (int)e;
-  if (fa.numRegs < LAUNCH_REGS) return -1;
-  e = cudaFuncSetAttribute(cross_attn_tcgen05, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-  if (e != cudaSuccess) return (int)e;
+  static KernelReady ready;
+  const int rc = kernel_ready(ready, cross_attn_tcgen05, SMEM, LAUNCH_REGS);
+  if (rc != 0) return rc;
+  cudaError_t e;
   const int sms = device_sms();
   cross_attn_tcgen05<<<(unsigned)(p.items < sms ? p.items : sms), THREADS, SMEM, s>>>(tq, tk, tv, p);
   e = cudaGetLastError();

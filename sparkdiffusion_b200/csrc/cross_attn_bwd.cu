@@ -495,10 +495,11 @@ int cross_bwd_splits(int B, int H, int Hkv, int Lq, int Lk) {
 int launch_cross_attn_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
                           const CrossBwdParams& p, cudaStream_t s) {
   using namespace bwd;
-  cudaError_t e = cudaFuncSetAttribute(cross_bwd_dq_tcgen05, cudaFuncAttributeMaxDynamicSharedMemorySize, DQ_SMEM);
-  if (e == cudaSuccess)
-    e = cudaFuncSetAttribute(cross_bwd_dkdv_tcgen05, cudaFuncAttributeMaxDynamicSharedMemorySize, KV_SMEM);
-  if (e != cudaSuccess) return (int)e;
+  static KernelReady ready_dq, ready_dkdv;
+  int rc = kernel_ready(ready_dq, cross_bwd_dq_tcgen05, DQ_SMEM);
+  if (rc == 0) rc = kernel_ready(ready_dkdv, cross_bwd_dkdv_tcgen05, KV_SMEM);
+  if (rc != 0) return rc;
+  cudaError_t e;
   cross_bwd_dq_tcgen05<<<(unsigned)((int64_t)p.NQT * p.B * p.H), DQ_THREADS, DQ_SMEM, s>>>(tq, tk, tv, tdo, p);
   if ((e = cudaGetLastError()) != cudaSuccess) return (int)e;
   cross_bwd_dkdv_tcgen05<<<(unsigned)((int64_t)p.NKT * p.B * p.Hkv * p.nsplit), THREADS, KV_SMEM, s>>>(tq, tk, tv, tdo,

@@ -300,13 +300,9 @@ template <int BN>
 static int launch_gemm_block_bn(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, int sms,
                                 cudaStream_t s) {
   using C = gemmb::Cfg<BN>;
-  // setmaxnreg redistributes the block's launch registers; an increase beyond them would wait
-  cudaFuncAttributes fa;
-  cudaError_t e = cudaFuncGetAttributes(&fa, gemm_block_tcgen05<BN>);
-  if (e != cudaSuccess) return (int)e;
-  if (fa.numRegs < gemmb::LAUNCH_REGS) return -1;
-  e = cudaFuncSetAttribute(gemm_block_tcgen05<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-  if (e != cudaSuccess) return (int)e;
+  static KernelReady ready;
+  const int rc = kernel_ready(ready, gemm_block_tcgen05<BN>, C::SMEM, gemmb::LAUNCH_REGS);
+  if (rc != 0) return rc;
   const int64_t tiles = (int64_t)((p.M + 127) / 128) * ((p.N + BN - 1) / BN);
   gemm_block_tcgen05<BN><<<(unsigned)(tiles < sms ? tiles : sms), gemmb::THREADS, C::SMEM, s>>>(ta, tb, p);
   return (int)cudaGetLastError();

@@ -16,6 +16,8 @@
 // element: memory bound.  A row stays in registers between its statistics and
 // its output (8 columns a vector, NV vectors a thread); rows up to 1024 columns
 // take a warp each (no barrier), longer ones a CTA.
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -435,6 +437,29 @@ static int device_sms() {
   return sms;
 }
 
+// What a kernel's launches need once per device: its dynamic shared memory
+// allowed and, where it splits its registers by setmaxnreg, as many of them as
+// the split assumes (an increase beyond the launch's would wait).  One static
+// KernelReady per kernel; a race of two first calls sets the same twice.
+struct KernelReady {
+  std::atomic<bool> done[64];
+};
+template <typename Kernel>
+static int kernel_ready(KernelReady& r, Kernel* k, int smem, int min_regs = 0) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (dev >= 0 && dev < 64 && r.done[dev].load(std::memory_order_acquire)) return 0;
+  if (min_regs > 0) {
+    cudaFuncAttributes fa;
+    if ((e = cudaFuncGetAttributes(&fa, k)) != cudaSuccess) return (int)e;
+    if (fa.numRegs < min_regs) return -1;
+  }
+  if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return (int)e;
+  if (dev >= 0 && dev < 64) r.done[dev].store(true, std::memory_order_release);
+  return 0;
+}
+
 // CTAs that walk M rows: all at once when they are few, else as many as the
 // SMs hold at `bytes` of shared memory a CTA
 static int64_t norm_ctas(int64_t M, const NormShape& s, size_t bytes, int most) {
@@ -455,16 +480,16 @@ static int ring_depth(size_t stage, int most) {
 }
 
 template <int NV, int kOut>
-static cudaError_t launch_norm_ring(const AddRmsNormParams& p, const NormShape& s, unsigned grid, size_t smem,
-                                    cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(add_rms_norm_ring_kernel<NV, kOut>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
-  if (e == cudaSuccess) add_rms_norm_ring_kernel<NV, kOut><<<grid, s.threads, smem, st>>>(p);
-  return e;
+static int launch_norm_ring(const AddRmsNormParams& p, const NormShape& s, unsigned grid, size_t smem,
+                            cudaStream_t st) {
+  static KernelReady ready;
+  const int rc = kernel_ready(ready, add_rms_norm_ring_kernel<NV, kOut>, 224 * 1024);
+  if (rc == 0) add_rms_norm_ring_kernel<NV, kOut><<<grid, s.threads, smem, st>>>(p);
+  return rc;
 }
 
 template <int kOut>
-static cudaError_t launch_norm_out(AddRmsNormParams p, cudaStream_t st) {
+static int launch_norm_out(AddRmsNormParams p, cudaStream_t st) {
   const NormShape s = norm_shape(p.K);
   const size_t stage = (size_t)p.K * ((p.x_fp32 ? 4 : 2) + (p.res ? (p.res_fp32 ? 4 : 2) : 0));
   p.ring = ring_depth(stage, norm::kRing);
@@ -475,13 +500,13 @@ static cudaError_t launch_norm_out(AddRmsNormParams p, cudaStream_t st) {
   if (s.nv == 1) add_rms_norm_warp_kernel<1, kOut><<<grid, s.threads, 0, st>>>(p);
   else if (s.nv == 2) add_rms_norm_warp_kernel<2, kOut><<<grid, s.threads, 0, st>>>(p);
   else add_rms_norm_warp_kernel<4, kOut><<<grid, s.threads, 0, st>>>(p);
-  return cudaSuccess;
+  return 0;
 }
 
 int launch_add_rms_norm(const AddRmsNormParams& p, cudaStream_t s) {
-  const cudaError_t e = p.y ? launch_norm_out<kOutBf16>(p, s)
-                            : p.scale_row ? launch_norm_out<kOutE4M3Row>(p, s) : launch_norm_out<kOutE4M3Block>(p, s);
-  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+  const int rc = p.y ? launch_norm_out<kOutBf16>(p, s)
+                     : p.scale_row ? launch_norm_out<kOutE4M3Row>(p, s) : launch_norm_out<kOutE4M3Block>(p, s);
+  return rc != 0 ? rc : (int)cudaGetLastError();
 }
 
 // the grid, and with it the order of dw's sums, follows from M, K and the
@@ -496,22 +521,22 @@ int add_rms_norm_bwd_parts(int64_t M, int K) {
 }
 
 template <int NV>
-static cudaError_t launch_norm_bwd_ring(AddRmsNormBwdParams p, int threads, unsigned grid, cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(add_rms_norm_bwd_ring_kernel<NV>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
+static int launch_norm_bwd_ring(AddRmsNormBwdParams p, int threads, unsigned grid, cudaStream_t st) {
+  static KernelReady ready;
+  const int rc = kernel_ready(ready, add_rms_norm_bwd_ring_kernel<NV>, 224 * 1024);
   const size_t stage = (size_t)p.K * ((p.h_fp32 ? 4 : 2) + 2 + (p.dh ? (p.dh_fp32 ? 4 : 2) : 0));
   p.ring = ring_depth((size_t)p.K * 10, norm::kRingBwd);
   const size_t smem = p.ring * stage;
-  if (e == cudaSuccess) add_rms_norm_bwd_ring_kernel<NV><<<grid, threads, smem, st>>>(p);
-  return e;
+  if (rc == 0) add_rms_norm_bwd_ring_kernel<NV><<<grid, threads, smem, st>>>(p);
+  return rc;
 }
 
 int launch_add_rms_norm_bwd(const AddRmsNormBwdParams& p, cudaStream_t st) {
   const NormShape s = norm_shape(p.K);
   const unsigned grid = (unsigned)norm_bwd_ctas(p.M, p.K);
-  cudaError_t e = cudaSuccess;
+  int rc = 0;
   if (!s.warp_row) {
-    e = s.nv == 2 ? launch_norm_bwd_ring<2>(p, s.threads, grid, st) : launch_norm_bwd_ring<4>(p, s.threads, grid, st);
+    rc = s.nv == 2 ? launch_norm_bwd_ring<2>(p, s.threads, grid, st) : launch_norm_bwd_ring<4>(p, s.threads, grid, st);
   } else if (s.nv == 1) {
     add_rms_norm_bwd_warp_kernel<1><<<grid, s.threads, 0, st>>>(p);
   } else if (s.nv == 2) {
@@ -519,8 +544,8 @@ int launch_add_rms_norm_bwd(const AddRmsNormBwdParams& p, cudaStream_t st) {
   } else {
     add_rms_norm_bwd_warp_kernel<4><<<grid, s.threads, 0, st>>>(p);
   }
-  if (e == cudaSuccess) e = cudaGetLastError();
-  if (e != cudaSuccess) return (int)e;
+  if (rc == 0) rc = (int)cudaGetLastError();
+  if (rc != 0) return rc;
   if (p.dw) {
     const int parts = add_rms_norm_bwd_parts(p.M, p.K);
     dw_reduce_kernel<<<(p.K + 31) / 32, 256, 0, st>>>(p.dw_part, parts, p.K, p.dw, p.w_fp32);

@@ -698,62 +698,80 @@ SCALE_BLOCK = 128  # values that share a scale
 E4M3 = torch.float8_e4m3fn
 
 
-def _one_device(what: str, *ts: torch.Tensor | None) -> torch.device:
-    """The CUDA device all of ``ts`` live on (the launch goes to it, on its current stream)."""
-    dev = None
+def _device_of(what: str, *ts: torch.Tensor | None) -> int:
+    """Index of the CUDA device all of ``ts`` live on (the launch goes to it, on its current stream)."""
+    dev = -2
     for t in ts:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError(f"{what}: CUDA tensors required (no CPU fallback)")
-        if dev is not None and t.device != dev:
-            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-        dev = t.device
+        if t is not None:
+            d = t.get_device()  # -1: CPU
+            if d != dev:
+                if d < 0:
+                    raise ValueError(f"{what}: CUDA tensors required (no CPU fallback)")
+                if dev >= 0:
+                    raise ValueError(f"{what}: tensors on cuda:{dev} and cuda:{d}")
+                dev = d
     return dev
 
 
-def _call_on(dev: torch.device, name: str, *args) -> None:
-    """``_lib.call`` on ``dev`` with its current stream as the last argument."""
-    with torch.cuda.device(dev):
-        _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+def _call_on(dev: int, name: str, *args) -> None:
+    """The library's ``name`` on device ``dev``, its current stream as the last argument."""
+    if torch._C._cuda_getDevice() == dev:
+        rc = getattr(_lib.lib(), name)(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(_lib.lib(), name)(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc != 0:
+        _lib.check(rc, name)
 
 
-def _rows(t: torch.Tensor, K: int, what: str, dtypes=(BF16, torch.float32)) -> tuple[torch.Tensor, int]:
-    """``t [..., K]`` as ``([M, K]`` with unit column stride and 16-byte rows, its row stride)``; copies what is not."""
-    if t.dtype not in dtypes:
-        raise ValueError(f"{what}: {' or '.join(str(d) for d in dtypes)} required, got {t.dtype}")
+def _rows(t: torch.Tensor, K: int, what: str) -> tuple[torch.Tensor, int, int, int]:
+    """``t [..., K]`` (bf16 or fp32) as rows the kernels take, unit column stride
+    and 16-byte rows (copied where it is not): ``(rows, address, is fp32, row stride)``."""
+    if t.dtype is BF16:
+        fp32, mask = 0, 7
+    elif t.dtype is torch.float32:
+        fp32, mask = 1, 3
+    else:
+        raise ValueError(f"{what}: bf16 or fp32 required, got {t.dtype}")
     if t.dim() < 1 or t.shape[-1] != K:
         raise ValueError(f"{what}: last dimension must be {K}, got shape {tuple(t.shape)}")
-    t2 = t.reshape(-1, K)
-    el = t.element_size()
-    if (t2.stride(1) != 1 or t2.data_ptr() % 16 or (t2.shape[0] > 1 and (t2.stride(0) < K or t2.stride(0) * el % 16))):
-        t2 = t2.clone(memory_format=torch.contiguous_format)
-    return t2, (t2.stride(0) if t2.shape[0] > 1 else K)
+    if t.dim() != 2:
+        t = t.reshape(-1, K)
+    ld, cs = t.stride()
+    if cs != 1 or t.data_ptr() & 15 or (t.shape[0] > 1 and (ld < K or ld & mask)):
+        t = t.clone(memory_format=torch.contiguous_format)
+        ld = K
+    return t, t.data_ptr(), fp32, ld if t.shape[0] > 1 else K
 
 
-def _fp32(t: torch.Tensor | None) -> int:
-    return int(t is not None and t.dtype == torch.float32)
+def _norm_weight(weight: torch.Tensor, K: int, what: str) -> tuple[torch.Tensor, int]:
+    """``weight`` as a dense 16-byte aligned vector, and whether it is fp32."""
+    fp32 = weight.dtype is torch.float32
+    if weight.numel() != K or not (fp32 or weight.dtype is BF16):
+        raise ValueError(f"{what}: weight must have {K} bf16 or fp32 elements")
+    if not weight.is_contiguous() or weight.data_ptr() & 15:
+        weight = weight.clone(memory_format=torch.contiguous_format)
+    return weight, int(fp32)
 
 
 def _norm_args(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None, what: str):
-    dev = _one_device(what, x, weight, residual)
+    dev = _device_of(what, x, weight, residual)
     if x.dim() < 1:
         raise ValueError(f"{what}: x must have a last dimension")
     K = x.shape[-1]
     if K == 0 or K % 8 or K > 16384:
         raise ValueError(f"{what}: the last dimension must be a multiple of 8, at most 16384, got {K}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"{what}: residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
-    x2, x_ld = _rows(x, K, f"{what}: x")
-    r2, r_ld = (None, 0) if residual is None else _rows(residual, K, f"{what}: residual")
-    if weight.numel() != K or weight.dtype not in (BF16, torch.float32):
-        raise ValueError(f"{what}: weight must have {K} bf16 or fp32 elements")
-    w = weight.reshape(-1).contiguous()
-    if w.data_ptr() % 16:
-        w = w.clone()
-    h = None if residual is None else torch.empty(x.shape, device=dev, dtype=residual.dtype)
-    head = (_ptr(x2), _fp32(x2), x_ld, _ptr(r2), _fp32(r2), r_ld, _ptr(w), _fp32(w), x2.shape[0], K)
-    return dev, head, (x2, r2, w), h
+    xr, xp, xf, x_ld = _rows(x, K, what)
+    rr, rp, rf, r_ld, h = None, None, 0, 0, None
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError(f"{what}: residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
+        rr, rp, rf, r_ld = _rows(residual, K, what)
+        h = torch.empty(x.shape, device=x.device, dtype=residual.dtype)
+    w, wf = _norm_weight(weight, K, what)
+    M = xr.shape[0]
+    # the rows travel along: a copy made above has to live until its kernel is launched
+    return dev, M, K, (xp, xf, x_ld, rp, rf, r_ld, w.data_ptr(), wf, M, K), h, (xr, rr, w)
 
 
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
@@ -764,20 +782,19 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     one shape, ``weight`` bf16 or fp32.  ``rstd`` (fp32, one per row) receives
     the row factors.  Beside ``train.rms_norm``; differentiable as
     ``train.add_rms_norm``."""
-    dev, head, keep, h = _norm_args(x, weight, residual, "add_rms_norm")
-    y = torch.empty(x.shape, device=dev, dtype=BF16)
-    M = head[8]
-    if rstd is not None and (rstd.device != dev or rstd.dtype != torch.float32 or rstd.numel() != M
+    dev, M, K, head, h, keep = _norm_args(x, weight, residual, "add_rms_norm")
+    y = torch.empty(x.shape, device=x.device, dtype=BF16)
+    if rstd is not None and (rstd.get_device() != dev or rstd.dtype != torch.float32 or rstd.numel() != M
                              or not rstd.is_contiguous()):
         raise ValueError("add_rms_norm: rstd must be a contiguous fp32 tensor of one value per row")
     if M:
-        _call_on(dev, "rola_b200_add_rms_norm", *head, eps, _ptr(h), _ptr(y), _ptr(rstd))
+        _call_on(dev, "rola_b200_add_rms_norm", *head, eps, _ptr(h), y.data_ptr(), _ptr(rstd))
     return y, (x if h is None else h)
 
 
 def _block_scales(M: int, K: int, dev) -> torch.Tensor:
     """``[M, ceil(K/128)]`` fp32 scales, stored one block's column after the other (what the product reads)."""
-    return torch.empty((K + SCALE_BLOCK - 1) // SCALE_BLOCK, M, device=dev, dtype=torch.float32).t()
+    return torch.empty_strided((M, (K + SCALE_BLOCK - 1) // SCALE_BLOCK), (1, M), device=dev, dtype=torch.float32)
 
 
 def add_rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, residual: torch.Tensor | None = None,
@@ -788,18 +805,17 @@ def add_rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, 
     row, ``scale [...]``, for ``qkv_gemm_fp8``.  Scales are ``max|y|/448 + 1e-12``."""
     if block not in (SCALE_BLOCK, None):
         raise ValueError("add_rms_norm_e4m3: block must be 128, or None for one scale per row")
-    dev, head, keep, h = _norm_args(x, weight, residual, "add_rms_norm_e4m3")
-    M, K = head[8], head[9]
-    yq = torch.empty(x.shape, device=dev, dtype=E4M3)
-    scale = torch.empty(M, device=dev, dtype=torch.float32) if block is None else _block_scales(M, K, dev)
-    sM, sK = (1, 0) if block is None else scale.stride()
-    if M:
-        _call_on(dev, "rola_b200_add_rms_norm_e4m3", *head, eps, _ptr(h), _ptr(yq), _ptr(scale), sM, sK, block or 0)
-    lead = x.shape[:-1]
+    dev, M, K, head, h, keep = _norm_args(x, weight, residual, "add_rms_norm_e4m3")
+    yq = torch.empty(x.shape, device=x.device, dtype=E4M3)
     if block is None:
-        scale = scale.view(lead)
-    elif len(lead) != 1:
-        scale = scale.unflatten(0, lead) if lead else scale[0]
+        scale, sM, sK, blk = torch.empty(M, device=x.device, dtype=torch.float32), 1, 0, 0
+    else:
+        scale, sM, sK, blk = _block_scales(M, K, x.device), 1, M, block
+    if M:
+        _call_on(dev, "rola_b200_add_rms_norm_e4m3", *head, eps, _ptr(h), yq.data_ptr(), scale.data_ptr(), sM, sK, blk)
+    if x.dim() != 2:
+        lead = x.shape[:-1]
+        scale = scale.view(lead) if block is None else scale.unflatten(0, lead) if lead else scale[0]
     return yq, scale, (x if h is None else h)
 
 
@@ -810,35 +826,30 @@ def add_rms_norm_bwd(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, 
     and row factors: ``dy`` is the gradient of y, ``dh`` of h (None: zero).  dx
     and dresidual share one tensor where their types agree."""
     what = "add_rms_norm_bwd"
-    dev = _one_device(what, h, weight, rstd, dy, dh)
+    dev = _device_of(what, h, weight, rstd, dy, dh)
     K = h.shape[-1]
     if dy.shape != h.shape or (dh is not None and dh.shape != h.shape):
         raise ValueError(f"{what}: dy and dh must have the shape of h")
     for d in (x_dtype, res_dtype):
         if d not in (BF16, torch.float32, None):
             raise ValueError(f"{what}: bf16 or fp32 gradients only")
-    h2, h_ld = _rows(h, K, f"{what}: h")
-    dy2, dy_ld = _rows(dy.to(BF16), K, f"{what}: dy")
-    dh2, dh_ld = (None, 0) if dh is None else _rows(dh, K, f"{what}: dh")
-    M = h2.shape[0]
+    hr, hp, hf, h_ld = _rows(h, K, what)
+    yr, yp, _, dy_ld = _rows(dy if dy.dtype is BF16 else dy.to(BF16), K, what)
+    dr, dp, df, dh_ld = (None, None, 0, 0) if dh is None else _rows(dh, K, what)
+    M = hr.shape[0]
     if rstd.dtype != torch.float32 or rstd.numel() != M or not rstd.is_contiguous():
         raise ValueError(f"{what}: rstd must be add_rms_norm's row factors")
-    if weight.numel() != K or weight.dtype not in (BF16, torch.float32):
-        raise ValueError(f"{what}: weight must have {K} bf16 or fp32 elements")
-    w = weight.reshape(-1).contiguous()
-    if w.data_ptr() % 16:
-        w = w.clone()
-    dx = torch.empty(h.shape, device=dev, dtype=x_dtype)
+    w, wf = _norm_weight(weight, K, what)
+    dx = torch.empty(h.shape, device=h.device, dtype=x_dtype)
     dres = None if res_dtype is None else dx if res_dtype == x_dtype else torch.empty_like(dx, dtype=res_dtype)
-    dw = torch.zeros_like(w) if need_dw and M == 0 else torch.empty_like(w) if need_dw else None
+    dw = None if not need_dw else torch.empty_like(w) if M else torch.zeros_like(w)
     if M:
         nb = _lib.lib().rola_b200_add_rms_norm_bwd_workspace(M, K) if need_dw else 0
-        with torch.cuda.device(dev):
-            ws = torch.empty(nb, device=dev, dtype=torch.uint8) if nb else None
-        _call_on(dev, "rola_b200_add_rms_norm_bwd", _ptr(h2), _fp32(h2), h_ld, _ptr(w), _fp32(w), _ptr(rstd),
-                 _ptr(dy2), dy_ld, _ptr(dh2), _fp32(dh2), dh_ld, M, K, _ptr(dx), _fp32(dx),
-                 _ptr(None if dres is dx else dres), _fp32(dres), _ptr(dw), _ptr(ws), nb)
-    return dx, dres, None if dw is None else dw.view(weight.shape)
+        ws = torch.empty(nb, device=h.device, dtype=torch.uint8) if nb else None
+        _call_on(dev, "rola_b200_add_rms_norm_bwd", hp, hf, h_ld, w.data_ptr(), wf, rstd.data_ptr(), yp, dy_ld, dp, df,
+                 dh_ld, M, K, dx.data_ptr(), int(x_dtype is torch.float32), None if dres is dx else _ptr(dres),
+                 int(res_dtype is torch.float32), _ptr(dw), _ptr(ws), nb)
+    return dx, dres, dw
 
 
 def quantize_blocks_e4m3(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -846,16 +857,15 @@ def quantize_blocks_e4m3(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     scale fp32 [M, ceil(K/128)])``, one scale per row and 128 columns: the
     operand of ``gemm_fp8_block`` where no norm precedes the product."""
     what = "quantize_blocks_e4m3"
-    dev = _one_device(what, x)
+    dev = _device_of(what, x)
     if x.dim() != 2 or x.shape[1] == 0 or x.shape[1] % 8 or x.shape[1] > 16384:
         raise ValueError(f"{what}: [M, K] with K a multiple of 8, at most 16384, required")
     M, K = x.shape
-    x2, ld = _rows(x, K, f"{what}: x")
-    xq = torch.empty(M, K, device=dev, dtype=E4M3)
-    scale = _block_scales(M, K, dev)
+    xr, xp, xf, ld = _rows(x, K, what)
+    xq = torch.empty(M, K, device=x.device, dtype=E4M3)
+    scale = _block_scales(M, K, x.device)
     if M:
-        _call_on(dev, "rola_b200_quantize_blocks_e4m3", _ptr(x2), _fp32(x2), ld, M, K, _ptr(xq), _ptr(scale),
-                 *scale.stride())
+        _call_on(dev, "rola_b200_quantize_blocks_e4m3", xp, xf, ld, M, K, xq.data_ptr(), scale.data_ptr(), 1, M)
     return xq, scale
 
 
@@ -864,15 +874,20 @@ def quantize_tiles_e4m3(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     fp32 [ceil(N/128), ceil(K/128)])``, one scale per 128 x 128 block; done once
     per weight."""
     what = "quantize_tiles_e4m3"
-    dev = _one_device(what, w)
+    dev = _device_of(what, w)
     if w.dim() != 2 or w.shape[1] == 0 or w.shape[1] % 8 or max(w.shape) > 65536 or w.shape[0] == 0:
         raise ValueError(f"{what}: [N, K] with K a multiple of 8, both at most 65536, required")
     N, K = w.shape
-    w2, ld = _rows(w, K, f"{what}: w")
-    wq = torch.empty(N, K, device=dev, dtype=E4M3)
-    scale = torch.empty((N + 127) // 128, (K + 127) // 128, device=dev, dtype=torch.float32)
-    _call_on(dev, "rola_b200_quantize_tiles_e4m3", _ptr(w2), _fp32(w2), ld, N, K, _ptr(wq), _ptr(scale))
+    wr, wp, wf, ld = _rows(w, K, what)
+    wq = torch.empty(N, K, device=w.device, dtype=E4M3)
+    scale = torch.empty((N + 127) // 128, (K + 127) // 128, device=w.device, dtype=torch.float32)
+    _call_on(dev, "rola_b200_quantize_tiles_e4m3", wp, wf, ld, N, K, wq.data_ptr(), scale.data_ptr())
     return wq, scale
+
+
+def _dense16(t: torch.Tensor) -> torch.Tensor:
+    """``t``, copied unless dense and 16-byte aligned."""
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
 
 
 def gemm_fp8_block(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_scale: torch.Tensor,
@@ -883,62 +898,74 @@ def gemm_fp8_block(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_
     ``quantize_tiles_e4m3``), fp32 sums.  Beside ``qkv_gemm_fp8``, whose scales
     are one per row.  N % 8 == 0, K % 16 == 0."""
     what = "gemm_fp8_block"
-    dev = _one_device(what, xq, x_scale, wq, w_scale, bias)
-    if xq.dtype != E4M3 or wq.dtype != E4M3:
+    dev = _device_of(what, xq, x_scale, wq, w_scale, bias)
+    if xq.dtype is not E4M3 or wq.dtype is not E4M3:
         raise ValueError(f"{what}: float8_e4m3fn operands required")
     if xq.dim() != 2 or wq.dim() != 2 or xq.shape[1] != wq.shape[1]:
         raise ValueError(f"{what}: weight {tuple(wq.shape)} does not match x {tuple(xq.shape)}")
-    (M, K), N = xq.shape, wq.shape[0]
-    nk = (K + SCALE_BLOCK - 1) // SCALE_BLOCK
-    if K == 0 or N == 0 or K % 16 or N % 8 or max(N, K) > 65536:
+    M, K = xq.shape
+    N = wq.shape[0]
+    nk, nn = (K + SCALE_BLOCK - 1) // SCALE_BLOCK, (N + SCALE_BLOCK - 1) // SCALE_BLOCK
+    if K == 0 or N == 0 or K % 16 or N % 8 or N > 65536 or K > 65536:
         raise ValueError(f"{what}: K must be a multiple of 16 and N of 8, both at most 65536, got K={K}, N={N}")
-    if x_scale.dtype != torch.float32 or tuple(x_scale.shape) != (M, nk):
+    if x_scale.dtype is not torch.float32 or x_scale.shape != (M, nk):
         raise ValueError(f"{what}: x_scale must be fp32 {(M, nk)}, got {tuple(x_scale.shape)}")
-    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != ((N + 127) // 128, nk):
-        raise ValueError(f"{what}: w_scale must be fp32 {((N + 127) // 128, nk)}, got {tuple(w_scale.shape)}")
-    if bias is not None and bias.numel() != N:
-        raise ValueError(f"{what}: bias must have {N} elements")
-    b = None if bias is None else bias.reshape(-1).to(BF16).contiguous()
-    xq, wq, b = (t if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0)
-                 else t.clone(memory_format=torch.contiguous_format) for t in (xq, wq, b))
+    if w_scale.dtype is not torch.float32 or w_scale.shape != (nn, nk):
+        raise ValueError(f"{what}: w_scale must be fp32 {(nn, nk)}, got {tuple(w_scale.shape)}")
+    if bias is not None:
+        if bias.numel() != N:
+            raise ValueError(f"{what}: bias must have {N} elements")
+        bias = _dense16(bias if bias.dtype is BF16 else bias.to(BF16))
+    xq, wq = _dense16(xq), _dense16(wq)
     w_scale = w_scale.contiguous()
-    out = torch.empty(M, N, device=dev, dtype=BF16)
+    out = torch.empty(M, N, device=xq.device, dtype=BF16)
     if M:
-        _call_on(dev, "rola_b200_gemm_fp8_block", _ptr(xq), _ptr(x_scale), *x_scale.stride(), _ptr(wq), _ptr(w_scale),
-                 _ptr(b), _ptr(out), M, N, K)
+        sM, sK = x_scale.stride()
+        _call_on(dev, "rola_b200_gemm_fp8_block", xq.data_ptr(), x_scale.data_ptr(), sM, sK, wq.data_ptr(),
+                 w_scale.data_ptr(), _ptr(bias), out.data_ptr(), M, N, K)
     return out
 
 
-def _head_view(t: torch.Tensor) -> torch.Tensor:
-    """``t [B, H, L, 128]`` as the kernels can map it: unit last stride, positive
-    strides of 16-byte multiples, 16-byte base (a broadcast or unaligned view is copied)."""
-    if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(
-            n == 1 or (s > 0 and s % 8 == 0) for n, s in zip(t.shape[:3], t.stride()[:3])):
-        return t
-    return _token_major(t)
+def _head_args(t: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int, int]]:
+    """``t [B, H, L, 128]`` as the kernels can map it, and ``(address, b, h, t
+    strides)``: unit last stride, positive strides of 16-byte multiples, 16-byte
+    base.  A broadcast or unaligned view is copied; the strides of dimensions of
+    size 1 carry no meaning and get one the maps accept."""
+    p, (sB, sH, sT, sD) = t.data_ptr(), t.stride()
+    if sD == 1 and sB > 0 and sH > 0 and sT > 0 and not (p & 15 or (sB | sH | sT) & 7):
+        return t, (p, sB, sH, sT)
+    st = tuple(HEAD_DIM if n == 1 else s for n, s in zip(t.shape, (sB, sH, sT)))
+    if sD != 1 or p & 15 or any(s <= 0 or s & 7 for s in st):
+        t = _token_major(t)
+        p = t.data_ptr()
+        st = tuple(HEAD_DIM if n == 1 else s for n, s in zip(t.shape, t.stride()[:3]))
+    return t, (p, *st)
 
 
-def _head_strides(t: torch.Tensor) -> tuple[int, int, int]:
-    """(b, h, t) strides; those of dimensions of size 1 carry no meaning and get one the maps accept."""
-    return tuple(s if n > 1 else max(HEAD_DIM, 8 * (abs(s) // 8)) for n, s in zip(t.shape[:3], t.stride()[:3]))
+def _token_major_empty(B: int, H: int, L: int, dev) -> torch.Tensor:
+    """``[B, H, L, 128]`` view of a new token-major tensor."""
+    return torch.empty_strided((B, H, L, HEAD_DIM), (L * H * HEAD_DIM, HEAD_DIM, H * HEAD_DIM, 1), device=dev,
+                               dtype=BF16)
 
 
 def _cross_args(what: str, q, k, v, kv_lens):
-    dev = _one_device(what, q, k, v, kv_lens)
+    dev = _device_of(what, q, k, v, kv_lens)
     for n, t in (("q", q), ("k", k), ("v", v)):
-        if t.dtype != BF16:
+        if t.dtype is not BF16:
             raise ValueError(f"{what}: bf16 {n} required, got {t.dtype}")
         if t.dim() != 4 or t.shape[3] != HEAD_DIM:
             raise ValueError(f"{what}: {n} must be [B, H, L, 128], got {tuple(t.shape)}")
     B, H, Lq, _ = q.shape
-    Hkv, Lk = k.shape[1], k.shape[2]
-    if v.shape != k.shape or k.shape[0] != B:
+    Bk, Hkv, Lk, _ = k.shape
+    if v.shape != k.shape or Bk != B:
         raise ValueError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} must share a shape with q's batch {B}")
     if Hkv == 0 or H % Hkv:
         raise ValueError(f"{what}: {H} query heads are not a multiple of {Hkv} key heads")
-    if kv_lens is not None and (kv_lens.dtype != torch.int32 or tuple(kv_lens.shape) != (B,)):
-        raise ValueError(f"{what}: kv_lens must be int32 [{B}]")
-    return dev, (B, H, Hkv, Lq, Lk), None if kv_lens is None else kv_lens.contiguous()
+    if kv_lens is not None:
+        if kv_lens.dtype is not torch.int32 or kv_lens.shape != (B,):
+            raise ValueError(f"{what}: kv_lens must be int32 [{B}]")
+        kv_lens = kv_lens.contiguous()
+    return dev, (B, H, Hkv, Lq, Lk), kv_lens
 
 
 def cross_attention_fwd_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_lens: torch.Tensor | None = None,
@@ -946,19 +973,19 @@ def cross_attention_fwd_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k
     """``cross_attention`` and the rows' base-2 log-sum-exp ``[B*H, lse_rows(Lq)]``
     (fp32; +inf on padding rows and rows without keys), which
     ``cross_attention_bwd`` reads."""
-    what = "cross_attention"
-    dev, (B, H, Hkv, Lq, Lk), lens = _cross_args(what, q, k, v, kv_lens)
-    o = torch.empty(B, Lq, H, HEAD_DIM, device=dev, dtype=BF16).transpose(1, 2)
-    lse = torch.empty(B * H, lse_rows(Lq), device=dev, dtype=torch.float32) if need_lse else None
-    if o.numel() == 0:
+    dev, sizes, lens = _cross_args("cross_attention", q, k, v, kv_lens)
+    B, H, Hkv, Lq, Lk = sizes
+    o = _token_major_empty(B, H, Lq, q.device)
+    lse = torch.empty(B * H, lse_rows(Lq), device=q.device, dtype=torch.float32) if need_lse else None
+    if B == 0 or H == 0 or Lq == 0:
         return o, lse
     if Lk == 0:
         return o.zero_(), None if lse is None else lse.fill_(float("inf"))
-    q, k, v = _head_view(q), _head_view(k), _head_view(v)
-    nb = _lib.lib().rola_b200_cross_attn_workspace(B, H, Hkv, Lq, Lk)
-    ws = torch.empty(nb, device=dev, dtype=torch.uint8) if nb else None
-    _call_on(dev, "rola_b200_cross_attn", _ptr(q), *_head_strides(q), _ptr(k), *_head_strides(k), _ptr(v),
-             *_head_strides(v), _ptr(lens), B, H, Hkv, Lq, Lk, _ptr(o), *_head_strides(o), _ptr(lse), _ptr(ws), nb)
+    (q, qa), (k, ka), (v, va) = _head_args(q), _head_args(k), _head_args(v)
+    nb = _lib.lib().rola_b200_cross_attn_workspace(*sizes)
+    ws = torch.empty(nb, device=q.device, dtype=torch.uint8) if nb else None
+    _call_on(dev, "rola_b200_cross_attn", *qa, *ka, *va, _ptr(lens), *sizes, o.data_ptr(), Lq * H * HEAD_DIM, HEAD_DIM,
+             H * HEAD_DIM, _ptr(lse), _ptr(ws), nb)
     return o, lse
 
 
@@ -981,22 +1008,25 @@ def cross_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: to
     ``lse`` and ``do = dL/do``; dk and dv sum over the query heads of a key head.
     The same inputs give the same bits."""
     what = "cross_attention_bwd"
-    dev, (B, H, Hkv, Lq, Lk), lens = _cross_args(what, q, k, v, kv_lens)
-    _one_device(what, q, o, do, lse)
-    if o.shape != q.shape or do.shape != q.shape or o.dtype != BF16:
+    dev, sizes, lens = _cross_args(what, q, k, v, kv_lens)
+    B, H, Hkv, Lq, Lk = sizes
+    if _device_of(what, o, do, lse) != dev:
+        raise ValueError(f"{what}: o, do and lse must be on cuda:{dev}")
+    if o.shape != q.shape or do.shape != q.shape or o.dtype is not BF16:
         raise ValueError(f"{what}: o and do must have q's shape, o in bf16")
-    if lse.dtype != torch.float32 or tuple(lse.shape) != (B * H, lse_rows(Lq)) or not lse.is_contiguous():
+    if lse.dtype is not torch.float32 or lse.shape != (B * H, lse_rows(Lq)) or not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be the forward's")
-    dq = torch.empty(B, Lq, H, HEAD_DIM, device=dev, dtype=BF16).transpose(1, 2)
-    dk, dv = torch.empty(2, B, Lk, Hkv, HEAD_DIM, device=dev, dtype=BF16).transpose(2, 3)
+    dq = _token_major_empty(B, H, Lq, q.device)
+    dk, dv = _token_major_empty(B, Hkv, Lk, q.device), _token_major_empty(B, Hkv, Lk, q.device)
     if q.numel() == 0 or k.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    q, k, v, o, do = (_head_view(t) for t in (q, k, v, o, do.to(BF16)))
-    nb = _lib.lib().rola_b200_cross_attn_bwd_workspace(B, H, Hkv, Lq, Lk)
+    (q, qa), (k, ka), (v, va), (o, oa) = _head_args(q), _head_args(k), _head_args(v), _head_args(o)
+    do, da = _head_args(do if do.dtype is BF16 else do.to(BF16))
+    nb = _lib.lib().rola_b200_cross_attn_bwd_workspace(*sizes)
     if nb == 0:
         raise ValueError(f"{what}: bad sizes")
-    ws = torch.empty(nb, device=dev, dtype=torch.uint8)
-    _call_on(dev, "rola_b200_cross_attn_bwd", _ptr(q), *_head_strides(q), _ptr(k), *_head_strides(k), _ptr(v),
-             *_head_strides(v), _ptr(o), *_head_strides(o), _ptr(do), *_head_strides(do), _ptr(lens), _ptr(lse), B, H,
-             Hkv, Lq, Lk, _ptr(dq), *_head_strides(dq), _ptr(dk), _ptr(dv), *_head_strides(dk), _ptr(ws), nb)
+    ws = torch.empty(nb, device=q.device, dtype=torch.uint8)
+    _call_on(dev, "rola_b200_cross_attn_bwd", *qa, *ka, *va, *oa, *da, _ptr(lens), lse.data_ptr(), *sizes,
+             dq.data_ptr(), Lq * H * HEAD_DIM, HEAD_DIM, H * HEAD_DIM, dk.data_ptr(), dv.data_ptr(),
+             Lk * Hkv * HEAD_DIM, HEAD_DIM, Hkv * HEAD_DIM, ws.data_ptr(), nb)
     return dq, dk, dv

@@ -236,4 +236,5 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if not q.is_cuda:
         raise RuntimeError("the B200 training path runs on CUDA tensors only")
     dt = q.dtype
-    return CrossAttention.apply(*(t.to(torch.bfloat16) for t in (q, k, v)), kv_lens).to(dt)
+    o = CrossAttention.apply(*(t.to(torch.bfloat16) for t in (q, k, v)), kv_lens)
+    return o if dt == torch.bfloat16 else o.to(dt)
