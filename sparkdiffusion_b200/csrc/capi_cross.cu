@@ -178,9 +178,9 @@ int rola_b200_cross_attn(const void* q, int64_t q_sB, int64_t q_sH, int64_t q_sT
   p.out = BFm(out), p.o_sB = o_sB, p.o_sH = o_sH, p.o_sT = o_sT;
   p.lse = lse, p.lse_ld = 128 * ((Lq + 127) / 128);
   p.B = B, p.H = H, p.Hkv = Hkv, p.G = H / Hkv, p.Lq = Lq, p.Lk = Lk;
-  p.pack = pl.pack, p.nqt = pl.nqt, p.nqp = pl.nqp, p.nsplit = pl.nsplit;
+  p.pack = pl.pack, p.nqt = pl.nqt, p.nsplit = pl.nsplit;
   p.Hgrid = pl.pack ? Hkv : H;
-  p.items = (int64_t)pl.nqp * pl.nsplit * B * p.Hgrid;
+  p.items = (int64_t)pl.nqt * pl.nsplit * B * p.Hgrid;
   p.part_o = static_cast<float*>(workspace);
   p.part_lse = p.part_o ? p.part_o + (size_t)pl.nsplit * B * H * Lq * 128 : nullptr;
   p.q_bytes = pl.pack ? 256u * (uint32_t)(p.G * Lq) : 32768u;

@@ -9,21 +9,20 @@
 // then P and l share the older maximum (the quotient is the same, P is at most
 // 2^8 and rounds with the same relative error).
 //
-// Work items are (pair of 128-row query tiles, batch and head, slice of the
-// keys); persistent CTAs, one per SM, walk them.  An encoder's states are few
-// keys (512: four tiles), so an item is short and its ends must overlap its
-// neighbours: the tiles' S products of the next item are issued right behind the
-// last P V of this one, its Q tiles are loaded ahead through a ring of three,
-// and the correction warps store an item's output while the next item's softmax
-// runs.  Both query tiles of an item use each K and V tile once it is in shared
-// memory (half the L2 reads of one tile per K/V load).  Roles (512 threads,
-// registers split by setmaxnreg):
-//   warp 0          TMA producer: Q ring (3 x 32 KB), K/V ring (4 x 32 KB)
-//   warp 1          MMA issuer and TMEM owner: S = Q K^T (shared memory), O += P V
-//                   (P in TMEM over the S columns, in chunks of 32 keys).  It also
-//                   clears the V rows past len[b] (their P is 0, but 0 * NaN is not)
-//   warps 4-7, 8-11 softmax of tile 0 / 1, thread = row = TMEM lane
-//   warps 12-15     rescale O, then scale by 1/l and store
+// The work is a stream of units, one 128 x 128 tile of scores each: the key tiles
+// of an item (128 query rows of a head, or a slice of their keys), item after
+// item, on persistent CTAs, one per SM.  A unit is a chain, S = Q K^T -> softmax
+// -> O += P V, whose softmax takes longer than its products; what keeps the
+// tensor core busy is the number of units in flight.  Tensor memory holds three
+// S tiles beside one O, so there are three, each with a softmax warpgroup of its
+// own, and they run across the items' ends: an encoder's states are few keys (512:
+// four units), and the S products of the next item are issued while this one
+// finishes.  m and l pass from unit to unit through shared memory, in order.
+//   warp 0        TMA producer: Q tiles (2 x 32 KB) and a K/V ring (5 x 32 KB)
+//   warp 1        MMA issuer and TMEM owner.  It also clears the V rows past len[b]
+//                 (their P is 0, but 0 * NaN is not)
+//   warpgroup g = 1, 2, 3: the units u with u % 3 == g - 1; thread = row = TMEM lane.
+//                 The unit that ends an item scales its O by 1/l and stores it.
 // Few rows: the keys of an item are cut into slices, each leaves O/l in fp32 and
 // its log-sum-exp, and combine_kernel joins them.  When the G query heads of a
 // key head have 128 rows or fewer together, they form one tile (one read of K/V
@@ -36,27 +35,30 @@ namespace rola {
 namespace xattn {
 constexpr int THREADS = 512;
 constexpr int LAUNCH_REGS = 128;  // 65536 / 512
-constexpr int REGS_LOAD = 56, REGS_CORR = 96, REGS_SOFTMAX = 176;
-static_assert(128 * (REGS_LOAD + REGS_CORR + 2 * REGS_SOFTMAX) <= THREADS * LAUNCH_REGS, "register split");
+constexpr int REGS_LOAD = 56, REGS_SOFTMAX = 152;
+static_assert(128 * (REGS_LOAD + 3 * REGS_SOFTMAX) <= THREADS * LAUNCH_REGS, "register split");
 constexpr int BOX = 16384;        // [128 rows x 64 bf16], 128-byte swizzle
 constexpr int TILE = 2 * BOX;     // 128 rows x 128 columns
-constexpr int NQ = 3, NKV = 4;
+constexpr int NQ = 2, NKV = 5, NS = 3;
 constexpr int OFF_Q = 0;
 constexpr int OFF_KV = NQ * TILE;
-constexpr int OFF_ALPHA = OFF_KV + NKV * TILE;  // [2][128] rescale factors
-constexpr int OFF_L = OFF_ALPHA + 1024;         // [2][128] row sums
+constexpr int OFF_M = OFF_KV + NKV * TILE;  // [2][128] running maxima after even / odd units
+constexpr int OFF_L = OFF_M + 1024;         // [2][128] running sums
 constexpr int OFF_BAR = OFF_L + 1024;
 constexpr int SMEM = OFF_BAR + 512;
+constexpr int O_COL = 128 * NS;   // S of unit u at column 128 (u % 3), its P in the upper 64 of those; O behind them
 constexpr float RESCALE = 8.0f;   // log2 growth of the maximum that triggers a rescale of O
 enum : int {
   QF = 0, QE = QF + NQ, KF = QE + NQ, KE = KF + NKV,
-  SF = KE + NKV,   // S of tile t in TMEM
-  PF = SF + 2,     // P chunk c of tile t in TMEM: PF + 4 t + c, 4 warp arrivals
-  OF = PF + 8,     // O of tile t final
-  AR = OF + 2,     // rescale factors of tile t published (each step), 4 arrivals
-  LF = AR + 2,     // row sums of tile t published (end of item), 4 arrivals
-  OC = LF + 2,     // O of tile t may be accumulated into, 4 arrivals
-  DRAIN = OC + 2,
+  SF = KE + NKV,     // S of a unit in TMEM: SF + u % 3
+  PB = SF + NS,      // P of keys [64, 128) in TMEM, 4 warp arrivals
+  PA = PB + NS,      // P of keys [0, 64)
+  PV = PA + NS,      // P V of a unit done
+  MR = PV + NS,      // m after unit u published: MR + u % 3, 4 arrivals (a single barrier would not do: the unit
+                     // that waits may find it two phases behind, which parity cannot tell from done)
+  LR = MR + NS,      // l after unit u published, 4 arrivals
+  OE = LR + NS,      // O read by the item's epilogue (phase: item), 4 arrivals
+  DRAIN = OE + 1,
   COUNT
 };
 static_assert(8 * COUNT + 16 <= 512, "barrier region");
@@ -69,27 +71,33 @@ __device__ __forceinline__ int kv_len(const int32_t* lens, int b, int Lk) {
 }
 
 struct CrossItem {
-  int b, h, m0, nt, i0, cnt, split;  // h: head of the grid (key head when packed); key tiles [i0, i0 + cnt)
+  int b, h, m, i0, cnt, split;  // h: head of the grid (key head when packed); query tile m; key tiles [i0, i0 + cnt)
   int len;
 };
-__device__ __forceinline__ CrossItem cross_item(const CrossAttnParams& p, int64_t w) {
+__device__ __forceinline__ CrossItem cross_item(const CrossAttnParams& p, uint32_t w) {
   CrossItem it;
-  const int qp = (int)(w % p.nqp);
-  int64_t r = w / p.nqp;
-  it.split = (int)(r % p.nsplit);
-  r /= p.nsplit;
-  it.h = (int)(r % p.Hgrid);
-  it.b = (int)(r / p.Hgrid);
-  it.m0 = 2 * qp;
-  it.nt = min(2, p.nqt - it.m0);
+  uint32_t r = w / (uint32_t)p.nqt;
+  it.m = (int)(w - r * (uint32_t)p.nqt);
+  it.split = 0;
+  if (p.nsplit > 1) {
+    const uint32_t t = r / (uint32_t)p.nsplit;
+    it.split = (int)(r - t * (uint32_t)p.nsplit);
+    r = t;
+  }
+  it.b = (int)(r / (uint32_t)p.Hgrid);
+  it.h = (int)(r - (uint32_t)it.b * (uint32_t)p.Hgrid);
   it.len = kv_len(p.kv_lens, it.b, p.Lk);
-  const int n = (it.len + 127) / 128;
-  it.i0 = (int)((int64_t)n * it.split / p.nsplit);
-  it.cnt = (int)((int64_t)n * (it.split + 1) / p.nsplit) - it.i0;
+  const int n = (it.len + 127) >> 7;
+  it.i0 = 0;
+  it.cnt = n;
+  if (p.nsplit > 1) {
+    it.i0 = (int)((uint32_t)n * (uint32_t)it.split / (uint32_t)p.nsplit);
+    it.cnt = (int)((uint32_t)n * (uint32_t)(it.split + 1) / (uint32_t)p.nsplit) - it.i0;
+  }
   return it;
 }
-// row r of tile m -> head and token; false past the last row
-__device__ __forceinline__ bool cross_row(const CrossAttnParams& p, const CrossItem& it, int m, int r, int& h, int& t) {
+// row r of the item's tile -> head and token; false past the last row
+__device__ __forceinline__ bool cross_row(const CrossAttnParams& p, const CrossItem& it, int r, int& h, int& t) {
   if (p.pack) {
     const int g = r / p.Lq;
     h = it.h * p.G + g;
@@ -97,8 +105,42 @@ __device__ __forceinline__ bool cross_row(const CrossAttnParams& p, const CrossI
     return g < p.G;
   }
   h = it.h;
-  t = m * 128 + r;
+  t = it.m * 128 + r;
   return t < p.Lq;
+}
+
+// Walks the units of a CTA: the key tiles of its items that have any, in order
+struct CrossCursor {
+  uint32_t w;       // the item after this one
+  CrossItem it;
+  int i, u, j;      // key tile within the item, unit and item count of the CTA
+  bool live;
+};
+__device__ __forceinline__ void cursor_item(const CrossAttnParams& p, CrossCursor& c) {
+  c.live = false;
+  c.i = 0;
+  for (; c.w < (uint32_t)p.items; c.w += gridDim.x) {
+    c.it = cross_item(p, c.w);
+    if (c.it.cnt > 0) {
+      c.w += gridDim.x;
+      c.live = true;
+      return;
+    }
+  }
+}
+__device__ __forceinline__ CrossCursor cursor_first(const CrossAttnParams& p) {
+  CrossCursor c;
+  c.w = blockIdx.x;
+  c.u = c.j = 0;
+  cursor_item(p, c);
+  return c;
+}
+__device__ __forceinline__ void cursor_next(const CrossAttnParams& p, CrossCursor& c) {
+  ++c.u;
+  if (++c.i == c.it.cnt) {
+    ++c.j;
+    cursor_item(p, c);
+  }
 }
 
 // shared memory row r >= valid of a [128 x 128] V tile := 0 (whole 128-byte rows, so the swizzle does not matter)
@@ -111,6 +153,21 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int valid, int lane) {
   __syncwarp();
 }
 
+// 16 fp32 values -> bf16, one 32-byte store (a whole sector of the lane's row) where the row is 32-byte aligned
+__device__ __forceinline__ void store16_bf16(__nv_bfloat16* dst, const float* f, bool wide) {
+  uint32_t w[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = pack_bf2(f[2 * e], f[2 * e + 1]);
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  }
+}
+
 __global__ void __launch_bounds__(xattn::THREADS, 1)
     cross_attn_tcgen05(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                        const __grid_constant__ CUtensorMap tv, const CrossAttnParams p) {
@@ -120,10 +177,12 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
   auto bar = [&](int i) { return base + OFF_BAR + 8u * i; };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem1k + OFF_BAR + 8 * COUNT);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem1k + OFF_BAR + 8 * COUNT + 8);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // broadcast values are warp-uniform to the compiler too: the MMA warp's addresses and
+  // descriptors stay in uniform registers, which its instructions need
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < COUNT; ++i) mbar_init(bar(i), (i >= PF && i < OF) || (i >= AR && i < DRAIN) ? 4 : 1);
+    for (int i = 0; i < COUNT; ++i) mbar_init(bar(i), (i >= PB && i < PV) || (i >= MR && i < DRAIN) ? 4 : 1);
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tq);
@@ -137,364 +196,377 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  const uint32_t id_qk = idesc_bf16_f32(128, 128, false, false);
-  const uint32_t id_pv = idesc_bf16_f32(128, 128, false, true);
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_LOAD));
     if (warp == 0 && lane == 0) {
       // ------------------------------------------------------------ TMA
-      int rq = 0, r = 0;
+      // in the order the MMAs consume: K of units 0, 1, 2, then V(u), K(u + 3)
+      int r = 0, nq = 0;
       bool ok = true;
-      auto load_q = [&](const CrossItem& it, int t) {
-        const int e = rq % NQ;
-        if (!ok || !(ok = mbar_wait(bar(QE + e), ((rq / NQ) & 1) ^ 1, abort_flag, kDevTimeoutMma))) return;
-        const uint32_t dst = base + OFF_Q + e * TILE;
-        const int h = p.pack ? it.h * p.G : it.h;
-        mbar_expect_tx(bar(QF + e), p.q_bytes);
-        tma_load_4d(dst, &tq, bar(QF + e), 0, (it.m0 + t) * 128, h, it.b);
-        tma_load_4d(dst + BOX, &tq, bar(QF + e), 64, (it.m0 + t) * 128, h, it.b);
-        ++rq;
-      };
-      auto load_kv = [&](const CUtensorMap* m, const CrossItem& it, int i) {
+      auto load_kv = [&](const CUtensorMap* m, const CrossCursor& c) {
         const int e = r % NKV;
         if (!ok || !(ok = mbar_wait(bar(KE + e), ((r / NKV) & 1) ^ 1, abort_flag, kDevTimeoutMma))) return;
         const uint32_t dst = base + OFF_KV + e * TILE;
-        const int h = p.pack ? it.h : it.h / p.G;
+        const int h = p.pack ? c.it.h : c.it.h / p.G;
         mbar_expect_tx(bar(KF + e), TILE);
-        tma_load_4d(dst, m, bar(KF + e), 0, i * 128, h, it.b);
-        tma_load_4d(dst + BOX, m, bar(KF + e), 64, i * 128, h, it.b);
+        tma_load_4d(dst, m, bar(KF + e), 0, (c.it.i0 + c.i) * 128, h, c.it.b);
+        tma_load_4d(dst + BOX, m, bar(KF + e), 64, (c.it.i0 + c.i) * 128, h, c.it.b);
         ++r;
       };
-      for (int64_t w = blockIdx.x; w < p.items && ok; w += gridDim.x) {
-        const CrossItem it = cross_item(p, w);
-        if (it.cnt == 0) continue;
-        load_q(it, 0);
-        load_kv(&tk, it, it.i0);
-        if (it.nt == 2) load_q(it, 1);
-        for (int i = 0; i < it.cnt && ok; ++i) {
-          load_kv(&tv, it, it.i0 + i);
-          if (i + 1 < it.cnt) load_kv(&tk, it, it.i0 + i + 1);
+      CrossCursor ck = cursor_first(p), cv = ck;
+      auto load_k = [&] {
+        if (!ck.live) return;
+        if (ck.i == 0) {
+          const int e = ck.j % NQ;
+          if (!ok || !(ok = mbar_wait(bar(QE + e), ((ck.j / NQ) & 1) ^ 1, abort_flag, kDevTimeoutMma))) return;
+          const uint32_t dst = base + OFF_Q + e * TILE;
+          const int h = p.pack ? ck.it.h * p.G : ck.it.h;
+          mbar_expect_tx(bar(QF + e), p.q_bytes);
+          tma_load_4d(dst, &tq, bar(QF + e), 0, ck.it.m * 128, h, ck.it.b);
+          tma_load_4d(dst + BOX, &tq, bar(QF + e), 64, ck.it.m * 128, h, ck.it.b);
+          nq = ck.j + 1;
         }
+        load_kv(&tk, ck);
+        cursor_next(p, ck);
+      };
+      for (int n = 0; n < NS; ++n) load_k();
+      while (cv.live && ok) {
+        load_kv(&tv, cv);
+        cursor_next(p, cv);
+        load_k();
       }
       // no copy may still target shared memory when the CTA exits; the waits
       // ignore the abort flag and share one limit
       const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
       bool drained = true;
-      for (int n = max(0, rq - NQ); n < rq && drained; ++n)
+      for (int n = max(0, nq - NQ); n < nq && drained; ++n)
         drained = mbar_wait_until(bar(QF + n % NQ), (n / NQ) & 1, deadline);
       for (int n = max(0, r - NKV); n < r && drained; ++n)
         drained = mbar_wait_until(bar(KF + n % NKV), (n / NKV) & 1, deadline);
     } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA
-      // the whole warp follows the sequence (it clears V rows together); lane 0 issues
-      int rq = 0, r = 0;
-      int steps[2] = {0, 0};
+      // the whole warp follows the sequence (it clears V rows together); one elected
+      // lane issues.  S runs three units ahead of P V.
+      constexpr uint32_t id_qk = idesc_bf16_f32(128, 128, false, false);
+      constexpr uint32_t id_pv = idesc_bf16_f32(128, 128, false, true);
+      constexpr uint32_t hi = sdesc_hi(1024);
       bool ok = true;
       auto wait = [&](int i, uint32_t parity, int code) {
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(i), parity, abort_flag, code));
         tc_fence_after();
         return ok;
       };
-      auto next_item = [&](int64_t& w, CrossItem& it) {
-        for (; w < p.items; w += gridDim.x) {
-          it = cross_item(p, w);
-          if (it.cnt > 0) {
-            w += gridDim.x;
-            return true;
-          }
+      // key tiles of the next item that has any, from w on; 0 at the end
+      auto next_item = [&](uint32_t& w, int& left, int& tail) {
+        left = 0;
+        for (; w < (uint32_t)p.items && left == 0; w += gridDim.x) {
+          const CrossItem it = cross_item(p, w);
+          left = __shfl_sync(0xffffffffu, it.cnt, 0);
+          // valid keys of the item's last tile, where rows past them may hold anything
+          const int valid = it.len - (it.i0 + it.cnt - 1) * 128;
+          tail = __shfl_sync(0xffffffffu, it.len < p.Lk && valid < 128 ? valid : 128, 0);
         }
-        return false;
       };
-      // S_t = Q_t K^T with Q ring entry eq and K ring entry ek
-      auto issue_s = [&](int t, int eq, int ek, bool last_of_q, bool last_of_k) {
-        if (lane == 0) {
-          const uint32_t sq = base + OFF_Q + eq * TILE, sk = base + OFF_KV + ek * TILE;
+      int e = 0;          // ring entry consumed next, and its phase
+      uint32_t e_ph = 0;
+      auto pop = [&] {
+        if (++e == NKV) {
+          e = 0;
+          e_ph ^= 1u;
+        }
+      };
+      uint32_t ws = blockIdx.x, wv = blockIdx.x;
+      int s_left, s_tail, v_left, v_tail;
+      next_item(ws, s_left, s_tail);
+      next_item(wv, v_left, v_tail);
+      bool s_first = true, v_first = true;
+      int eq = 0, gs = 0, g = 0;
+      uint32_t q_ph = 0, g_ph = 0, o_ph = 1;
+      auto issue_s = [&] {  // S of the next unit
+        if (s_left == 0 || !ok) return;
+        if (s_first && !wait(QF + eq, q_ph, kDevTimeoutLoad)) return;
+        if (!wait(KF + e, e_ph, kDevTimeoutLoad)) return;
+        const bool last = s_left == 1;
+        if (elect_one()) {
+          const uint32_t dq = sdesc_lo(base + OFF_Q + eq * TILE, 16), dk = sdesc_lo(base + OFF_KV + e * TILE, 16);
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk) {
-            const uint32_t off = (kk >> 2) * BOX + (kk & 3) * 32;
-            mma_bf16_ss(tmem + 128 * t, sdesc_sw128(sq + off, 16, 1024), sdesc_sw128(sk + off, 16, 1024), id_qk,
-                        kk > 0 ? 1u : 0u);
+            const uint32_t off = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
+            mma_bf16_ss_lo(tmem + 128 * gs, dq + off, hi, dk + off, hi, id_qk, kk > 0 ? 1u : 0u);
           }
-          mma_commit(bar(SF + t));
-          if (last_of_q) mma_commit(bar(QE + eq));
-          if (last_of_k) mma_commit(bar(KE + ek));
+          mma_commit(bar(SF + gs));
+          mma_commit(bar(KE + e));
+          if (last) mma_commit(bar(QE + eq));
         }
         __syncwarp();
-      };
-      int64_t w = blockIdx.x;
-      CrossItem cur, nxt;
-      bool have = next_item(w, cur);
-      int eq[2] = {0, 0}, eq_next[2] = {0, 0}, ek = 0;
-      auto open_item = [&](const CrossItem& it, int t) {  // S_t(0) of an item: its Q tile, and its first K tile once
-        if (t == 0) {
-          ek = r % NKV;
-          if (!wait(KF + ek, (r / NKV) & 1, kDevTimeoutLoad)) return;
-          ++r;
+        pop();
+        gs = gs == NS - 1 ? 0 : gs + 1;
+        s_first = last;
+        if (last) {
+          if (++eq == NQ) {
+            eq = 0;
+            q_ph ^= 1u;
+          }
+          next_item(ws, s_left, s_tail);
+        } else {
+          --s_left;
         }
-        eq_next[t] = rq % NQ;
-        if (!wait(QF + eq_next[t], (rq / NQ) & 1, kDevTimeoutLoad)) return;
-        ++rq;
-        issue_s(t, eq_next[t], ek, it.cnt == 1, t == it.nt - 1);
       };
-      if (have)
-        for (int t = 0; t < cur.nt && ok; ++t) open_item(cur, t);
-      while (have && ok) {
-        eq[0] = eq_next[0], eq[1] = eq_next[1];
-        const bool more = next_item(w, nxt);
-        for (int i = 0; i < cur.cnt && ok; ++i) {
-          const bool last = i + 1 == cur.cnt;
-          const int ev = r % NKV;
-          if (!wait(KF + ev, (r / NKV) & 1, kDevTimeoutLoad)) break;
-          ++r;
-          const int valid = cur.len - (cur.i0 + i) * 128;
-          if (valid < 128 && cur.len < p.Lk) clear_rows(smem1k + OFF_KV + ev * TILE, valid, lane);
-          const uint32_t sv = base + OFF_KV + ev * TILE;
-          for (int t = 0; t < cur.nt && ok; ++t) {
-            const uint32_t ph = steps[t] & 1;
-            if (!wait(OC + t, ph, kDevTimeoutSoftmax)) break;
-            for (int c = 0; c < 4 && ok; ++c) {
-              if (!wait(PF + 4 * t + c, ph, kDevTimeoutSoftmax)) break;
-              if (lane == 0) {
+      for (int n = 0; n < NS; ++n) issue_s();
+      while (v_left > 0 && ok) {
+        const bool last = v_left == 1;
+        if (!wait(KF + e, e_ph, kDevTimeoutLoad)) break;
+        if (last && v_tail < 128) clear_rows(smem1k + OFF_KV + e * TILE, v_tail, lane);
+        // O of the previous item has been read
+        if (v_first && !wait(OE, o_ph, kDevTimeoutSoftmax)) break;
+        const uint32_t dv = sdesc_lo(base + OFF_KV + e * TILE, BOX), tp = tmem + 128 * g + 64;
 #pragma unroll
-                for (int k2 = 0; k2 < 2; ++k2) {
-                  const int kk = 2 * c + k2;
-                  mma_bf16_ts(tmem + 256 + 128 * t, tmem + 128 * t + kk * 8, sdesc_sw128(sv + kk * 2048, BOX, 1024),
-                              id_pv, (i > 0 || kk > 0) ? 1u : 0u);
-                }
-              }
-              __syncwarp();
+        for (int half = 1; half >= 0; --half) {  // keys [64, 128) first, as the softmax hands them over
+          if (!wait((half ? PB : PA) + g, g_ph, kDevTimeoutSoftmax)) break;
+          if (elect_one()) {
+#pragma unroll
+            for (int k4 = 0; k4 < 4; ++k4) {
+              const int kk = 4 * half + k4;
+              mma_bf16_ts_lo(tmem + O_COL, tp + 8 * kk, dv + ((kk * 2048) >> 4), hi, id_pv,
+                             (!v_first || half == 0 || k4 > 0) ? 1u : 0u);
             }
-            if (!ok) break;
-            ++steps[t];
-            if (lane == 0) {
-              if (t == cur.nt - 1) mma_commit(bar(KE + ev));
-              if (last) mma_commit(bar(OF + t));
-            }
-            __syncwarp();
-            if (!last) {
-              if (t == 0) {
-                ek = r % NKV;
-                if (!wait(KF + ek, (r / NKV) & 1, kDevTimeoutLoad)) break;
-                ++r;
-              }
-              issue_s(t, eq[t], ek, i + 2 == cur.cnt, t == cur.nt - 1);
-            } else if (more && t < nxt.nt) {
-              open_item(nxt, t);
+            if (half == 0) {
+              mma_commit(bar(KE + e));
+              mma_commit(bar(PV + g));
             }
           }
+          __syncwarp();
         }
-        if (ok && more && nxt.nt > cur.nt) open_item(nxt, 1);
-        have = more;
-        cur = nxt;
+        if (!ok) break;
+        pop();
+        issue_s();  // into the buffer whose P V was just issued
+        if (++g == NS) {
+          g = 0;
+          g_ph ^= 1u;
+        }
+        v_first = last;
+        if (last) {
+          o_ph ^= 1u;
+          next_item(wv, v_left, v_tail);
+        } else {
+          --v_left;
+        }
       }
       // every MMA issued has completed before TMEM is freed, also on the abort path
-      if (lane == 0) {
+      if (elect_one()) {
         mma_commit(bar(DRAIN));
         mbar_wait_until(bar(DRAIN), 0, globaltimer_ns() + kWaitLimitNs);
       }
       __syncwarp();
     }
-  } else if (warp >= 12) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_CORR));
-    // --------------------------------------------------- correction and output
-    const int q = warp & 3, row = q * 32 + lane;
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    // ------------------------------------------------------- softmax and output
+    const int g = (warp >> 2) - 1, q = warp & 3, row = q * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q * 32) << 16;
-    const float* s_alpha = reinterpret_cast<const float*>(smem1k + OFF_ALPHA);
-    const float* s_l = reinterpret_cast<const float*>(smem1k + OFF_L);
-    int pub[2] = {0, 0}, fin[2] = {0, 0};  // phases of AR, and of LF and OF, passed
+    const uint32_t tS = tmem + 128 * g + lane_off, tO = tmem + O_COL + lane_off;
+    float* s_m = reinterpret_cast<float*>(smem1k + OFF_M) + row;
+    float* s_l = reinterpret_cast<float*>(smem1k + OFF_L) + row;
+    const float scale = p.qk_scale;
+    const bool wide = ((reinterpret_cast<uintptr_t>(p.out) >> 1) | p.o_sB | p.o_sH | p.o_sT) % 16 == 0;
     bool ok = true;
-    // output of a row of item `it`: v = O / l (zeros for an item without keys)
-    auto out_row = [&](const CrossItem& it, int t, float inv_l, bool zero) {
-      int h, tok;
-      const bool live = cross_row(p, it, it.m0 + t, row, h, tok);
-      const uint32_t tO = tmem + 256 + 128 * t + lane_off;
-      const int64_t prow = p.nsplit > 1 ? (((int64_t)it.split * p.B + it.b) * p.H + h) * p.Lq + tok : 0;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t v[32];
-        if (!zero) {
-          __syncwarp();  // the stores below diverge, the load is warp-collective
-          tmem_ld32(tO + 32 * c, v);
-          tmem_ld_wait();
-        }
-        float f[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) f[e] = zero ? 0.f : __uint_as_float(v[e]) * inv_l;
-        if (live && p.nsplit > 1) {
-          if (!zero) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + prow * 128 + 32 * c);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
-          }
-        } else if (live) {
-          uint4* dst = reinterpret_cast<uint4*>(p.out + it.b * p.o_sB + h * p.o_sH + tok * p.o_sT + 32 * c);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            dst[e] = make_uint4(pack_bf2(f[8 * e], f[8 * e + 1]), pack_bf2(f[8 * e + 2], f[8 * e + 3]),
-                                pack_bf2(f[8 * e + 4], f[8 * e + 5]), pack_bf2(f[8 * e + 6], f[8 * e + 7]));
-        }
-      }
-    };
     auto wait = [&](int i, uint32_t parity, int code) {
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(i), parity, abort_flag, code));
       return ok;
     };
-    CrossItem prev;
-    prev.nt = 0;
-    auto finish = [&](int t) {  // the previous item's tile t
-      if (t >= prev.nt || !ok) return;
-      if (!wait(LF + t, fin[t] & 1, kDevTimeoutSoftmax)) return;
-      const float inv_l = 1.0f / s_l[t * 128 + row];
-      if (!wait(OF + t, fin[t] & 1, kDevTimeoutMma)) return;
-      ++fin[t];
-      tc_fence_after();
-      out_row(prev, t, inv_l, false);
-    };
-    for (int64_t w = blockIdx.x; w < p.items && ok; w += gridDim.x) {
+    int u = 0, items = 0;
+    for (uint32_t w = blockIdx.x; w < (uint32_t)p.items && ok; w += gridDim.x) {
       const CrossItem it = cross_item(p, w);
       if (it.cnt == 0) {
-        for (int t = 0; t < it.nt; ++t) {
-          out_row(it, t, 0.f, true);
+        // no keys: zeros (one warpgroup in turn; no unit, nothing to wait for)
+        if (items % 3 == g) {
           int h, tok;
-          const bool live = cross_row(p, it, it.m0 + t, row, h, tok);
+          const bool live = cross_row(p, it, row, h, tok);
           if (p.nsplit > 1) {
             if (live) p.part_lse[(((int64_t)it.split * p.B + it.b) * p.H + h) * p.Lq + tok] = -INFINITY;
-          } else if (p.lse && (live || !p.pack)) {
-            p.lse[((int64_t)it.b * p.H + h) * p.lse_ld + tok] = INFINITY;
+          } else {
+            if (live) {
+              uint4* dst = reinterpret_cast<uint4*>(p.out + it.b * p.o_sB + h * p.o_sH + tok * p.o_sT);
+#pragma unroll
+              for (int c = 0; c < 16; ++c) dst[c] = make_uint4(0u, 0u, 0u, 0u);
+            }
+            if (p.lse && (live || !p.pack)) p.lse[((int64_t)it.b * p.H + h) * p.lse_ld + tok] = INFINITY;
           }
         }
+        ++items;
         continue;
       }
-      for (int i = 0; i < it.cnt && ok; ++i) {
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (i == 0) finish(t);
-          if (t >= it.nt || !wait(AR + t, pub[t] & 1, kDevTimeoutSoftmax)) continue;
-          ++pub[t];
-          const float alpha = s_alpha[t * 128 + row];
-          if (i > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-            tc_fence_after();
-            const uint32_t tO = tmem + 256 + 128 * t + lane_off;
-            const uint64_t a2 = f2_pack(alpha, alpha);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t ov[32];
-              tmem_ld32(tO + 32 * c, ov);
-              tmem_ld_wait();
-#pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                float o0, o1;
-                f2_unpack(mul_f32x2(f2_pack(__uint_as_float(ov[2 * e]), __uint_as_float(ov[2 * e + 1])), a2), o0, o1);
-                ov[2 * e] = __float_as_uint(o0);
-                ov[2 * e + 1] = __float_as_uint(o1);
-              }
-              tmem_st32(tO + 32 * c, ov);
-            }
-            tmem_st_wait();
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(OC + t));
-        }
-      }
-      prev = it;
-    }
-    for (int t = 0; t < 2; ++t) finish(t);
-  } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
-    // -------------------------------------------------------------- softmax
-    const int t = (warp - 4) >> 2, q = warp & 3, row = q * 32 + lane;
-    const uint32_t tS = tmem + 128 * t + ((uint32_t)(q * 32) << 16);
-    float* s_alpha = reinterpret_cast<float*>(smem1k + OFF_ALPHA) + t * 128 + row;
-    float* s_l = reinterpret_cast<float*>(smem1k + OFF_L) + t * 128 + row;
-    const float scale = p.qk_scale;
-    int steps = 0;
-    bool ok = true;
-    for (int64_t w = blockIdx.x; w < p.items && ok; w += gridDim.x) {
-      const CrossItem it = cross_item(p, w);
-      if (it.cnt == 0 || t >= it.nt) continue;
-      float m_run = 0.f, l_run = 0.f;
-      for (int i = 0; i < it.cnt; ++i, ++steps) {
-        ok = __all_sync(0xffffffffu, mbar_wait(bar(SF + t), steps & 1, abort_flag, kDevTimeoutMma));
-        if (!ok) break;
+      for (int i = 0; i < it.cnt && ok; ++i, ++u) {
+        if (u % NS != g) continue;
+        const uint32_t ph = (u / NS) & 1;
+        if (!wait(SF + g, ph, kDevTimeoutMma)) break;
         tc_fence_after();
-        uint32_t v[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&v[c * 32]));
-        tmem_ld_wait();
+        // maximum of the row; the upper 64 scores stay in registers (P takes their
+        // place in TMEM), the lower 64 are read again for the exponentials
         const int valid = it.len - (it.i0 + i) * 128;
-        if (valid < 128) {
+        uint32_t hi[64];
+        float mx;
+        {
+          uint32_t lo[64];
+          tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&lo[0]));
+          tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&lo[32]));
+          tmem_ld_wait();
+          if (valid < 64) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (c >= valid) v[c] = __float_as_uint(-INFINITY);
-        }
-        float mx8[8];
+            for (int c = 0; c < 64; ++c)
+              if (c >= valid) lo[c] = __float_as_uint(-INFINITY);
+          }
+          float m4[4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          mx8[k] = __uint_as_float(v[k]);
+          for (int k = 0; k < 4; ++k) {
+            m4[k] = __uint_as_float(lo[k]);
 #pragma unroll
-          for (int j = 0; j < 7; ++j)
-            mx8[k] = max3f(mx8[k], __uint_as_float(v[k + 8 + 16 * j]), __uint_as_float(v[k + 16 + 16 * j]));
-          mx8[k] = fmaxf(mx8[k], __uint_as_float(v[k + 120]));
+            for (int e = 0; e < 7; ++e)
+              m4[k] = max3f(m4[k], __uint_as_float(lo[k + 4 + 8 * e]), __uint_as_float(lo[k + 8 + 8 * e]));
+            m4[k] = fmaxf(m4[k], __uint_as_float(lo[k + 60]));
+          }
+          tmem_ld32(tS + 64, *reinterpret_cast<uint32_t(*)[32]>(&hi[0]));
+          tmem_ld32(tS + 96, *reinterpret_cast<uint32_t(*)[32]>(&hi[32]));
+          tmem_ld_wait();
+          if (valid < 128) {
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (64 + c >= valid) hi[c] = __float_as_uint(-INFINITY);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              m4[k] = max3f(m4[k], __uint_as_float(hi[k + 8 * e]), __uint_as_float(hi[k + 4 + 8 * e]));
+          }
+          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         }
-        const float mx = max3f(fmaxf(mx8[0], mx8[1]), max3f(mx8[2], mx8[3], mx8[4]), max3f(mx8[5], mx8[6], mx8[7]));
-        const float m_new = mx * scale;
-        float alpha = 1.f;
-        if (i == 0) {
-          m_run = fmaxf(m_new, -FLT_MAX);  // finite, should every score of the tile be -inf
-        } else if (m_new - m_run > RESCALE) {
-          alpha = ex2_approx(m_run - m_new);
-          m_run = m_new;
+        // m after this unit, from the unit before (published in unit order)
+        float m = fmaxf(mx * scale, -FLT_MAX), alpha = 1.f;  // finite, should every score be -inf
+        if (u > 0 && !wait(MR + (u + NS - 1) % NS, ((u - 1) / NS) & 1, kDevTimeoutSoftmax)) break;
+        if (i > 0) {
+          const float m_prev = s_m[128 * ((u & 1) ^ 1)];
+          if (m - m_prev > RESCALE) {
+            alpha = ex2_approx(m_prev - m);
+          } else {
+            m = m_prev;
+          }
         }
-        *s_alpha = alpha;
+        s_m[128 * (u & 1)] = m;
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(AR + t));
-        const uint64_t sc2 = f2_pack(scale, scale), nm2 = f2_pack(-m_run, -m_run);
-        uint64_t rs2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-        auto publish_p = [&](int c) {
-          tmem_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar(PF + 4 * t + c));
-        };
+        if (lane == 0) mbar_arrive(bar(MR + g));
+        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+          // O of the units before, once the last of them is in
+          if (!wait(PV + (u + NS - 1) % NS, ((u - 1) / NS) & 1, kDevTimeoutMma)) break;
+          tc_fence_after();
+          const uint64_t a2 = f2_pack(alpha, alpha);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+          for (int c = 0; c < 4; ++c) {
+            uint32_t ov[32];
+            tmem_ld32(tO + 32 * c, ov);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              float o0, o1;
+              f2_unpack(mul_f32x2(f2_pack(__uint_as_float(ov[2 * e]), __uint_as_float(ov[2 * e + 1])), a2), o0, o1);
+              ov[2 * e] = __float_as_uint(o0);
+              ov[2 * e + 1] = __float_as_uint(o1);
+            }
+            tmem_st32(tO + 32 * c, ov);
+          }
+          tmem_st_wait();
+        }
+        const uint64_t sc2 = f2_pack(scale, scale), nm2 = f2_pack(-m, -m);
+        uint64_t rs2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+        // P of 32 keys, packed bf16, over 16 columns of the upper half of S
+        auto exp32 = [&](const uint32_t* v, int c) {
           uint32_t pw[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float x0, x1;
-            f2_unpack(fma_f32x2(f2_pack(__uint_as_float(v[32 * c + 2 * e]), __uint_as_float(v[32 * c + 2 * e + 1])),
-                                sc2, nm2),
-                      x0, x1);
+            f2_unpack(fma_f32x2(f2_pack(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sc2, nm2), x0, x1);
             const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
             rs2[e & 1] = add_f32x2(rs2[e & 1], f2_pack(p0, p1));
             pw[e] = pack_bf2(p0, p1);
           }
-          if (c > 0) publish_p(c - 1);
-          tmem_st16(tS + c * 16, pw);
+          tmem_st16(tS + 64 + 16 * c, pw);
+        };
+        auto publish = [&](int b) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(b + g));
+        };
+        exp32(hi, 2);
+        exp32(hi + 32, 3);
+        {
+          uint32_t lo[64];
+          tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&lo[0]));
+          tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&lo[32]));
+          publish(PB);
+          tmem_ld_wait();
+          if (valid < 64) {
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (c >= valid) lo[c] = __float_as_uint(-INFINITY);
+          }
+          exp32(lo, 0);
+          exp32(lo + 32, 1);
+          publish(PA);
         }
-        publish_p(3);
         float ra, rb, rc, rd;
         f2_unpack(rs2[0], ra, rb);
         f2_unpack(rs2[1], rc, rd);
-        l_run = l_run * alpha + ((ra + rc) + (rb + rd));
+        float l = (ra + rc) + (rb + rd);
+        if (u > 0 && !wait(LR + (u + NS - 1) % NS, ((u - 1) / NS) & 1, kDevTimeoutSoftmax)) break;
+        if (i > 0) l = fmaf(s_l[128 * ((u & 1) ^ 1)], alpha, l);
+        s_l[128 * (u & 1)] = l;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(LR + g));
+        if (i + 1 < it.cnt) continue;
+
+        // ------------------------------------------------- the item's output
+        int h, tok;
+        const bool live = cross_row(p, it, row, h, tok);
+        const float inv_l = 1.0f / l, lse = m + log2f(l);
+        if (!wait(PV + g, ph, kDevTimeoutMma)) break;
+        tc_fence_after();
+        const int64_t prow = (((int64_t)it.split * p.B + it.b) * p.H + h) * p.Lq + tok;
+        __nv_bfloat16* dst = p.out + it.b * p.o_sB + h * p.o_sH + tok * p.o_sT;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[64];
+          __syncwarp();  // the stores below diverge, the load is warp-collective
+          tmem_ld32(tO + 64 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+          tmem_ld32(tO + 64 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+          tmem_ld_wait();
+          if (c == 1) {
+            // O is in registers: the next item may start its own
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(OE));
+          }
+          float f[64];
+#pragma unroll
+          for (int e = 0; e < 64; ++e) f[e] = __uint_as_float(v[e]) * inv_l;
+          if (live && p.nsplit > 1) {
+            float4* d4 = reinterpret_cast<float4*>(p.part_o + prow * 128 + 64 * c);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) d4[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
+          } else if (live) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store16_bf16(dst + 64 * c + 16 * e, f + 16 * e, wide);
+          }
+        }
+        if (p.nsplit > 1) {
+          if (live) p.part_lse[prow] = lse;
+        } else if (p.lse && (live || !p.pack)) {
+          p.lse[((int64_t)it.b * p.H + h) * p.lse_ld + tok] = live ? lse : INFINITY;
+        }
       }
-      // the correction warps have taken this item's last factors, hence the previous
-      // item's row sums too: a one-step item could otherwise overtake them
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(OC + t), (steps - 1) & 1, abort_flag, kDevTimeoutSoftmax));
-      if (!ok) break;
-      *s_l = l_run;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(LF + t));
-      int h, tok;
-      const bool live = cross_row(p, it, it.m0 + t, row, h, tok);
-      const float lse = m_run + log2f(l_run);
-      if (p.nsplit > 1) {
-        if (live) p.part_lse[(((int64_t)it.split * p.B + it.b) * p.H + h) * p.Lq + tok] = lse;
-      } else if (p.lse && (live || !p.pack)) {
-        p.lse[((int64_t)it.b * p.H + h) * p.lse_ld + tok] = live ? lse : INFINITY;
-      }
+      ++items;
     }
   }
   tc_fence_before();
@@ -550,8 +622,7 @@ CrossAttnPlan cross_attn_plan(int B, int H, int Hkv, int Lq, int Lk) {
   const int G = H / Hkv;
   pl.pack = G > 1 && (int64_t)G * Lq <= 128;
   pl.nqt = pl.pack ? 1 : (Lq + 127) / 128;
-  pl.nqp = (pl.nqt + 1) / 2;
-  const int64_t items = (int64_t)pl.nqp * B * (pl.pack ? Hkv : H);
+  const int64_t items = (int64_t)pl.nqt * B * (pl.pack ? Hkv : H);
   const int ntk = (Lk + 127) / 128, sms = device_sms();
   pl.nsplit = 1;
   if (items < sms && ntk >= 4) {

@@ -231,7 +231,7 @@ int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBl
 // cross_attn.cu -----------------------------------------------------------
 struct CrossAttnPlan {
   bool pack;     // the G query heads of a key head share one tile (G * Lq <= 128)
-  int nqt, nqp;  // 128-row query tiles and pairs of them, per (b, head of the grid)
+  int nqt;       // 128-row query tiles per (b, head of the grid)
   int nsplit;    // slices of the keys
 };
 CrossAttnPlan cross_attn_plan(int B, int H, int Hkv, int Lq, int Lk);
@@ -242,10 +242,10 @@ struct CrossAttnParams {
   float* lse;              // [B*H, lse_ld] base-2 log-sum-exp (+inf: padding, rows without keys), or nullptr
   float* part_o;           // nsplit > 1: [nsplit, B*H, Lq, 128] and [nsplit, B*H, Lq]
   float* part_lse;
-  int64_t items;           // nqp * nsplit * B * Hgrid
+  int64_t items;           // nqt * nsplit * B * Hgrid
   int B, H, Hkv, G, Lq, Lk;
   int Hgrid;               // Hkv when packed, else H
-  int pack, nqt, nqp, nsplit, lse_ld;
+  int pack, nqt, nsplit, lse_ld;
   uint32_t q_bytes;        // bytes of one Q tile load
   float qk_scale;          // D^-1/2 * log2(e)
 };
