@@ -18,9 +18,12 @@
 // own, and they run across the items' ends: an encoder's states are few keys (512:
 // four units), and the S products of the next item are issued while this one
 // finishes.  m and l pass from unit to unit through shared memory, in order.
-//   warp 0        TMA producer: Q tiles (2 x 32 KB) and a K/V ring (5 x 32 KB)
-//   warp 1        MMA issuer and TMEM owner.  It also clears the V rows past len[b]
-//                 (their P is 0, but 0 * NaN is not)
+//   warp 0        TMA producer of Q (2 x 32 KB) and K tiles (2 x 32 KB)
+//   warp 3        TMA producer of V tiles (3 x 32 KB)
+//   warp 1        issues S; owner of the tensor memory
+//   warp 2        issues P V.  It also clears the V rows past len[b] (their P is 0,
+//                 but 0 * NaN is not).  One warp for both products was the limit:
+//                 2150 clocks a unit to issue what takes the tensor core 1024
 //   warpgroup g = 1, 2, 3: the units u with u % 3 == g - 1; thread = row = TMEM lane.
 //                 The unit that ends an item scales its O by 1/l and stores it.
 // Few rows: the keys of an item are cut into slices, each leaves O/l in fp32 and
@@ -39,26 +42,27 @@ constexpr int REGS_LOAD = 56, REGS_SOFTMAX = 152;
 static_assert(128 * (REGS_LOAD + 3 * REGS_SOFTMAX) <= THREADS * LAUNCH_REGS, "register split");
 constexpr int BOX = 16384;        // [128 rows x 64 bf16], 128-byte swizzle
 constexpr int TILE = 2 * BOX;     // 128 rows x 128 columns
-constexpr int NQ = 2, NKV = 5, NS = 3;
+constexpr int NQ = 2, NK = 2, NV = 3, NS = 3;
 constexpr int OFF_Q = 0;
-constexpr int OFF_KV = NQ * TILE;
-constexpr int OFF_M = OFF_KV + NKV * TILE;  // [2][128] running maxima after even / odd units
+constexpr int OFF_K = NQ * TILE, OFF_V = OFF_K + NK * TILE;
+constexpr int OFF_M = OFF_V + NV * TILE;  // [2][128] running maxima after even / odd units
 constexpr int OFF_L = OFF_M + 1024;         // [2][128] running sums
 constexpr int OFF_BAR = OFF_L + 1024;
 constexpr int SMEM = OFF_BAR + 512;
 constexpr int O_COL = 128 * NS;   // S of unit u at column 128 (u % 3), its P in the upper 64 of those; O behind them
 constexpr float RESCALE = 8.0f;   // log2 growth of the maximum that triggers a rescale of O
 enum : int {
-  QF = 0, QE = QF + NQ, KF = QE + NQ, KE = KF + NKV,
-  SF = KE + NKV,     // S of a unit in TMEM: SF + u % 3
+  QF = 0, QE = QF + NQ, KF = QE + NQ, KE = KF + NK, VF = KE + NK, VE = VF + NV,
+  SF = VE + NV,      // S of a unit in TMEM: SF + u % 3
   PB = SF + NS,      // P of keys [64, 128) in TMEM, 4 warp arrivals
   PA = PB + NS,      // P of keys [0, 64)
-  PV = PA + NS,      // P V of a unit done
+  PV = PA + NS,      // P V of a unit done (its S columns are free, O holds it)
   MR = PV + NS,      // m after unit u published: MR + u % 3, 4 arrivals (a single barrier would not do: the unit
                      // that waits may find it two phases behind, which parity cannot tell from done)
   LR = MR + NS,      // l after unit u published, 4 arrivals
   OE = LR + NS,      // O read by the item's epilogue (phase: item), 4 arrivals
-  DRAIN = OE + 1,
+  DRAIN_S = OE + 1,
+  DRAIN_P,
   COUNT
 };
 static_assert(8 * COUNT + 16 <= 512, "barrier region");
@@ -70,78 +74,68 @@ __device__ __forceinline__ int kv_len(const int32_t* lens, int b, int Lk) {
   return lens ? min(max(lens[b], 0), Lk) : Lk;
 }
 
-struct CrossItem {
-  int b, h, m, i0, cnt, split;  // h: head of the grid (key head when packed); query tile m; key tiles [i0, i0 + cnt)
-  int len;
-};
-__device__ __forceinline__ CrossItem cross_item(const CrossAttnParams& p, uint32_t w) {
-  CrossItem it;
-  uint32_t r = w / (uint32_t)p.nqt;
-  it.m = (int)(w - r * (uint32_t)p.nqt);
-  it.split = 0;
-  if (p.nsplit > 1) {
-    const uint32_t t = r / (uint32_t)p.nsplit;
-    it.split = (int)(r - t * (uint32_t)p.nsplit);
-    r = t;
-  }
-  it.b = (int)(r / (uint32_t)p.Hgrid);
-  it.h = (int)(r - (uint32_t)it.b * (uint32_t)p.Hgrid);
-  it.len = kv_len(p.kv_lens, it.b, p.Lk);
-  const int n = (it.len + 127) >> 7;
-  it.i0 = 0;
-  it.cnt = n;
-  if (p.nsplit > 1) {
-    it.i0 = (int)((uint32_t)n * (uint32_t)it.split / (uint32_t)p.nsplit);
-    it.cnt = (int)((uint32_t)n * (uint32_t)(it.split + 1) / (uint32_t)p.nsplit) - it.i0;
-  }
-  return it;
-}
-// row r of the item's tile -> head and token; false past the last row
-__device__ __forceinline__ bool cross_row(const CrossAttnParams& p, const CrossItem& it, int r, int& h, int& t) {
-  if (p.pack) {
-    const int g = r / p.Lq;
-    h = it.h * p.G + g;
-    t = r - g * p.Lq;
-    return g < p.G;
-  }
-  h = it.h;
-  t = it.m * 128 + r;
-  return t < p.Lq;
-}
+// Walks the items of a CTA, w = blockIdx.x, + gridDim.x, ...: query tile m
+// fastest, then the slice, the head of the grid (key head when packed), the
+// batch.  The digits are advanced by the step's own digits with carries; a
+// division per item cost each role about 2500 clocks.
+struct CrossItems {
+  uint32_t w;
+  int m, split, h, b;
+  int dm, ds, dh, db;
+  int len, i0, cnt;  // valid keys; key tiles [i0, i0 + cnt) of the item
 
-// Walks the units of a CTA: the key tiles of its items that have any, in order
-struct CrossCursor {
-  uint32_t w;       // the item after this one
-  CrossItem it;
-  int i, u, j;      // key tile within the item, unit and item count of the CTA
-  bool live;
-};
-__device__ __forceinline__ void cursor_item(const CrossAttnParams& p, CrossCursor& c) {
-  c.live = false;
-  c.i = 0;
-  for (; c.w < (uint32_t)p.items; c.w += gridDim.x) {
-    c.it = cross_item(p, c.w);
-    if (c.it.cnt > 0) {
-      c.w += gridDim.x;
-      c.live = true;
-      return;
+  __device__ __forceinline__ static void digits(const CrossAttnParams& p, uint32_t w, int& m, int& s, int& h, int& b) {
+    uint32_t r = w / (uint32_t)p.nqt;
+    m = (int)(w - r * (uint32_t)p.nqt);
+    uint32_t t = r / (uint32_t)p.nsplit;
+    s = (int)(r - t * (uint32_t)p.nsplit);
+    b = (int)(t / (uint32_t)p.Hgrid);
+    h = (int)(t - (uint32_t)b * (uint32_t)p.Hgrid);
+  }
+  __device__ __forceinline__ void range(const CrossAttnParams& p) {
+    if (w >= (uint32_t)p.items) return;
+    len = kv_len(p.kv_lens, b, p.Lk);
+    const int n = (len + 127) >> 7;
+    i0 = 0;
+    cnt = n;
+    if (p.nsplit > 1) {
+      i0 = (int)((uint32_t)n * (uint32_t)split / (uint32_t)p.nsplit);
+      cnt = (int)((uint32_t)n * (uint32_t)(split + 1) / (uint32_t)p.nsplit) - i0;
     }
   }
-}
-__device__ __forceinline__ CrossCursor cursor_first(const CrossAttnParams& p) {
-  CrossCursor c;
-  c.w = blockIdx.x;
-  c.u = c.j = 0;
-  cursor_item(p, c);
-  return c;
-}
-__device__ __forceinline__ void cursor_next(const CrossAttnParams& p, CrossCursor& c) {
-  ++c.u;
-  if (++c.i == c.it.cnt) {
-    ++c.j;
-    cursor_item(p, c);
+  __device__ __forceinline__ explicit CrossItems(const CrossAttnParams& p) : w(blockIdx.x) {
+    digits(p, w, m, split, h, b);
+    digits(p, gridDim.x, dm, ds, dh, db);
+    range(p);
   }
-}
+  __device__ __forceinline__ bool live(const CrossAttnParams& p) const { return w < (uint32_t)p.items; }
+  __device__ __forceinline__ void next(const CrossAttnParams& p) {
+    w += gridDim.x;
+    m += dm;
+    int c = m >= p.nqt;
+    m -= c ? p.nqt : 0;
+    split += ds + c;
+    c = split >= p.nsplit;
+    split -= c ? p.nsplit : 0;
+    h += dh + c;
+    c = h >= p.Hgrid;
+    h -= c ? p.Hgrid : 0;
+    b += db + c;
+    range(p);
+  }
+  // row r of the tile -> head and token; false past the last row
+  __device__ __forceinline__ bool row(const CrossAttnParams& p, int r, int& head, int& t) const {
+    if (p.pack) {
+      const int g = r / p.Lq;
+      head = h * p.G + g;
+      t = r - g * p.Lq;
+      return g < p.G;
+    }
+    head = h;
+    t = m * 128 + r;
+    return t < p.Lq;
+  }
+};
 
 // shared memory row r >= valid of a [128 x 128] V tile := 0 (whole 128-byte rows, so the swizzle does not matter)
 __device__ __forceinline__ void clear_rows(uint8_t* tile, int valid, int lane) {
@@ -182,7 +176,7 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < COUNT; ++i) mbar_init(bar(i), (i >= PB && i < PV) || (i >= MR && i < DRAIN) ? 4 : 1);
+    for (int i = 0; i < COUNT; ++i) mbar_init(bar(i), (i >= PB && i < PV) || (i >= MR && i < DRAIN_S) ? 4 : 1);
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tq);
@@ -200,164 +194,155 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_LOAD));
-    if (warp == 0 && lane == 0) {
-      // ------------------------------------------------------------ TMA
-      // in the order the MMAs consume: K of units 0, 1, 2, then V(u), K(u + 3)
-      int r = 0, nq = 0;
-      bool ok = true;
-      auto load_kv = [&](const CUtensorMap* m, const CrossCursor& c) {
-        const int e = r % NKV;
-        if (!ok || !(ok = mbar_wait(bar(KE + e), ((r / NKV) & 1) ^ 1, abort_flag, kDevTimeoutMma))) return;
-        const uint32_t dst = base + OFF_KV + e * TILE;
-        const int h = p.pack ? c.it.h : c.it.h / p.G;
-        mbar_expect_tx(bar(KF + e), TILE);
-        tma_load_4d(dst, m, bar(KF + e), 0, (c.it.i0 + c.i) * 128, h, c.it.b);
-        tma_load_4d(dst + BOX, m, bar(KF + e), 64, (c.it.i0 + c.i) * 128, h, c.it.b);
-        ++r;
-      };
-      CrossCursor ck = cursor_first(p), cv = ck;
-      auto load_k = [&] {
-        if (!ck.live) return;
-        if (ck.i == 0) {
-          const int e = ck.j % NQ;
-          if (!ok || !(ok = mbar_wait(bar(QE + e), ((ck.j / NQ) & 1) ^ 1, abort_flag, kDevTimeoutMma))) return;
-          const uint32_t dst = base + OFF_Q + e * TILE;
-          const int h = p.pack ? ck.it.h * p.G : ck.it.h;
+    constexpr uint32_t hi = sdesc_hi(1024);
+    bool ok = true;
+    // warp-wide wait of the issuing warps
+    auto wait = [&](int i, uint32_t parity, int code) {
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(i), parity, abort_flag, code));
+      tc_fence_after();
+      return ok;
+    };
+    if (warp == 0) {
+      if (lane == 0) {
+        // ------------------------------------------------------ TMA: Q and K
+        int q = 0, k = 0;  // tiles loaded
+        for (CrossItems it(p); it.live(p) && ok; it.next(p)) {
+          if (it.cnt == 0) continue;
+          const int e = q % NQ;
+          if (!(ok = mbar_wait(bar(QE + e), ((q / NQ) & 1) ^ 1, abort_flag, kDevTimeoutMma))) break;
           mbar_expect_tx(bar(QF + e), p.q_bytes);
-          tma_load_4d(dst, &tq, bar(QF + e), 0, ck.it.m * 128, h, ck.it.b);
-          tma_load_4d(dst + BOX, &tq, bar(QF + e), 64, ck.it.m * 128, h, ck.it.b);
-          nq = ck.j + 1;
+          const int hq = p.pack ? it.h * p.G : it.h, hk = p.pack ? it.h : it.h / p.G;
+          tma_load_4d(base + OFF_Q + e * TILE, &tq, bar(QF + e), 0, it.m * 128, hq, it.b);
+          tma_load_4d(base + OFF_Q + e * TILE + BOX, &tq, bar(QF + e), 64, it.m * 128, hq, it.b);
+          ++q;
+          for (int i = it.i0; i < it.i0 + it.cnt; ++i, ++k) {
+            const int f = k % NK;
+            if (!(ok = mbar_wait(bar(KE + f), ((k / NK) & 1) ^ 1, abort_flag, kDevTimeoutMma))) break;
+            mbar_expect_tx(bar(KF + f), TILE);
+            tma_load_4d(base + OFF_K + f * TILE, &tk, bar(KF + f), 0, i * 128, hk, it.b);
+            tma_load_4d(base + OFF_K + f * TILE + BOX, &tk, bar(KF + f), 64, i * 128, hk, it.b);
+          }
         }
-        load_kv(&tk, ck);
-        cursor_next(p, ck);
-      };
-      for (int n = 0; n < NS; ++n) load_k();
-      while (cv.live && ok) {
-        load_kv(&tv, cv);
-        cursor_next(p, cv);
-        load_k();
+        // no copy may still target shared memory when the CTA exits; the waits
+        // ignore the abort flag and share one limit
+        const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
+        bool drained = true;
+        for (int n = max(0, q - NQ); n < q && drained; ++n)
+          drained = mbar_wait_until(bar(QF + n % NQ), (n / NQ) & 1, deadline);
+        for (int n = max(0, k - NK); n < k && drained; ++n)
+          drained = mbar_wait_until(bar(KF + n % NK), (n / NK) & 1, deadline);
       }
-      // no copy may still target shared memory when the CTA exits; the waits
-      // ignore the abort flag and share one limit
-      const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
-      bool drained = true;
-      for (int n = max(0, nq - NQ); n < nq && drained; ++n)
-        drained = mbar_wait_until(bar(QF + n % NQ), (n / NQ) & 1, deadline);
-      for (int n = max(0, r - NKV); n < r && drained; ++n)
-        drained = mbar_wait_until(bar(KF + n % NKV), (n / NKV) & 1, deadline);
+    } else if (warp == 3) {
+      if (lane == 0) {
+        // ------------------------------------------------------------ TMA: V
+        int k = 0;
+        for (CrossItems it(p); it.live(p) && ok; it.next(p)) {
+          const int hk = p.pack ? it.h : it.h / p.G;
+          for (int i = it.i0; i < it.i0 + it.cnt; ++i, ++k) {
+            const int f = k % NV;
+            if (!(ok = mbar_wait(bar(VE + f), ((k / NV) & 1) ^ 1, abort_flag, kDevTimeoutMma))) break;
+            mbar_expect_tx(bar(VF + f), TILE);
+            tma_load_4d(base + OFF_V + f * TILE, &tv, bar(VF + f), 0, i * 128, hk, it.b);
+            tma_load_4d(base + OFF_V + f * TILE + BOX, &tv, bar(VF + f), 64, i * 128, hk, it.b);
+          }
+        }
+        const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
+        bool drained = true;
+        for (int n = max(0, k - NV); n < k && drained; ++n)
+          drained = mbar_wait_until(bar(VF + n % NV), (n / NV) & 1, deadline);
+      }
     } else if (warp == 1) {
-      // ---------------------------------------------------------------- MMA
-      // the whole warp follows the sequence (it clears V rows together); one elected
-      // lane issues.  S runs three units ahead of P V.
+      // ------------------------------------------------------- MMA: S = Q K^T
       constexpr uint32_t id_qk = idesc_bf16_f32(128, 128, false, false);
-      constexpr uint32_t id_pv = idesc_bf16_f32(128, 128, false, true);
-      constexpr uint32_t hi = sdesc_hi(1024);
-      bool ok = true;
-      auto wait = [&](int i, uint32_t parity, int code) {
-        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(i), parity, abort_flag, code));
-        tc_fence_after();
-        return ok;
-      };
-      // key tiles of the next item that has any, from w on; 0 at the end
-      auto next_item = [&](uint32_t& w, int& left, int& tail) {
-        left = 0;
-        for (; w < (uint32_t)p.items && left == 0; w += gridDim.x) {
-          const CrossItem it = cross_item(p, w);
-          left = __shfl_sync(0xffffffffu, it.cnt, 0);
-          // valid keys of the item's last tile, where rows past them may hold anything
-          const int valid = it.len - (it.i0 + it.cnt - 1) * 128;
-          tail = __shfl_sync(0xffffffffu, it.len < p.Lk && valid < 128 ? valid : 128, 0);
-        }
-      };
-      int e = 0;          // ring entry consumed next, and its phase
-      uint32_t e_ph = 0;
-      auto pop = [&] {
-        if (++e == NKV) {
-          e = 0;
-          e_ph ^= 1u;
-        }
-      };
-      uint32_t ws = blockIdx.x, wv = blockIdx.x;
-      int s_left, s_tail, v_left, v_tail;
-      next_item(ws, s_left, s_tail);
-      next_item(wv, v_left, v_tail);
-      bool s_first = true, v_first = true;
-      int eq = 0, gs = 0, g = 0;
-      uint32_t q_ph = 0, g_ph = 0, o_ph = 1;
-      auto issue_s = [&] {  // S of the next unit
-        if (s_left == 0 || !ok) return;
-        if (s_first && !wait(QF + eq, q_ph, kDevTimeoutLoad)) return;
-        if (!wait(KF + e, e_ph, kDevTimeoutLoad)) return;
-        const bool last = s_left == 1;
-        if (elect_one()) {
-          const uint32_t dq = sdesc_lo(base + OFF_Q + eq * TILE, 16), dk = sdesc_lo(base + OFF_KV + e * TILE, 16);
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {
-            const uint32_t off = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
-            mma_bf16_ss_lo(tmem + 128 * gs, dq + off, hi, dk + off, hi, id_qk, kk > 0 ? 1u : 0u);
-          }
-          mma_commit(bar(SF + gs));
-          mma_commit(bar(KE + e));
-          if (last) mma_commit(bar(QE + eq));
-        }
-        __syncwarp();
-        pop();
-        gs = gs == NS - 1 ? 0 : gs + 1;
-        s_first = last;
-        if (last) {
-          if (++eq == NQ) {
-            eq = 0;
-            q_ph ^= 1u;
-          }
-          next_item(ws, s_left, s_tail);
-        } else {
-          --s_left;
-        }
-      };
-      for (int n = 0; n < NS; ++n) issue_s();
-      while (v_left > 0 && ok) {
-        const bool last = v_left == 1;
-        if (!wait(KF + e, e_ph, kDevTimeoutLoad)) break;
-        if (last && v_tail < 128) clear_rows(smem1k + OFF_KV + e * TILE, v_tail, lane);
-        // O of the previous item has been read
-        if (v_first && !wait(OE, o_ph, kDevTimeoutSoftmax)) break;
-        const uint32_t dv = sdesc_lo(base + OFF_KV + e * TILE, BOX), tp = tmem + 128 * g + 64;
-#pragma unroll
-        for (int half = 1; half >= 0; --half) {  // keys [64, 128) first, as the softmax hands them over
-          if (!wait((half ? PB : PA) + g, g_ph, kDevTimeoutSoftmax)) break;
+      int eq = 0, ek = 0, g = 0;
+      uint32_t q_ph = 0, k_ph = 0, g_ph = 1;  // g_ph: the buffer's previous unit is done (passes at first)
+      for (CrossItems it(p); it.live(p) && ok; it.next(p)) {
+        const int cnt = __shfl_sync(0xffffffffu, it.cnt, 0);
+        if (cnt == 0) continue;
+        if (!wait(QF + eq, q_ph, kDevTimeoutLoad)) break;
+        const uint32_t dq = sdesc_lo(base + OFF_Q + eq * TILE, 16);
+        for (int i = 0; i < cnt; ++i) {
+          if (!wait(KF + ek, k_ph, kDevTimeoutLoad) || !wait(PV + g, g_ph, kDevTimeoutMma)) break;
           if (elect_one()) {
+            const uint32_t dk = sdesc_lo(base + OFF_K + ek * TILE, 16);
 #pragma unroll
-            for (int k4 = 0; k4 < 4; ++k4) {
-              const int kk = 4 * half + k4;
-              mma_bf16_ts_lo(tmem + O_COL, tp + 8 * kk, dv + ((kk * 2048) >> 4), hi, id_pv,
-                             (!v_first || half == 0 || k4 > 0) ? 1u : 0u);
+            for (int kk = 0; kk < 8; ++kk) {
+              const uint32_t off = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
+              mma_bf16_ss_lo(tmem + 128 * g, dq + off, hi, dk + off, hi, id_qk, kk > 0 ? 1u : 0u);
             }
-            if (half == 0) {
-              mma_commit(bar(KE + e));
-              mma_commit(bar(PV + g));
-            }
+            mma_commit(bar(SF + g));
+            mma_commit(bar(KE + ek));
+            if (i + 1 == cnt) mma_commit(bar(QE + eq));
           }
           __syncwarp();
+          if (++ek == NK) {
+            ek = 0;
+            k_ph ^= 1u;
+          }
+          if (++g == NS) {
+            g = 0;
+            g_ph ^= 1u;
+          }
         }
-        if (!ok) break;
-        pop();
-        issue_s();  // into the buffer whose P V was just issued
-        if (++g == NS) {
-          g = 0;
-          g_ph ^= 1u;
-        }
-        v_first = last;
-        if (last) {
-          o_ph ^= 1u;
-          next_item(wv, v_left, v_tail);
-        } else {
-          --v_left;
+        if (++eq == NQ) {
+          eq = 0;
+          q_ph ^= 1u;
         }
       }
       // every MMA issued has completed before TMEM is freed, also on the abort path
       if (elect_one()) {
-        mma_commit(bar(DRAIN));
-        mbar_wait_until(bar(DRAIN), 0, globaltimer_ns() + kWaitLimitNs);
+        mma_commit(bar(DRAIN_S));
+        mbar_wait_until(bar(DRAIN_S), 0, globaltimer_ns() + kWaitLimitNs);
+      }
+      __syncwarp();
+    } else {
+      // ------------------------------------------------------- MMA: O += P V
+      constexpr uint32_t id_pv = idesc_bf16_f32(128, 128, false, true);
+      int ev = 0, g = 0;
+      uint32_t v_ph = 0, g_ph = 0, o_ph = 1;
+      for (CrossItems it(p); it.live(p) && ok; it.next(p)) {
+        const int cnt = __shfl_sync(0xffffffffu, it.cnt, 0);
+        if (cnt == 0) continue;
+        // valid keys of the item's last tile, where rows past them may hold anything
+        const int valid = it.len - (it.i0 + it.cnt - 1) * 128;
+        const int tail = __shfl_sync(0xffffffffu, it.len < p.Lk ? valid : 128, 0);
+        for (int i = 0; i < cnt && ok; ++i) {
+          if (!wait(VF + ev, v_ph, kDevTimeoutLoad)) break;
+          if (tail < 128 && i + 1 == cnt) clear_rows(smem1k + OFF_V + ev * TILE, tail, lane);
+          // O of the previous item has been read
+          if (i == 0 && !wait(OE, o_ph, kDevTimeoutSoftmax)) break;
+          const uint32_t dv = sdesc_lo(base + OFF_V + ev * TILE, BOX), tp = tmem + 128 * g + 64;
+#pragma unroll
+          for (int half = 1; half >= 0; --half) {  // keys [64, 128) first, as the softmax hands them over
+            if (!wait((half ? PB : PA) + g, g_ph, kDevTimeoutSoftmax)) break;
+            if (elect_one()) {
+#pragma unroll
+              for (int k4 = 0; k4 < 4; ++k4) {
+                const int kk = 4 * half + k4;
+                mma_bf16_ts_lo(tmem + O_COL, tp + 8 * kk, dv + ((kk * 2048) >> 4), hi, id_pv,
+                               (i > 0 || half == 0 || k4 > 0) ? 1u : 0u);
+              }
+              if (half == 0) {
+                mma_commit(bar(VE + ev));
+                mma_commit(bar(PV + g));
+              }
+            }
+            __syncwarp();
+          }
+          if (++ev == NV) {
+            ev = 0;
+            v_ph ^= 1u;
+          }
+          if (++g == NS) {
+            g = 0;
+            g_ph ^= 1u;
+          }
+        }
+        o_ph ^= 1u;
+      }
+      if (elect_one()) {
+        mma_commit(bar(DRAIN_P));
+        mbar_wait_until(bar(DRAIN_P), 0, globaltimer_ns() + kWaitLimitNs);
       }
       __syncwarp();
     }
@@ -377,13 +362,12 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
       return ok;
     };
     int u = 0, items = 0;
-    for (uint32_t w = blockIdx.x; w < (uint32_t)p.items && ok; w += gridDim.x) {
-      const CrossItem it = cross_item(p, w);
+    for (CrossItems it(p); it.live(p) && ok; it.next(p)) {
       if (it.cnt == 0) {
         // no keys: zeros (one warpgroup in turn; no unit, nothing to wait for)
         if (items % 3 == g) {
           int h, tok;
-          const bool live = cross_row(p, it, row, h, tok);
+          const bool live = it.row(p, row, h, tok);
           if (p.nsplit > 1) {
             if (live) p.part_lse[(((int64_t)it.split * p.B + it.b) * p.H + h) * p.Lq + tok] = -INFINITY;
           } else {
@@ -529,37 +513,38 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
 
         // ------------------------------------------------- the item's output
         int h, tok;
-        const bool live = cross_row(p, it, row, h, tok);
+        const bool live = it.row(p, row, h, tok);
         const float inv_l = 1.0f / l, lse = m + log2f(l);
         if (!wait(PV + g, ph, kDevTimeoutMma)) break;
         tc_fence_after();
         const int64_t prow = (((int64_t)it.split * p.B + it.b) * p.H + h) * p.Lq + tok;
         __nv_bfloat16* dst = p.out + it.b * p.o_sB + h * p.o_sH + tok * p.o_sT;
+        uint32_t v[128];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t v[64];
-          __syncwarp();  // the stores below diverge, the load is warp-collective
-          tmem_ld32(tO + 64 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-          tmem_ld32(tO + 64 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-          tmem_ld_wait();
-          if (c == 1) {
-            // O is in registers: the next item may start its own
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(OE));
-          }
-          float f[64];
+        for (int c = 0; c < 4; ++c) tmem_ld32(tO + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
+        tmem_ld_wait();
+        // O is in registers: the next item may start its own
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(OE));
+        if (live) {
+          if (p.nsplit > 1) {
+            float4* d4 = reinterpret_cast<float4*>(p.part_o + prow * 128);
 #pragma unroll
-          for (int e = 0; e < 64; ++e) f[e] = __uint_as_float(v[e]) * inv_l;
-          if (live && p.nsplit > 1) {
-            float4* d4 = reinterpret_cast<float4*>(p.part_o + prow * 128 + 64 * c);
+            for (int e = 0; e < 32; ++e)
+              d4[e] = make_float4(__uint_as_float(v[4 * e]) * inv_l, __uint_as_float(v[4 * e + 1]) * inv_l,
+                                  __uint_as_float(v[4 * e + 2]) * inv_l, __uint_as_float(v[4 * e + 3]) * inv_l);
+          } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) d4[e] = make_float4(f[4 * e], f[4 * e + 1], f[4 * e + 2], f[4 * e + 3]);
-          } else if (live) {
+            for (int e = 0; e < 8; ++e) {
+              float f[16];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) store16_bf16(dst + 64 * c + 16 * e, f + 16 * e, wide);
+              for (int k = 0; k < 16; ++k) f[k] = __uint_as_float(v[16 * e + k]) * inv_l;
+              store16_bf16(dst + 16 * e, f, wide);
+            }
           }
         }
+        __syncwarp();
         if (p.nsplit > 1) {
           if (live) p.part_lse[prow] = lse;
         } else if (p.lse && (live || !p.pack)) {
