@@ -185,18 +185,21 @@ int rola_b200_cross_attn(const void* q, int64_t q_sB, int64_t q_sH, int64_t q_sT
   p.part_lse = p.part_o ? p.part_o + (size_t)pl.nsplit * B * H * Lq * 128 : nullptr;
   p.q_bytes = pl.pack ? 256u * (uint32_t)(p.G * Lq) : 32768u;
   p.qk_scale = (float)(0.08838834764831845 * 1.4426950408889634);  // 128^-0.5 * log2(e)
-  CUtensorMap tq, tk, tv;
+  CUtensorMap tq, tk, tv, to;
   if (pl.pack) {  // one box holds the G heads of a key head, Lq rows each
     const uint64_t dims[4] = {128, (uint64_t)Lq, (uint64_t)H, (uint64_t)B};
-    const uint64_t strides[3] = {(uint64_t)q_sT * 2, (uint64_t)q_sH * 2, (uint64_t)q_sB * 2};
     const uint32_t box[4] = {64, (uint32_t)Lq, (uint32_t)p.G, 1};
-    ROLA_TRY(make_map(&tq, q, 4, dims, strides, box, "cross_attn: q"));
+    const uint64_t qs[3] = {(uint64_t)q_sT * 2, (uint64_t)q_sH * 2, (uint64_t)q_sB * 2};
+    const uint64_t os[3] = {(uint64_t)o_sT * 2, (uint64_t)o_sH * 2, (uint64_t)o_sB * 2};
+    ROLA_TRY(make_map(&tq, q, 4, dims, qs, box, "cross_attn: q"));
+    ROLA_TRY(make_map(&to, out, 4, dims, os, box, "cross_attn: out"));
   } else {
     ROLA_TRY(make_head_map(&tq, q, 128, q_sB, q_sH, q_sT, Lq, H, B, "cross_attn: q"));
+    ROLA_TRY(make_head_map(&to, out, 128, o_sB, o_sH, o_sT, Lq, H, B, "cross_attn: out"));
   }
   ROLA_TRY(make_head_map(&tk, k, 128, k_sB, k_sH, k_sT, Lk, Hkv, B, "cross_attn: k"));
   ROLA_TRY(make_head_map(&tv, v, 128, v_sB, v_sH, v_sT, Lk, Hkv, B, "cross_attn: v"));
-  return cuda_status(launch_cross_attn(tq, tk, tv, p, S(stream)), what);
+  return cuda_status(launch_cross_attn(tq, tk, tv, to, p, S(stream)), what);
 }
 
 struct CrossBwdLayout {

@@ -123,6 +123,22 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   }
 }
 
+// The same in few instructions, for warps whose waits are on the path of every
+// step: bounded by attempts (each is at least a shared-memory round trip and may
+// suspend the thread, so 2^20 of them last tens of milliseconds or longer; a
+// legitimate wait lasts microseconds).
+__device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity, volatile int* abort_flag, int err_code) {
+  for (uint32_t n = 0; !mbar_try_wait(bar, parity); ++n) {
+    if ((n & 1023u) == 1023u && *abort_flag) return false;
+    if (n >= (1u << 20)) {
+      *abort_flag = 1;
+      set_device_error(err_code);
+      return false;
+    }
+  }
+  return true;
+}
+
 // Wait for a phase regardless of the CTA abort flag, until the globaltimer
 // passes `deadline`.  Used to drain bulk copies still in flight into shared
 // memory before a CTA exits (also on the abort path, where mbar_wait would
@@ -180,6 +196,12 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, uint32_t src,
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(m)),
                "r"(src), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* m, uint32_t src, int x, int y, int z, int w) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(m)),
+               "r"(src), "r"(x), "r"(y), "r"(z), "r"(w)
                : "memory");
 }
 __device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }

@@ -18,14 +18,16 @@
 // own, and they run across the items' ends: an encoder's states are few keys (512:
 // four units), and the S products of the next item are issued while this one
 // finishes.  m and l pass from unit to unit through shared memory, in order.
-//   warp 0        TMA producer of Q (2 x 32 KB) and K tiles (2 x 32 KB)
+//   warp 0        TMA producer of Q (2 x 32 KB) and K tiles (2 x 32 KB); it also stores
+//                 an item's output, left in the item's Q tile, before the tile is loaded
+//                 again (rows stored by the lanes themselves held their warps 2500 clocks)
 //   warp 3        TMA producer of V tiles (3 x 32 KB)
 //   warp 1        issues S; owner of the tensor memory
 //   warp 2        issues P V.  It also clears the V rows past len[b] (their P is 0,
 //                 but 0 * NaN is not).  One warp for both products was the limit:
 //                 2150 clocks a unit to issue what takes the tensor core 1024
 //   warpgroup g = 1, 2, 3: the units u with u % 3 == g - 1; thread = row = TMEM lane.
-//                 The unit that ends an item scales its O by 1/l and stores it.
+//                 The unit that ends an item scales its O by 1/l and leaves it in bf16.
 // Few rows: the keys of an item are cut into slices, each leaves O/l in fp32 and
 // its log-sum-exp, and combine_kernel joins them.  When the G query heads of a
 // key head have 128 rows or fewer together, they form one tile (one read of K/V
@@ -52,7 +54,8 @@ constexpr int SMEM = OFF_BAR + 512;
 constexpr int O_COL = 128 * NS;   // S of unit u at column 128 (u % 3), its P in the upper 64 of those; O behind them
 constexpr float RESCALE = 8.0f;   // log2 growth of the maximum that triggers a rescale of O
 enum : int {
-  QF = 0, QE = QF + NQ, KF = QE + NQ, KE = KF + NK, VF = KE + NK, VE = VF + NV,
+  QF = 0, QE = QF + NQ,  // QE: the item's output is in its Q tile, 4 warp arrivals
+  KF = QE + NQ, KE = KF + NK, VF = KE + NK, VE = VF + NV,
   SF = VE + NV,      // S of a unit in TMEM: SF + u % 3
   PB = SF + NS,      // P of keys [64, 128) in TMEM, 4 warp arrivals
   PA = PB + NS,      // P of keys [0, 64)
@@ -147,24 +150,10 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int valid, int lane) {
   __syncwarp();
 }
 
-// 16 fp32 values -> bf16, one 32-byte store (a whole sector of the lane's row) where the row is 32-byte aligned
-__device__ __forceinline__ void store16_bf16(__nv_bfloat16* dst, const float* f, bool wide) {
-  uint32_t w[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = pack_bf2(f[2 * e], f[2 * e + 1]);
-  if (wide) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]),
-                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-  } else {
-    reinterpret_cast<uint4*>(dst)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    reinterpret_cast<uint4*>(dst)[1] = make_uint4(w[4], w[5], w[6], w[7]);
-  }
-}
-
 __global__ void __launch_bounds__(xattn::THREADS, 1)
     cross_attn_tcgen05(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
-                       const __grid_constant__ CUtensorMap tv, const CrossAttnParams p) {
+                       const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap to,
+                       const CrossAttnParams p) {
   using namespace xattn;
   extern __shared__ __align__(1024) uint8_t smem1k[];
   const uint32_t base = smem_u32(smem1k);
@@ -176,12 +165,13 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < COUNT; ++i) mbar_init(bar(i), (i >= PB && i < PV) || (i >= MR && i < DRAIN_S) ? 4 : 1);
+    for (int i = 0; i < COUNT; ++i) mbar_init(bar(i), (i >= QE && i < KF) || (i >= PB && i < PV) || (i >= MR && i < DRAIN_S) ? 4 : 1);
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tq);
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
+    if (p.nsplit == 1) prefetch_tmap(&to);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), 512);
@@ -198,31 +188,47 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
     bool ok = true;
     // warp-wide wait of the issuing warps
     auto wait = [&](int i, uint32_t parity, int code) {
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(i), parity, abort_flag, code));
+      if (ok) ok = __all_sync(0xffffffffu, mbar_spin(bar(i), parity, abort_flag, code));
       tc_fence_after();
       return ok;
     };
     if (warp == 0) {
       if (lane == 0) {
-        // ------------------------------------------------------ TMA: Q and K
+        // -------------------------------------------- TMA: Q and K; the output
         int q = 0, k = 0;  // tiles loaded
+        int om[NQ], oh[NQ], ob[NQ];  // the items whose Q tiles are loaded
+        // output of the item in Q tile e, the n-th of that tile
+        auto store_out = [&](int e, int n) {
+          if (!mbar_spin(bar(QE + e), n & 1, abort_flag, kDevTimeoutSoftmax)) return false;
+          if (p.nsplit == 1) {
+            tma_store_4d(&to, base + OFF_Q + e * TILE, 0, om[e] * 128, oh[e], ob[e]);
+            tma_store_4d(&to, base + OFF_Q + e * TILE + BOX, 64, om[e] * 128, oh[e], ob[e]);
+            tma_store_commit();
+            tma_store_wait_read();
+          }
+          return true;
+        };
         for (CrossItems it(p); it.live(p) && ok; it.next(p)) {
           if (it.cnt == 0) continue;
           const int e = q % NQ;
-          if (!(ok = mbar_wait(bar(QE + e), ((q / NQ) & 1) ^ 1, abort_flag, kDevTimeoutMma))) break;
+          if (q >= NQ && !(ok = store_out(e, q / NQ - 1))) break;
           mbar_expect_tx(bar(QF + e), p.q_bytes);
           const int hq = p.pack ? it.h * p.G : it.h, hk = p.pack ? it.h : it.h / p.G;
           tma_load_4d(base + OFF_Q + e * TILE, &tq, bar(QF + e), 0, it.m * 128, hq, it.b);
           tma_load_4d(base + OFF_Q + e * TILE + BOX, &tq, bar(QF + e), 64, it.m * 128, hq, it.b);
+          om[e] = it.m;
+          oh[e] = hq;
+          ob[e] = it.b;
           ++q;
           for (int i = it.i0; i < it.i0 + it.cnt; ++i, ++k) {
             const int f = k % NK;
-            if (!(ok = mbar_wait(bar(KE + f), ((k / NK) & 1) ^ 1, abort_flag, kDevTimeoutMma))) break;
+            if (!(ok = mbar_spin(bar(KE + f), ((k / NK) & 1) ^ 1, abort_flag, kDevTimeoutMma))) break;
             mbar_expect_tx(bar(KF + f), TILE);
             tma_load_4d(base + OFF_K + f * TILE, &tk, bar(KF + f), 0, i * 128, hk, it.b);
             tma_load_4d(base + OFF_K + f * TILE + BOX, &tk, bar(KF + f), 64, i * 128, hk, it.b);
           }
         }
+        for (int n = max(0, q - NQ); n < q && ok; ++n) ok = store_out(n % NQ, n / NQ);
         // no copy may still target shared memory when the CTA exits; the waits
         // ignore the abort flag and share one limit
         const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
@@ -240,7 +246,7 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
           const int hk = p.pack ? it.h : it.h / p.G;
           for (int i = it.i0; i < it.i0 + it.cnt; ++i, ++k) {
             const int f = k % NV;
-            if (!(ok = mbar_wait(bar(VE + f), ((k / NV) & 1) ^ 1, abort_flag, kDevTimeoutMma))) break;
+            if (!(ok = mbar_spin(bar(VE + f), ((k / NV) & 1) ^ 1, abort_flag, kDevTimeoutMma))) break;
             mbar_expect_tx(bar(VF + f), TILE);
             tma_load_4d(base + OFF_V + f * TILE, &tv, bar(VF + f), 0, i * 128, hk, it.b);
             tma_load_4d(base + OFF_V + f * TILE + BOX, &tv, bar(VF + f), 64, i * 128, hk, it.b);
@@ -272,7 +278,6 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
             }
             mma_commit(bar(SF + g));
             mma_commit(bar(KE + ek));
-            if (i + 1 == cnt) mma_commit(bar(QE + eq));
           }
           __syncwarp();
           if (++ek == NK) {
@@ -355,13 +360,12 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
     float* s_m = reinterpret_cast<float*>(smem1k + OFF_M) + row;
     float* s_l = reinterpret_cast<float*>(smem1k + OFF_L) + row;
     const float scale = p.qk_scale;
-    const bool wide = ((reinterpret_cast<uintptr_t>(p.out) >> 1) | p.o_sB | p.o_sH | p.o_sT) % 16 == 0;
     bool ok = true;
     auto wait = [&](int i, uint32_t parity, int code) {
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(i), parity, abort_flag, code));
+      if (ok) ok = __all_sync(0xffffffffu, mbar_spin(bar(i), parity, abort_flag, code));
       return ok;
     };
-    int u = 0, items = 0;
+    int u = 0, j = 0, items = 0;  // units, items with keys, items
     for (CrossItems it(p); it.live(p) && ok; it.next(p)) {
       if (it.cnt == 0) {
         // no keys: zeros (one warpgroup in turn; no unit, nothing to wait for)
@@ -518,33 +522,42 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
         if (!wait(PV + g, ph, kDevTimeoutMma)) break;
         tc_fence_after();
         const int64_t prow = (((int64_t)it.split * p.B + it.b) * p.H + h) * p.Lq + tok;
-        __nv_bfloat16* dst = p.out + it.b * p.o_sB + h * p.o_sH + tok * p.o_sT;
-        uint32_t v[128];
+        // the row of the item's Q tile, whose last product is done: 16-byte chunk c of a
+        // box at c ^ (row & 7), the maps' swizzle
+        uint8_t* stage = smem1k + OFF_Q + (j % NQ) * TILE + row * 128;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tO + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
-        tmem_ld_wait();
-        // O is in registers: the next item may start its own
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(OE));
-        if (live) {
-          if (p.nsplit > 1) {
-            float4* d4 = reinterpret_cast<float4*>(p.part_o + prow * 128);
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              d4[e] = make_float4(__uint_as_float(v[4 * e]) * inv_l, __uint_as_float(v[4 * e + 1]) * inv_l,
-                                  __uint_as_float(v[4 * e + 2]) * inv_l, __uint_as_float(v[4 * e + 3]) * inv_l);
-          } else {
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[64];
+          __syncwarp();  // the stores of a slice's partial diverge, the load is warp-collective
+          tmem_ld32(tO + 64 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+          tmem_ld32(tO + 64 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+          tmem_ld_wait();
+          if (c == 1) {
+            // O is in registers: the next item may start its own
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(OE));
+          }
+          if (p.nsplit == 1) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              float f[16];
+              uint32_t w[4];
 #pragma unroll
-              for (int k = 0; k < 16; ++k) f[k] = __uint_as_float(v[16 * e + k]) * inv_l;
-              store16_bf16(dst + 16 * e, f, wide);
+              for (int k = 0; k < 4; ++k)
+                w[k] = pack_bf2(__uint_as_float(v[8 * e + 2 * k]) * inv_l, __uint_as_float(v[8 * e + 2 * k + 1]) * inv_l);
+              *reinterpret_cast<uint4*>(stage + c * BOX + ((e ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
+          } else if (live) {
+            float4* d4 = reinterpret_cast<float4*>(p.part_o + prow * 128 + 64 * c);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              d4[e] = make_float4(__uint_as_float(v[4 * e]) * inv_l, __uint_as_float(v[4 * e + 1]) * inv_l,
+                                  __uint_as_float(v[4 * e + 2]) * inv_l, __uint_as_float(v[4 * e + 3]) * inv_l);
           }
         }
+        fence_proxy_async_smem();
         __syncwarp();
+        if (lane == 0) mbar_arrive(bar(QE + j % NQ));
         if (p.nsplit > 1) {
           if (live) p.part_lse[prow] = lse;
         } else if (p.lse && (live || !p.pack)) {
@@ -552,6 +565,7 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
         }
       }
       ++items;
+      ++j;
     }
   }
   tc_fence_before();
@@ -617,15 +631,15 @@ CrossAttnPlan cross_attn_plan(int B, int H, int Hkv, int Lq, int Lk) {
   return pl;
 }
 
-int launch_cross_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CrossAttnParams& p,
-                      cudaStream_t s) {
+int launch_cross_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to,
+                      const CrossAttnParams& p, cudaStream_t s) {
   using namespace xattn;
   static KernelReady ready;
   const int rc = kernel_ready(ready, cross_attn_tcgen05, SMEM, LAUNCH_REGS);
   if (rc != 0) return rc;
   cudaError_t e;
   const int sms = device_sms();
-  cross_attn_tcgen05<<<(unsigned)(p.items < sms ? p.items : sms), THREADS, SMEM, s>>>(tq, tk, tv, p);
+  cross_attn_tcgen05<<<(unsigned)(p.items < sms ? p.items : sms), THREADS, SMEM, s>>>(tq, tk, tv, to, p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return (int)e;
   const int64_t rows = (int64_t)p.B * p.H * p.Lq;

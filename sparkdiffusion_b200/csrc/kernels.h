@@ -249,8 +249,9 @@ struct CrossAttnParams {
   uint32_t q_bytes;        // bytes of one Q tile load
   float qk_scale;          // D^-1/2 * log2(e)
 };
-int launch_cross_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CrossAttnParams& p,
-                      cudaStream_t s);
+// to: the output, boxes as q's
+int launch_cross_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& to,
+                      const CrossAttnParams& p, cudaStream_t s);
 
 // cross_attn_bwd.cu -------------------------------------------------------
 struct CrossBwdParams {
