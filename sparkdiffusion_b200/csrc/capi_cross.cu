@@ -241,11 +241,12 @@ int rola_b200_cross_attn_bwd(const void* q, int64_t q_sB, int64_t q_sH, int64_t 
              "%s: 16-byte aligned tensors required", what);
   const CrossBwdLayout f = cross_bwd_layout(B, H, Hkv, Lq, Lk);
   ROLA_CHECK(workspace_bytes >= f.total, "%s: workspace of %zu bytes < %zu", what, workspace_bytes, f.total);
-  CUtensorMap tq, tk, tv, tdo;
+  CUtensorMap tq, tk, tv, tdo, tdq;
   ROLA_TRY(make_head_map(&tq, q, 128, q_sB, q_sH, q_sT, Lq, H, B, "cross_attn_bwd: q", 64));
   ROLA_TRY(make_head_map(&tk, k, 128, k_sB, k_sH, k_sT, Lk, Hkv, B, "cross_attn_bwd: k", 64));
   ROLA_TRY(make_head_map(&tv, v, 128, v_sB, v_sH, v_sT, Lk, Hkv, B, "cross_attn_bwd: v", 64));
   ROLA_TRY(make_head_map(&tdo, dout, 128, do_sB, do_sH, do_sT, Lq, H, B, "cross_attn_bwd: dout", 64));
+  ROLA_TRY(make_head_map(&tdq, dq, 128, dq_sB, dq_sH, dq_sT, Lq, H, B, "cross_attn_bwd: dq", 64));
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   CrossBwdParams p{};
   p.kv_lens = kv_lens;
@@ -260,7 +261,7 @@ int rola_b200_cross_attn_bwd(const void* q, int64_t q_sB, int64_t q_sH, int64_t 
   ROLA_TRY(cuda_status(launch_attn_bwd_delta(BF(out), o_sB, o_sH, o_sT, BF(dout), do_sB, do_sH, do_sT, B, H, Lq,
                                              p.Lpad, const_cast<float*>(p.delta), S(stream)),
                        "cross_attn_bwd/delta"));
-  return cuda_status(launch_cross_attn_bwd(tq, tk, tv, tdo, p, S(stream)), what);
+  return cuda_status(launch_cross_attn_bwd(tq, tk, tv, tdo, tdq, p, S(stream)), what);
 }
 
 }  // extern "C"

@@ -30,42 +30,100 @@ __device__ __forceinline__ void clear_half_rows(uint8_t* half, int valid, int la
 }
 
 // ---------------------------------------------------------------------------
-// dq: one CTA per (128-row query tile, b, h); steps of 64 keys
+// dq: persistent CTAs walk items (128 query rows of a head) in steps of 64 keys.
+// A step is a chain, (S, dP) -> dS -> dQ, three in flight across the items' ends
+// (S and dP of a step take 128 columns of tensor memory, dQ 128), as the units of
+// cross_attn_tcgen05; one CTA per item spent more time on its ends than on the 8
+// steps of 512 keys (1.06 ms at 32760 x 512, 40 heads).
+//   warp 0   TMA producer of Q and dO (2 x 64 KB); it also stores an item's dQ,
+//            left in the item's Q tile, before that is loaded again
+//   warp 3   TMA producer of K (4 x 16 KB) and V (2 x 16 KB)
+//   warp 1   issues S and dP; owner of the tensor memory
+//   warp 2   issues dQ; clears the K rows past len[b] first
+//   warpgroups 1-3: dS of the steps u with u % 3 == warpgroup - 1 (thread = row);
+//            the step that ends an item leaves its dQ in bf16
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(bwd::DQ_THREADS, 1)
+namespace xdq {
+constexpr int THREADS = 512, LAUNCH_REGS = 128, REGS_LOAD = 56, REGS_SOFTMAX = 152;
+static_assert(128 * (REGS_LOAD + 3 * REGS_SOFTMAX) <= THREADS * LAUNCH_REGS, "register split");
+constexpr int NT = 2, NK = 4, NV = 2, NS = 3;
+constexpr int OFF_T = 0;                                // NT x (Q, dO)
+constexpr int OFF_K = OFF_T + NT * 2 * bwd::TILE, OFF_V = OFF_K + NK * bwd::HALF;
+constexpr int OFF_BAR = OFF_V + NV * bwd::HALF;
+constexpr int SMEM = OFF_BAR + 384;
+constexpr int ACC = 128 * NS;                           // TMEM: S of step u at 128 (u % 3), dP 64 behind, dQ at ACC
+enum : int {
+  TF = 0, TE = TF + NT,  // TE: the item's dQ is in its Q tile, 4 warp arrivals
+  KF = TE + NT, KE = KF + NK, VF = KE + NK, VE = VF + NV,
+  SF = VE + NV,          // S and dP of a step in TMEM
+  DS = SF + NS,          // dS of a step in TMEM, 4 arrivals
+  DQ = DS + NS,          // dQ of a step done
+  OE = DQ + NS,          // dQ of an item read, 4 arrivals
+  DRAIN_S = OE + 1, DRAIN_Q, COUNT
+};
+static_assert(8 * COUNT + 16 <= 384 && SMEM <= 227 * 1024, "shared memory");
+}  // namespace xdq
+
+// The items of a CTA, w = blockIdx.x, + gridDim.x, ...: query tile fastest, then
+// head and batch; digits advanced by the step's own with carries
+struct QueryItems {
+  uint32_t w;
+  int m, h, b, dm, dh, db;
+  int len, cnt;  // valid keys, steps of 64
+  __device__ __forceinline__ void range(const CrossBwdParams& p) {
+    if (!live(p)) return;
+    len = kv_len(p.kv_lens, b, p.Lk);
+    cnt = (len + 63) >> 6;
+  }
+  __device__ __forceinline__ explicit QueryItems(const CrossBwdParams& p) : w(blockIdx.x) {
+    auto digits = [&](uint32_t x, int& m_, int& h_, int& b_) {
+      const uint32_t r = x / (uint32_t)p.NQT;
+      m_ = (int)(x - r * (uint32_t)p.NQT);
+      b_ = (int)(r / (uint32_t)p.H);
+      h_ = (int)(r - (uint32_t)b_ * (uint32_t)p.H);
+    };
+    digits(w, m, h, b);
+    digits(gridDim.x, dm, dh, db);
+    range(p);
+  }
+  __device__ __forceinline__ bool live(const CrossBwdParams& p) const { return w < (uint32_t)(p.NQT * p.H * p.B); }
+  __device__ __forceinline__ void next(const CrossBwdParams& p) {
+    w += gridDim.x;
+    m += dm;
+    int c = m >= p.NQT;
+    m -= c ? p.NQT : 0;
+    h += dh + c;
+    c = h >= p.H;
+    h -= c ? p.H : 0;
+    b += db + c;
+    range(p);
+  }
+};
+
+__global__ void __launch_bounds__(xdq::THREADS, 1)
     cross_bwd_dq_tcgen05(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                          const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
-                         const CrossBwdParams p) {
-  using namespace bwd;
+                         const __grid_constant__ CUtensorMap tdq, const CrossBwdParams p) {
+  using namespace xdq;
+  constexpr int TILE = bwd::TILE, HALF = bwd::HALF, BOX = bwd::BOX, BOX128 = bwd::BOX128;
   extern __shared__ __align__(1024) uint8_t smem1k[];
   const uint32_t base = smem_u32(smem1k);
-  const uint32_t bars = base + DQ_OFF_BAR;
-  auto bar = [&](int i) { return bars + 8u * i; };
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem1k + DQ_OFF_BAR + 8 * G_COUNT);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem1k + DQ_OFF_BAR + 8 * G_COUNT + 8);
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int m = (int)(blockIdx.x % p.NQT), bh = (int)(blockIdx.x / p.NQT), b = bh / p.H, h = bh % p.H;
-  const int len = kv_len(p.kv_lens, b, p.Lk);
-  const int n = (len + 63) / 64;
+  auto bar = [&](int i) { return base + OFF_BAR + 8u * i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem1k + OFF_BAR + 8 * COUNT);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem1k + OFF_BAR + 8 * COUNT + 8);
+  // broadcast values are warp-uniform to the compiler too (uniform registers for the MMAs)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    mbar_init(bar(G_TILE), 1);
-    for (int s = 0; s < DQ_STAGES; ++s) {
-      mbar_init(bar(G_FULL0 + s), 1);
-      mbar_init(bar(G_EMPTY0 + s), 1);
-    }
-    for (int t = 0; t < DQ_NBUF; ++t) {
-      mbar_init(bar(G_SF0 + t), 1);
-      mbar_init(bar(G_DS0 + t), 4);
-    }
-    mbar_init(bar(G_ACC), 1);
+    for (int i = 0; i < COUNT; ++i)
+      mbar_init(bar(i), (i >= TE && i < KF) || (i >= DS && i < DQ) || i == OE ? 4 : 1);
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tq);
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
     prefetch_tmap(&tdo);
+    prefetch_tmap(&tdq);
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), 512);
@@ -74,139 +132,263 @@ __global__ void __launch_bounds__(bwd::DQ_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-
-  if (warp == 0) {
-    if (lane == 0 && n > 0) {
-      // ------------------------------------------------------------ TMA
-      mbar_expect_tx(bar(G_TILE), 2 * TILE);
-      load_tile(base + DQ_OFF_Q, &tq, bar(G_TILE), 128 * m, h, b);
-      load_tile(base + DQ_OFF_DO, &tdo, bar(G_TILE), 128 * m, h, b);
-      for (int i = 0; i < n; ++i) {
-        const int s = i % DQ_STAGES;
-        if (!mbar_wait(bar(G_EMPTY0 + s), ((i / DQ_STAGES) & 1) ^ 1, abort_flag, kDevTimeoutMma)) break;
-        const uint32_t dst = base + DQ_OFF_RING + s * DQ_ENTRY;
-        mbar_expect_tx(bar(G_FULL0 + s), 2 * HALF);
-        load_half(dst, &tk, bar(G_FULL0 + s), 64 * i, h / p.G, b);
-        load_half(dst + HALF, &tv, bar(G_FULL0 + s), 64 * i, h / p.G, b);
-      }
-      // no TMA may still target shared memory when the CTA exits
-      const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
-      bool drained = mbar_wait_until(bar(G_TILE), 0, deadline);
-      for (int i = max(0, n - DQ_STAGES); i < n && drained; ++i)
-        drained = mbar_wait_until(bar(G_FULL0 + i % DQ_STAGES), (i / DQ_STAGES) & 1, deadline);
-    }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ MMA
-    // S_i, dP_i, then dQ += dS_{i-2} K_{i-2}: the tensor core computes step i
-    // while steps i-2 and i-1 are in the softmax.  The whole warp follows (it
-    // clears K rows together), lane 0 issues.
-    const uint32_t id_s = idesc_bf16_f32(128, 64, false, false);
-    const uint32_t id_q = idesc_bf16_f32(128, 128, false, true);
-    bool ok = true;
-    auto wait = [&](int i, uint32_t parity, int code) {
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar(i), parity, abort_flag, code));
-      tc_fence_after();
-      return ok;
-    };
-    if (n > 0) wait(G_TILE, 0, kDevTimeoutLoad);
-    auto issue_dq = [&](int i) {
-      if (!wait(G_DS0 + i % DQ_NBUF, (i / DQ_NBUF) & 1, kDevTimeoutSoftmax)) return;
-      const int off = DQ_OFF_RING + (i % DQ_STAGES) * DQ_ENTRY;
-      if (len - 64 * i < 64 && len < p.Lk) clear_half_rows(smem1k + off, len - 64 * i, lane);
-      if (lane == 0) {
-        mma_step_ts(tmem + DQ_ACC, tmem + 128 * (i % DQ_NBUF), base + off, id_q, i > 0);  // dQ += dS K
-        mma_commit(bar(G_EMPTY0 + i % DQ_STAGES));
-      }
-      __syncwarp();
-    };
-    for (int i = 0; i < n && ok; ++i) {
-      const int s = i % DQ_STAGES;
-      if (!wait(G_FULL0 + s, (i / DQ_STAGES) & 1, kDevTimeoutLoad)) break;
-      if (lane == 0) {
-        const uint32_t sk = base + DQ_OFF_RING + s * DQ_ENTRY, sv = sk + HALF;
-        const uint32_t tb = tmem + 128 * (i % DQ_NBUF);
-        mma_step_ss(tb, base + DQ_OFF_Q, sk, id_s);        // S  = Q K^T
-        mma_step_ss(tb + 64, base + DQ_OFF_DO, sv, id_s);  // dP = dO V^T
-        mma_commit(bar(G_SF0 + i % DQ_NBUF));
-      }
-      __syncwarp();
-      if (i >= DQ_NBUF - 1) issue_dq(i - (DQ_NBUF - 1));
-    }
-    for (int i = max(0, n - (DQ_NBUF - 1)); i < n && ok; ++i) issue_dq(i);
-    if (lane == 0) {
-      mma_commit(bar(G_ACC));
-      // every MMA issued has completed before TMEM is freed, also on the abort path
-      mbar_wait_until(bar(G_ACC), 0, globaltimer_ns() + kWaitLimitNs);
-    }
-    __syncwarp();
-  } else if (warp >= 4) {
-    // -------------------------------------- dS of every third step, then the dQ epilogue
-    const int wg = (warp - 4) >> 2;
-    const int q = warp & 3;
-    const int r = q * 32 + lane;  // query row of the tile = TMEM lane
-    const uint32_t lane_off = (uint32_t)(q * 32) << 16;
-    const uint32_t tS = tmem + lane_off + 128 * wg, tdP = tS + 64;
-    const int tok = 128 * m + r;
-    const float lse = p.lse[(int64_t)bh * p.Lpad + tok];
-    const float dlt = p.delta[(int64_t)bh * p.Lpad + tok];
-    const uint64_t sc2 = f2_pack(p.qk_scale, p.qk_scale), nl2 = f2_pack(-lse, -lse);
-    bool ok = true;
-    for (int i = wg; i < n; i += DQ_NBUF) {
-      if (!__all_sync(0xffffffffu, mbar_wait(bar(G_SF0 + wg), (i / DQ_NBUF) & 1, abort_flag, kDevTimeoutMma))) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const int valid = len - 64 * i;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t sv[32], dv[32];
-        tmem_ld32(tS + 32 * c, sv);
-        tmem_ld32(tdP + 32 * c, dv);
-        tmem_ld_wait();
-        uint32_t w[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int col = 32 * c + 2 * e;
-          float x0, x1;
-          f2_unpack(fma_f32x2(f2_pack(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, nl2), x0, x1);
-          const float d0 = ex2_approx(x0) * (__uint_as_float(dv[2 * e]) - dlt);
-          const float d1 = ex2_approx(x1) * (__uint_as_float(dv[2 * e + 1]) - dlt);
-          w[e] = pack_bf2(col < valid ? d0 : 0.f, col + 1 < valid ? d1 : 0.f);
-        }
-        tmem_st16(tS + 16 * c, w);  // packed dS over the first 32 S columns of the buffer
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(G_DS0 + wg));
-    }
-    if (wg == 2) ok = false;  // the third warpgroup has no epilogue columns
-    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(G_ACC), 0, abort_flag, kDevTimeoutMma));
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  bool ok = true;
+  auto wait = [&](int i, uint32_t parity, int code) {
+    if (ok) ok = __all_sync(0xffffffffu, mbar_spin(bar(i), parity, abort_flag, code));
     tc_fence_after();
-    if (ok) {
-      const uint32_t tQ = tmem + DQ_ACC + lane_off + 64 * wg;
-      uint32_t v[64];
-      if (n > 0) {
-        tmem_ld32(tQ, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-        tmem_ld32(tQ + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-        tmem_ld_wait();
-      } else {
+    return ok;
+  };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_LOAD));
+    constexpr uint32_t hi = sdesc_hi(1024);
+    if (warp == 0) {
+      if (lane == 0) {
+        // ------------------------------------------ TMA: Q, dO; dQ of the items
+        int q = 0;
+        int om[NT], oh[NT], ob[NT];
+        auto store_out = [&](int e, int n) {
+          if (!mbar_spin(bar(TE + e), n & 1, abort_flag, kDevTimeoutSoftmax)) return false;
+          const uint32_t src = base + OFF_T + e * 2 * TILE;
 #pragma unroll
-        for (int e = 0; e < 64; ++e) v[e] = 0u;  // no keys
-      }
-      if (tok < p.Lq) {
-        uint4* dst = reinterpret_cast<uint4*>(p.dq + b * p.dq_sB + h * p.dq_sH + tok * p.dq_sT + 64 * wg);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint32_t w4[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            w4[e] = pack_bf2(__uint_as_float(v[8 * c + 2 * e]) * kSmScale, __uint_as_float(v[8 * c + 2 * e + 1]) * kSmScale);
-          dst[c] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
+          for (int c = 0; c < 4; ++c)
+            if (om[e] * 128 + 64 * (c & 1) < p.Lq)  // 64-row boxes: the second may lie past the last row
+              tma_store_4d(&tdq, src + (c >> 1) * BOX128 + (c & 1) * BOX, 64 * (c >> 1), om[e] * 128 + 64 * (c & 1), oh[e],
+                           ob[e]);
+          tma_store_commit();
+          tma_store_wait_read();
+          return true;
+        };
+        for (QueryItems it(p); it.live(p) && ok; it.next(p)) {
+          if (it.cnt == 0) continue;
+          const int e = q % NT;
+          if (q >= NT && !(ok = store_out(e, q / NT - 1))) break;
+          mbar_expect_tx(bar(TF + e), 2 * TILE);
+          load_tile(base + OFF_T + e * 2 * TILE, &tq, bar(TF + e), 128 * it.m, it.h, it.b);
+          load_tile(base + OFF_T + e * 2 * TILE + TILE, &tdo, bar(TF + e), 128 * it.m, it.h, it.b);
+          om[e] = it.m;
+          oh[e] = it.h;
+          ob[e] = it.b;
+          ++q;
         }
+        for (int n = max(0, q - NT); n < q && ok; ++n) ok = store_out(n % NT, n / NT);
+        // no copy may still target shared memory when the CTA exits; the waits
+        // ignore the abort flag and share one limit
+        const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
+        bool drained = true;
+        for (int n = max(0, q - NT); n < q && drained; ++n)
+          drained = mbar_wait_until(bar(TF + n % NT), (n / NT) & 1, deadline);
       }
+    } else if (warp == 3) {
+      if (lane == 0) {
+        // ------------------------------------------------------ TMA: K and V
+        int k = 0;
+        for (QueryItems it(p); it.live(p) && ok; it.next(p)) {
+          const int hk = it.h / p.G;
+          for (int i = 0; i < it.cnt; ++i, ++k) {
+            const int ek = k % NK, ev = k % NV;
+            if (!(ok = mbar_spin(bar(KE + ek), ((k / NK) & 1) ^ 1, abort_flag, kDevTimeoutMma))) break;
+            mbar_expect_tx(bar(KF + ek), HALF);
+            load_half(base + OFF_K + ek * HALF, &tk, bar(KF + ek), 64 * i, hk, it.b);
+            if (!(ok = mbar_spin(bar(VE + ev), ((k / NV) & 1) ^ 1, abort_flag, kDevTimeoutMma))) {
+              ++k;  // this K is on its way, its V is not
+              break;
+            }
+            mbar_expect_tx(bar(VF + ev), HALF);
+            load_half(base + OFF_V + ev * HALF, &tv, bar(VF + ev), 64 * i, hk, it.b);
+          }
+        }
+        const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
+        bool drained = true;
+        for (int n = max(0, k - NK); n < k && drained; ++n)
+          drained = mbar_wait_until(bar(KF + n % NK), (n / NK) & 1, deadline);
+        const int v = ok ? k : k - 1;
+        for (int n = max(0, v - NV); n < v && drained; ++n)
+          drained = mbar_wait_until(bar(VF + n % NV), (n / NV) & 1, deadline);
+      }
+    } else if (warp == 1) {
+      // ------------------------------------- MMA: S = Q K^T, dP = dO V^T
+      constexpr uint32_t id_s = idesc_bf16_f32(128, 64, false, false);
+      int et = 0, ek = 0, ev = 0, g = 0;
+      uint32_t t_ph = 0, k_ph = 0, v_ph = 0, g_ph = 1;
+      for (QueryItems it(p); it.live(p) && ok; it.next(p)) {
+        const int cnt = __shfl_sync(0xffffffffu, it.cnt, 0);
+        if (cnt == 0) continue;
+        if (!wait(TF + et, t_ph, kDevTimeoutLoad)) break;
+        const uint32_t dq = sdesc_lo(base + OFF_T + et * 2 * TILE, 16), ddo = sdesc_lo(base + OFF_T + et * 2 * TILE + TILE, 16);
+        for (int i = 0; i < cnt; ++i) {
+          if (!wait(KF + ek, k_ph, kDevTimeoutLoad) || !wait(VF + ev, v_ph, kDevTimeoutLoad) ||
+              !wait(DQ + g, g_ph, kDevTimeoutMma))
+            break;
+          if (elect_one()) {
+            const uint32_t dk = sdesc_lo(base + OFF_K + ek * HALF, 16), dv = sdesc_lo(base + OFF_V + ev * HALF, 16);
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+              const uint32_t ka = ((kk >> 2) * BOX128 + (kk & 3) * 32) >> 4, kb = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
+              mma_bf16_ss_lo(tmem + 128 * g, dq + ka, hi, dk + kb, hi, id_s, kk > 0 ? 1u : 0u);
+            }
+#pragma unroll
+            for (int kk = 0; kk < 8; ++kk) {
+              const uint32_t ka = ((kk >> 2) * BOX128 + (kk & 3) * 32) >> 4, kb = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
+              mma_bf16_ss_lo(tmem + 128 * g + 64, ddo + ka, hi, dv + kb, hi, id_s, kk > 0 ? 1u : 0u);
+            }
+            mma_commit(bar(SF + g));
+            mma_commit(bar(VE + ev));
+          }
+          __syncwarp();
+          if (++ek == NK) ek = 0, k_ph ^= 1u;
+          if (++ev == NV) ev = 0, v_ph ^= 1u;
+          if (++g == NS) g = 0, g_ph ^= 1u;
+        }
+        if (++et == NT) et = 0, t_ph ^= 1u;
+      }
+      // every MMA issued has completed before TMEM is freed, also on the abort path
+      if (elect_one()) {
+        mma_commit(bar(DRAIN_S));
+        mbar_wait_until(bar(DRAIN_S), 0, globaltimer_ns() + kWaitLimitNs);
+      }
+      __syncwarp();
+    } else {
+      // ------------------------------------------------- MMA: dQ += dS K
+      constexpr uint32_t id_q = idesc_bf16_f32(128, 128, false, true);
+      int ek = 0, g = 0;
+      uint32_t g_ph = 0, o_ph = 1;
+      for (QueryItems it(p); it.live(p) && ok; it.next(p)) {
+        const int cnt = __shfl_sync(0xffffffffu, it.cnt, 0);
+        if (cnt == 0) continue;
+        const int valid = it.len - 64 * (it.cnt - 1);  // keys of the last step
+        const int tail = __shfl_sync(0xffffffffu, it.len < p.Lk ? valid : 64, 0);
+        for (int i = 0; i < cnt; ++i) {
+          // dS is in place, hence S has been computed from this K (which may be cleared now)
+          if (!wait(DS + g, g_ph, kDevTimeoutSoftmax)) break;
+          if (i == 0 && !wait(OE, o_ph, kDevTimeoutSoftmax)) break;  // dQ of the previous item has been read
+          if (tail < 64 && i + 1 == cnt) clear_half_rows(smem1k + OFF_K + ek * HALF, tail, lane);
+          if (elect_one()) {
+            const uint32_t dk = sdesc_lo(base + OFF_K + ek * HALF, BOX);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_bf16_ts_lo(tmem + ACC, tmem + 128 * g + 8 * kk, dk + ((kk * 2048) >> 4), hi, id_q,
+                             (i > 0 || kk > 0) ? 1u : 0u);
+            mma_commit(bar(DQ + g));
+            mma_commit(bar(KE + ek));
+          }
+          __syncwarp();
+          if (++ek == NK) ek = 0;
+          if (++g == NS) g = 0, g_ph ^= 1u;
+        }
+        o_ph ^= 1u;
+      }
+      if (elect_one()) {
+        mma_commit(bar(DRAIN_Q));
+        mbar_wait_until(bar(DRAIN_Q), 0, globaltimer_ns() + kWaitLimitNs);
+      }
+      __syncwarp();
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    // -------------------------------------------------- dS, and dQ of an item
+    const int g = (warp >> 2) - 1, q = warp & 3, row = q * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(q * 32) << 16;
+    const uint32_t tS = tmem + 128 * g + lane_off, tdP = tS + 64, tQ = tmem + ACC + lane_off;
+    const uint64_t sc2 = f2_pack(p.qk_scale, p.qk_scale);
+    int u = 0, j = 0, items = 0;  // steps, items with keys, items
+    uint32_t ph = 0;              // of this warpgroup's steps
+    // the row's log-sum-exp and delta, one item ahead
+    auto stat = [&](const QueryItems& it, const float* t) {
+      return it.live(p) ? __ldg(t + ((int64_t)it.b * p.H + it.h) * p.Lpad + 128 * it.m + row) : 0.f;
+    };
+    QueryItems it(p);
+    float lse_next = stat(it, p.lse), dlt_next = stat(it, p.delta);
+    while (it.live(p) && ok) {
+      const int m = it.m, h = it.h, b = it.b, len = it.len, cnt = it.cnt;
+      const float lse = lse_next, dlt = dlt_next;
+      it.next(p);
+      lse_next = stat(it, p.lse);
+      dlt_next = stat(it, p.delta);
+      if (cnt == 0) {
+        // no keys: zeros (one warpgroup in turn; no step, nothing to wait for)
+        const int tok = 128 * m + row;
+        if (items % 3 == g && tok < p.Lq) {
+          uint4* dst = reinterpret_cast<uint4*>(p.dq + b * p.dq_sB + h * p.dq_sH + tok * p.dq_sT);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) dst[c] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+        ++items;
+        continue;
+      }
+      const uint64_t nl2 = f2_pack(-lse, -lse), nd2 = f2_pack(-dlt, -dlt);
+      for (int i = 0; i < cnt; ++i, ++u) {
+        if (u % NS != g) continue;
+        if (!wait(SF + g, ph, kDevTimeoutMma)) break;
+        const int valid = len - 64 * i;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t sv[32], dv[32];
+          tmem_ld32(tS + 32 * c, sv);
+          tmem_ld32(tdP + 32 * c, dv);
+          tmem_ld_wait();
+          uint32_t w[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float x0, x1, d0, d1;
+            f2_unpack(fma_f32x2(f2_pack(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2, nl2), x0, x1);
+            const uint64_t pd = mul_f32x2(
+                f2_pack(ex2_approx(x0), ex2_approx(x1)),
+                add_f32x2(f2_pack(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])), nd2));
+            f2_unpack(pd, d0, d1);
+            w[e] = pack_bf2(d0, d1);
+          }
+          if (valid < 64) {  // by selection: past len[b] the products may be anything
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int col = 32 * c + 2 * e;
+              w[e] = col + 1 < valid ? w[e] : col < valid ? w[e] & 0xffffu : 0u;
+            }
+          }
+          tmem_st16(tS + 16 * c, w);  // packed dS over the first 32 S columns of the step
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(DS + g));
+        if (i + 1 == cnt) {
+          if (!wait(DQ + g, ph, kDevTimeoutMma)) break;
+          // the row of the item's Q tile, whose last product is done: 16-byte chunk c of a
+          // box at c ^ (row & 7), the maps' swizzle
+          uint8_t* stage = smem1k + OFF_T + (j % NT) * 2 * TILE + row * 128;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            uint32_t v[64];
+            tmem_ld32(tQ + 64 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+            tmem_ld32(tQ + 64 * c + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+            tmem_ld_wait();
+            if (c == 1) {
+              // dQ is in registers: the next item may start its own
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(bar(OE));
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              uint32_t w4[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                w4[k] = pack_bf2(__uint_as_float(v[8 * e + 2 * k]) * bwd::kSmScale,
+                                 __uint_as_float(v[8 * e + 2 * k + 1]) * bwd::kSmScale);
+              *reinterpret_cast<uint4*>(stage + c * BOX128 + ((e ^ (row & 7)) << 4)) =
+                  make_uint4(w4[0], w4[1], w4[2], w4[3]);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(TE + j % NT));
+        }
+        ph ^= 1u;
+      }
+      ++j;
+      ++items;
     }
   }
   tc_fence_before();
@@ -493,14 +675,16 @@ int cross_bwd_splits(int B, int H, int Hkv, int Lq, int Lk) {
 }
 
 int launch_cross_attn_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
-                          const CrossBwdParams& p, cudaStream_t s) {
+                          const CUtensorMap& tdq, const CrossBwdParams& p, cudaStream_t s) {
   using namespace bwd;
   static KernelReady ready_dq, ready_dkdv;
-  int rc = kernel_ready(ready_dq, cross_bwd_dq_tcgen05, DQ_SMEM);
+  int rc = kernel_ready(ready_dq, cross_bwd_dq_tcgen05, xdq::SMEM, xdq::LAUNCH_REGS);
   if (rc == 0) rc = kernel_ready(ready_dkdv, cross_bwd_dkdv_tcgen05, KV_SMEM);
   if (rc != 0) return rc;
   cudaError_t e;
-  cross_bwd_dq_tcgen05<<<(unsigned)((int64_t)p.NQT * p.B * p.H), DQ_THREADS, DQ_SMEM, s>>>(tq, tk, tv, tdo, p);
+  const int64_t items = (int64_t)p.NQT * p.B * p.H;
+  const int sms = device_sms();
+  cross_bwd_dq_tcgen05<<<(unsigned)(items < sms ? items : sms), xdq::THREADS, xdq::SMEM, s>>>(tq, tk, tv, tdo, tdq, p);
   if ((e = cudaGetLastError()) != cudaSuccess) return (int)e;
   cross_bwd_dkdv_tcgen05<<<(unsigned)((int64_t)p.NKT * p.B * p.Hkv * p.nsplit), THREADS, KV_SMEM, s>>>(tq, tk, tv, tdo,
                                                                                                   p);

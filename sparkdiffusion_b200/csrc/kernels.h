@@ -267,7 +267,8 @@ struct CrossBwdParams {
   float qk_scale;
 };
 int cross_bwd_splits(int B, int H, int Hkv, int Lq, int Lk);
+// 64-row boxes; tdq: the output dq
 int launch_cross_attn_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
-                          const CrossBwdParams& p, cudaStream_t s);
+                          const CUtensorMap& tdq, const CrossBwdParams& p, cudaStream_t s);
 
 }  // namespace rola
