@@ -1016,6 +1016,12 @@ def cross_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: to
         raise ValueError(f"{what}: o and do must have q's shape, o in bf16")
     if lse.dtype is not torch.float32 or lse.shape != (B * H, lse_rows(Lq)) or not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be the forward's")
+    return _cross_bwd(dev, sizes, q, k, v, o, do, lse, lens)
+
+
+def _cross_bwd(dev: int, sizes: tuple, q, k, v, o, do, lse, lens):
+    """``cross_attention_bwd`` of checked arguments (the autograd function's are its own forward's)."""
+    B, H, Hkv, Lq, Lk = sizes
     dq = _token_major_empty(B, H, Lq, q.device)
     dk, dv = _token_major_empty(B, Hkv, Lk, q.device), _token_major_empty(B, Hkv, Lk, q.device)
     if q.numel() == 0 or k.numel() == 0:
@@ -1024,7 +1030,7 @@ def cross_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: to
     do, da = _head_args(do if do.dtype is BF16 else do.to(BF16))
     nb = _lib.lib().rola_b200_cross_attn_bwd_workspace(*sizes)
     if nb == 0:
-        raise ValueError(f"{what}: bad sizes")
+        raise ValueError("cross_attention_bwd: bad sizes")
     ws = torch.empty(nb, device=q.device, dtype=torch.uint8)
     _call_on(dev, "rola_b200_cross_attn_bwd", *qa, *ka, *va, *oa, *da, _ptr(lens), lse.data_ptr(), *sizes,
              dq.data_ptr(), Lq * H * HEAD_DIM, HEAD_DIM, H * HEAD_DIM, dk.data_ptr(), dv.data_ptr(),

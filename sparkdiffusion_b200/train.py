@@ -180,6 +180,17 @@ def dense_training_forward(layer, x: torch.Tensor, freqs: torch.Tensor) -> torch
     return layer.o(o.transpose(1, 2).reshape(b, s, n * d))
 
 
+def _differentiable_once(backward):
+    """``once_differentiable`` where a graph of the gradient is asked for (its
+    own differentiation then raises); without one, nothing around the kernels."""
+    once = once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
 class AddRMSNorm(torch.autograd.Function):
     """``ops.add_rms_norm`` with its backward kernel; saves h and the row factors."""
 
@@ -193,7 +204,7 @@ class AddRMSNorm(torch.autograd.Function):
         return (y, h) if residual is not None else y
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, dy, dh=None):
         h, weight, rstd = ctx.saved_tensors
         if dy is None:
@@ -222,10 +233,12 @@ class CrossAttention(torch.autograd.Function):
         return o
 
     @staticmethod
-    @once_differentiable
+    @_differentiable_once
     def backward(ctx, do):
-        q, k, v, o, lse, kv_lens = ctx.saved_tensors
-        return (*ops.cross_attention_bwd(q, k, v, o, do, lse, kv_lens), None)
+        q, k, v, o, lse, lens = ctx.saved_tensors
+        B, H, Lq, _ = q.shape
+        lens = None if lens is None else lens.contiguous()
+        return (*ops._cross_bwd(q.get_device(), (B, H, k.shape[1], Lq, k.shape[2]), q, k, v, o, do, lse, lens), None)
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -235,6 +248,6 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     ``dense_attention``, which takes one length."""
     if not q.is_cuda:
         raise RuntimeError("the B200 training path runs on CUDA tensors only")
-    dt = q.dtype
-    o = CrossAttention.apply(*(t.to(torch.bfloat16) for t in (q, k, v)), kv_lens)
-    return o if dt == torch.bfloat16 else o.to(dt)
+    dt, bf16 = q.dtype, torch.bfloat16
+    o = CrossAttention.apply(*(t if t.dtype is bf16 else t.to(bf16) for t in (q, k, v)), kv_lens)
+    return o if dt is bf16 else o.to(dt)
