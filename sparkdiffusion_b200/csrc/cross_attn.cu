@@ -614,8 +614,11 @@ __global__ void cross_lse_pad_kernel(float* lse, int64_t rows, int Lq, int ld) {
   if (g < rows * pad) lse[(g / pad) * ld + Lq + g % pad] = INFINITY;
 }
 
-// How the keys are cut: with at least one item per SM they are not (every slice
-// costs an fp32 partial); with fewer, into slices of two key tiles or more.
+// How the keys are cut: into as many slices as give every SM one item at most
+// (a second, partly filled round costs more than it balances: 32 items of 64 key
+// tiles in us, slices 1 | 4 | 5 | 8: 57 | 29 | 40 | 32), of 8 key tiles or more (a
+// slice costs its ends and an fp32 partial: 12 items of 64 tiles, 8 | 12 slices:
+// 17.8 | 19.2; 12 items of 4 tiles, 1 | 2: 9.5 | 11.9).
 CrossAttnPlan cross_attn_plan(int B, int H, int Hkv, int Lq, int Lk) {
   CrossAttnPlan pl{};
   const int G = H / Hkv;
@@ -624,10 +627,8 @@ CrossAttnPlan cross_attn_plan(int B, int H, int Hkv, int Lq, int Lk) {
   const int64_t items = (int64_t)pl.nqt * B * (pl.pack ? Hkv : H);
   const int ntk = (Lk + 127) / 128, sms = device_sms();
   pl.nsplit = 1;
-  if (items < sms && ntk >= 4) {
-    const int64_t want = (sms + items - 1) / items;
-    pl.nsplit = (int)(want < ntk / 2 ? want : ntk / 2);
-  }
+  const int64_t most = sms / items;
+  if (most > 1 && ntk >= 16) pl.nsplit = (int)(most < ntk / 8 ? most : ntk / 8);
   return pl;
 }
 

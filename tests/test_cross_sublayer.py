@@ -38,6 +38,8 @@ ATTENTION = {
     "two_keys": (1, 2, 2, 3, 2, None),
     "one_token_split": (2, 3, 3, 1, 5000, (4999, 37)),
     "one_token_groups": (2, 10, 2, 1, 1100, (1100, 513)),
+    "one_token_groups_split": (2, 10, 2, 1, 2300, (2300, 130)),
+    "few_rows_split": (1, 2, 2, 130, 3000, None),
     "packed_128_rows": (1, 8, 1, 16, 700, (641,)),
     "unpacked_136_rows": (1, 8, 1, 17, 700, (641,)),
     "row_tail": (1, 2, 2, 129, 64, None),
