@@ -724,6 +724,11 @@ def _call_on(dev: int, name: str, *args) -> None:
         _lib.check(rc, name)
 
 
+def _empty_as(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A new dense tensor of ``t``'s shape."""
+    return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
+
+
 def _rows(t: torch.Tensor, K: int, what: str) -> tuple[torch.Tensor, int, int, int]:
     """``t [..., K]`` (bf16 or fp32) as rows the kernels take, unit column stride
     and 16-byte rows (copied where it is not): ``(rows, address, is fp32, row stride)``."""
@@ -767,7 +772,7 @@ def _norm_args(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | N
         if residual.shape != x.shape:
             raise ValueError(f"{what}: residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
         rr, rp, rf, r_ld = _rows(residual, K, what)
-        h = torch.empty(x.shape, device=x.device, dtype=residual.dtype)
+        h = _empty_as(x, residual.dtype)
     w, wf = _norm_weight(weight, K, what)
     M = xr.shape[0]
     # the rows travel along: a copy made above has to live until its kernel is launched
@@ -783,7 +788,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, resid
     the row factors.  Beside ``train.rms_norm``; differentiable as
     ``train.add_rms_norm``."""
     dev, M, K, head, h, keep = _norm_args(x, weight, residual, "add_rms_norm")
-    y = torch.empty(x.shape, device=x.device, dtype=BF16)
+    y = _empty_as(x, BF16)
     if rstd is not None and (rstd.get_device() != dev or rstd.dtype != torch.float32 or rstd.numel() != M
                              or not rstd.is_contiguous()):
         raise ValueError("add_rms_norm: rstd must be a contiguous fp32 tensor of one value per row")
@@ -806,7 +811,7 @@ def add_rms_norm_e4m3(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6, 
     if block not in (SCALE_BLOCK, None):
         raise ValueError("add_rms_norm_e4m3: block must be 128, or None for one scale per row")
     dev, M, K, head, h, keep = _norm_args(x, weight, residual, "add_rms_norm_e4m3")
-    yq = torch.empty(x.shape, device=x.device, dtype=E4M3)
+    yq = _empty_as(x, E4M3)
     if block is None:
         scale, sM, sK, blk = torch.empty(M, device=x.device, dtype=torch.float32), 1, 0, 0
     else:
@@ -840,12 +845,12 @@ def add_rms_norm_bwd(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, 
     if rstd.dtype != torch.float32 or rstd.numel() != M or not rstd.is_contiguous():
         raise ValueError(f"{what}: rstd must be add_rms_norm's row factors")
     w, wf = _norm_weight(weight, K, what)
-    dx = torch.empty(h.shape, device=h.device, dtype=x_dtype)
+    dx = _empty_as(h, x_dtype)
     dres = None if res_dtype is None else dx if res_dtype == x_dtype else torch.empty_like(dx, dtype=res_dtype)
     dw = None if not need_dw else torch.empty_like(w) if M else torch.zeros_like(w)
     if M:
         nb = _lib.lib().rola_b200_add_rms_norm_bwd_workspace(M, K) if need_dw else 0
-        ws = torch.empty(nb, device=h.device, dtype=torch.uint8) if nb else None
+        ws = h.new_empty(nb, dtype=torch.uint8) if nb else None
         _call_on(dev, "rola_b200_add_rms_norm_bwd", hp, hf, h_ld, w.data_ptr(), wf, rstd.data_ptr(), yp, dy_ld, dp, df,
                  dh_ld, M, K, dx.data_ptr(), int(x_dtype is torch.float32), None if dres is dx else _ptr(dres),
                  int(res_dtype is torch.float32), _ptr(dw), _ptr(ws), nb)
@@ -862,7 +867,7 @@ def quantize_blocks_e4m3(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise ValueError(f"{what}: [M, K] with K a multiple of 8, at most 16384, required")
     M, K = x.shape
     xr, xp, xf, ld = _rows(x, K, what)
-    xq = torch.empty(M, K, device=x.device, dtype=E4M3)
+    xq = _empty_as(x, E4M3)
     scale = _block_scales(M, K, x.device)
     if M:
         _call_on(dev, "rola_b200_quantize_blocks_e4m3", xp, xf, ld, M, K, xq.data_ptr(), scale.data_ptr(), 1, M)
@@ -879,7 +884,7 @@ def quantize_tiles_e4m3(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise ValueError(f"{what}: [N, K] with K a multiple of 8, both at most 65536, required")
     N, K = w.shape
     wr, wp, wf, ld = _rows(w, K, what)
-    wq = torch.empty(N, K, device=w.device, dtype=E4M3)
+    wq = _empty_as(w, E4M3)
     scale = torch.empty((N + 127) // 128, (K + 127) // 128, device=w.device, dtype=torch.float32)
     _call_on(dev, "rola_b200_quantize_tiles_e4m3", wp, wf, ld, N, K, wq.data_ptr(), scale.data_ptr())
     return wq, scale
@@ -918,7 +923,7 @@ def gemm_fp8_block(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_
         bias = _dense16(bias if bias.dtype is BF16 else bias.to(BF16))
     xq, wq = _dense16(xq), _dense16(wq)
     w_scale = w_scale.contiguous()
-    out = torch.empty(M, N, device=xq.device, dtype=BF16)
+    out = xq.new_empty((M, N), dtype=BF16)
     if M:
         sM, sK = x_scale.stride()
         _call_on(dev, "rola_b200_gemm_fp8_block", xq.data_ptr(), x_scale.data_ptr(), sM, sK, wq.data_ptr(),
@@ -976,14 +981,14 @@ def cross_attention_fwd_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k
     dev, sizes, lens = _cross_args("cross_attention", q, k, v, kv_lens)
     B, H, Hkv, Lq, Lk = sizes
     o = _token_major_empty(B, H, Lq, q.device)
-    lse = torch.empty(B * H, lse_rows(Lq), device=q.device, dtype=torch.float32) if need_lse else None
+    lse = q.new_empty((B * H, lse_rows(Lq)), dtype=torch.float32) if need_lse else None
     if B == 0 or H == 0 or Lq == 0:
         return o, lse
     if Lk == 0:
         return o.zero_(), None if lse is None else lse.fill_(float("inf"))
     (q, qa), (k, ka), (v, va) = _head_args(q), _head_args(k), _head_args(v)
     nb = _lib.lib().rola_b200_cross_attn_workspace(*sizes)
-    ws = torch.empty(nb, device=q.device, dtype=torch.uint8) if nb else None
+    ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
     _call_on(dev, "rola_b200_cross_attn", *qa, *ka, *va, _ptr(lens), *sizes, o.data_ptr(), Lq * H * HEAD_DIM, HEAD_DIM,
              H * HEAD_DIM, _ptr(lse), _ptr(ws), nb)
     return o, lse
@@ -1031,7 +1036,7 @@ def _cross_bwd(dev: int, sizes: tuple, q, k, v, o, do, lse, lens):
     nb = _lib.lib().rola_b200_cross_attn_bwd_workspace(*sizes)
     if nb == 0:
         raise ValueError("cross_attention_bwd: bad sizes")
-    ws = torch.empty(nb, device=q.device, dtype=torch.uint8)
+    ws = q.new_empty(nb, dtype=torch.uint8)
     _call_on(dev, "rola_b200_cross_attn_bwd", *qa, *ka, *va, *oa, *da, _ptr(lens), lse.data_ptr(), *sizes,
              dq.data_ptr(), Lq * H * HEAD_DIM, HEAD_DIM, H * HEAD_DIM, dk.data_ptr(), dv.data_ptr(),
              Lk * Hkv * HEAD_DIM, HEAD_DIM, Hkv * HEAD_DIM, ws.data_ptr(), nb)

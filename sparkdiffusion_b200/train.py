@@ -196,7 +196,7 @@ class AddRMSNorm(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, eps: float, residual):
-        rstd = torch.empty(x.numel() // max(1, x.shape[-1]), device=x.device, dtype=torch.float32)
+        rstd = x.new_empty(x.numel() // max(1, x.shape[-1]), dtype=torch.float32)
         y, h = ops.add_rms_norm(x, weight, eps, residual, rstd=rstd)
         ctx.save_for_backward(h, weight, rstd)
         ctx.x_dtype, ctx.res_dtype = x.dtype, None if residual is None else residual.dtype
