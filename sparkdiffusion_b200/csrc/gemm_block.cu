@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
         tile_coords(lt, m0, n0);
         for (int kb = 0; kb < nk; ++kb, ++it) {
           const int s = it % C::STAGES;
-          if (!mbar_wait(empty(s), ((it / C::STAGES) & 1) ^ 1, abort_flag, kDevTimeoutMma)) {
+          if (!mbar_spin(empty(s), ((it / C::STAGES) & 1) ^ 1, abort_flag, kDevTimeoutMma)) {
             ok = false;
             break;
           }
@@ -192,12 +192,12 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
       bool ok = true;
       for (int it = 0; it < total && ok; ++it) {
         const int a = it % C::NBUF, s = it % C::STAGES;
-        ok = mbar_wait(full(s), (it / C::STAGES) & 1, abort_flag, kDevTimeoutLoad);
+        ok = mbar_spin(full(s), (it / C::STAGES) & 1, abort_flag, kDevTimeoutLoad);
         const uint32_t sa = base + s * C::STAGE, sb = sa + C::A_BYTES;
 #pragma unroll
         for (int h = 0; h < C::STREAMS; ++h) {
           // the epilogue has read this accumulator (block it - NBUF)
-          ok = ok && mbar_wait(acc_empty(h, a), ((it / C::NBUF) & 1) ^ 1, abort_flag, kDevTimeoutSoftmax);
+          ok = ok && mbar_spin(acc_empty(h, a), ((it / C::NBUF) & 1) ^ 1, abort_flag, kDevTimeoutSoftmax);
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
       const float* ws = p.ws + (int64_t)min((n0 >> 7) + lane % C::STREAMS, (p.N - 1) >> 7) * p.ws_ld;
       for (int kb = 0; kb < nk; ++kb, ++it) {
         const int c = it % kScales;
-        ok = __all_sync(0xffffffffu, mbar_wait(sc_empty(c), ((it / kScales) & 1) ^ 1, abort_flag, kDevTimeoutSoftmax));
+        ok = __all_sync(0xffffffffu, mbar_spin(sc_empty(c), ((it / kScales) & 1) ^ 1, abort_flag, kDevTimeoutSoftmax));
         if (!ok) break;
         const uint32_t dst = base + C::OFF_SC + c * C::SC_FLOATS * 4;
 #pragma unroll
@@ -254,12 +254,12 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
         for (int i = 0; i < 16; ++i) acc[c][i] = 0ull;
       for (int kb = 0; kb < nk; ++kb, ++it) {
         const int a = it % C::NBUF, c = it % kScales;
-        ok = __all_sync(0xffffffffu, mbar_wait(sc_full(c), (it / kScales) & 1, abort_flag, kDevTimeoutLoad));
+        ok = __all_sync(0xffffffffu, mbar_spin(sc_full(c), (it / kScales) & 1, abort_flag, kDevTimeoutLoad));
         if (!ok) break;
         const float* sc = reinterpret_cast<const float*>(gbase + C::OFF_SC) + c * C::SC_FLOATS;
         const float s = sc[row] * sc[128 + h];
         const uint64_t s2 = f2_pack(s, s);
-        ok = __all_sync(0xffffffffu, mbar_wait(acc_full(h, a), (it / C::NBUF) & 1, abort_flag, kDevTimeoutMma));
+        ok = __all_sync(0xffffffffu, mbar_spin(acc_full(h, a), (it / C::NBUF) & 1, abort_flag, kDevTimeoutMma));
         if (!ok) break;
         if (lane == 0) mbar_arrive(sc_empty(c));
         tc_fence_after();
