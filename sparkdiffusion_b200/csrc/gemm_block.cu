@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
     const int q = warp & 3, group = (warp - 4) >> 2, h = C::STREAMS == 2 ? group : 0;
     const int row = q * 32 + lane;
     int it = 0;
-    bool ok = true;
+    bool ok = true, ready = false;
     for (int lt = 0; lt < my_tiles && ok; ++lt) {
       int m0, n0;
       tile_coords(lt, m0, n0);
@@ -253,31 +253,39 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[c][i] = 0ull;
       for (int kb = 0; kb < nk; ++kb, ++it) {
+        // the block's scales and accumulator (`ready`: found complete while the block
+        // before was still being added, so that the answer costs no time of its own)
         const int a = it % C::NBUF, c = it % kScales;
-        ok = __all_sync(0xffffffffu, mbar_spin(sc_full(c), (it / kScales) & 1, abort_flag, kDevTimeoutLoad));
-        if (!ok) break;
-        const float* sc = reinterpret_cast<const float*>(gbase + C::OFF_SC) + c * C::SC_FLOATS;
-        const float s = sc[row] * sc[128 + h];
-        const uint64_t s2 = f2_pack(s, s);
-        ok = __all_sync(0xffffffffu, mbar_spin(acc_full(h, a), (it / C::NBUF) & 1, abort_flag, kDevTimeoutMma));
-        if (!ok) break;
-        if (lane == 0) mbar_arrive(sc_empty(c));
+        if (!__all_sync(0xffffffffu, ready)) {
+          const bool got = mbar_spin(sc_full(c), (it / kScales) & 1, abort_flag, kDevTimeoutLoad) &&
+                           mbar_spin(acc_full(h, a), (it / C::NBUF) & 1, abort_flag, kDevTimeoutMma);
+          ok = __all_sync(0xffffffffu, got);
+          if (!ok) break;
+        }
         tc_fence_after();
         const uint32_t t = tmem + 128 * (C::NBUF * h + a) + (C::CW * group) % 128 + ((uint32_t)(q * 32) << 16);
         uint32_t v[2][32];
         tmem_ld32(t, v[0]);
+        const float* sc = reinterpret_cast<const float*>(gbase + C::OFF_SC) + c * C::SC_FLOATS;
+        const float s = sc[row] * sc[128 + h];
+        const uint64_t s2 = f2_pack(s, s);
 #pragma unroll
-        for (int c = 0; c < C::CW / 32; ++c) {
+        for (int i = 0; i < C::CW / 32; ++i) {
           tmem_ld_wait();
-          if (c + 1 < C::CW / 32) {
-            tmem_ld32(t + 32 * (c + 1), v[(c + 1) & 1]);
+          if (i + 1 < C::CW / 32) {
+            tmem_ld32(t + 32 * (i + 1), v[(i + 1) & 1]);
           } else {
             // the warp's part is in registers: the block NBUF further may overwrite it
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty(h, a));
+            if (lane == 0) {
+              mbar_arrive(acc_empty(h, a));
+              mbar_arrive(sc_empty(c));
+            }
+            const int n = it + 1;
+            ready = mbar_test(sc_full(n % kScales), (n / kScales) & 1) & mbar_test(acc_full(h, n % C::NBUF), (n / C::NBUF) & 1);
           }
-          scaled_add(acc[c], v[c & 1], s2);
+          scaled_add(acc[i], v[i & 1], s2);
         }
       }
       if (ok && m < p.M) {
