@@ -47,11 +47,11 @@ __device__ __forceinline__ void load8(const void* base, bool fp32, int64_t off, 
 __device__ __forceinline__ void store8(void* base, bool fp32, int64_t off, const float (&v)[8]) {
   if (fp32) {
     float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + off);
-    p[0] = make_float4(v[0], v[1], v[2], v[3]);
-    p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    __stcs(p, make_float4(v[0], v[1], v[2], v[3]));
+    __stcs(p + 1, make_float4(v[4], v[5], v[6], v[7]));
   } else {
-    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(base) + off) =
-        make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7]));
+    __stcs(reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(base) + off),
+           make_uint4(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]), pack_bf2(v[4], v[5]), pack_bf2(v[6], v[7])));
   }
 }
 // maximum that keeps a NaN of either side
