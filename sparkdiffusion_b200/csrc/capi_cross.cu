@@ -258,9 +258,7 @@ int rola_b200_cross_attn_bwd(const void* q, int64_t q_sB, int64_t q_sH, int64_t 
   p.B = B, p.H = H, p.Hkv = Hkv, p.G = H / Hkv, p.Lq = Lq, p.Lk = Lk;
   p.NQT = (Lq + 127) / 128, p.NKT = (Lk + 127) / 128, p.Lpad = 128 * p.NQT, p.nsplit = f.nsplit;
   p.qk_scale = (float)(0.08838834764831845 * 1.4426950408889634);
-  ROLA_TRY(cuda_status(launch_attn_bwd_delta(BF(out), o_sB, o_sH, o_sT, BF(dout), do_sB, do_sH, do_sT, B, H, Lq,
-                                             p.Lpad, const_cast<float*>(p.delta), S(stream)),
-                       "cross_attn_bwd/delta"));
+  p.o = BF(out), p.o_sB = o_sB, p.o_sH = o_sH, p.o_sT = o_sT;
   return cuda_status(launch_cross_attn_bwd(tq, tk, tv, tdo, tdq, p, S(stream)), what);
 }
 

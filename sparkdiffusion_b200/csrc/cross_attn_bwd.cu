@@ -1,7 +1,7 @@
 // Backward of the attention to another sequence's states (cross_attn.cu), on
 // tcgen05, without atomics.  From the forward's base-2 log-sum-exp:
 //
-//   delta[i] = sum_d dO[i, d] O[i, d]                  (attn_bwd_delta_kernel)
+//   delta[i] = sum_d dO[i, d] O[i, d]   (by the way, in the dq kernel, which has dO)
 //   P  = exp2(q.k D^-1/2 log2(e) - lse[i])             (recomputed, fp32; 0 past len[b])
 //   dP = dO V^T,  dS = P (dP - delta[i])
 //   dQ = D^-1/2 dS K                    query-stationary   (cross_bwd_dq_tcgen05)
@@ -42,19 +42,25 @@ __device__ __forceinline__ void clear_half_rows(uint8_t* half, int valid, int la
 //   warp 2   issues dQ; clears the K rows past len[b] first
 //   warpgroups 1-3: dS of the steps u with u % 3 == warpgroup - 1 (thread = row);
 //            the step that ends an item leaves its dQ in bf16
+//   warpgroup 4  delta of the items ahead, for this kernel and the next: dO from
+//            shared memory, O from global memory (a kernel of its own read dO once more
+//            and took 0.13 ms)
 // ---------------------------------------------------------------------------
 namespace xdq {
-constexpr int THREADS = 512, LAUNCH_REGS = 128, REGS_LOAD = 56, REGS_SOFTMAX = 152;
-static_assert(128 * (REGS_LOAD + 3 * REGS_SOFTMAX) <= THREADS * LAUNCH_REGS, "register split");
+constexpr int THREADS = 640, LAUNCH_REGS = 96;  // 65536 / 640, in steps of 8
+constexpr int REGS_LOAD = 56, REGS_SOFTMAX = 112, REGS_DELTA = 88;
+static_assert(128 * (REGS_LOAD + 3 * REGS_SOFTMAX + REGS_DELTA) <= THREADS * LAUNCH_REGS, "register split");
 constexpr int NT = 2, NK = 4, NV = 2, NS = 3;
 constexpr int OFF_T = 0;                                // NT x (Q, dO)
 constexpr int OFF_K = OFF_T + NT * 2 * bwd::TILE, OFF_V = OFF_K + NK * bwd::HALF;
-constexpr int OFF_BAR = OFF_V + NV * bwd::HALF;
+constexpr int OFF_DELTA = OFF_V + NV * bwd::HALF;       // [NT][128]
+constexpr int OFF_BAR = OFF_DELTA + NT * 512;
 constexpr int SMEM = OFF_BAR + 384;
 constexpr int ACC = 128 * NS;                           // TMEM: S of step u at 128 (u % 3), dP 64 behind, dQ at ACC
 enum : int {
   TF = 0, TE = TF + NT,  // TE: the item's dQ is in its Q tile, 4 warp arrivals
-  KF = TE + NT, KE = KF + NK, VF = KE + NK, VE = VF + NV,
+  DR = TE + NT,          // delta of the item's rows in shared memory, 4 arrivals
+  KF = DR + NT, KE = KF + NK, VF = KE + NK, VE = VF + NV,
   SF = VE + NV,          // S and dP of a step in TMEM
   DS = SF + NS,          // dS of a step in TMEM, 4 arrivals
   DQ = DS + NS,          // dQ of a step done
@@ -285,6 +291,39 @@ __global__ void __launch_bounds__(xdq::THREADS, 1)
       }
       __syncwarp();
     }
+  } else if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_DELTA));
+    // ------------------------------------------------------------------ delta
+    const int row = (warp & 3) * 32 + lane;
+    int j = 0;
+    for (QueryItems it(p); it.live(p) && ok; it.next(p)) {
+      if (it.cnt == 0) continue;
+      const int e = j % NT, tok = 128 * it.m + row;
+      const uint8_t* dos = smem1k + OFF_T + e * 2 * TILE + TILE + row * 128;
+      const uint4* o = reinterpret_cast<const uint4*>(p.o + it.b * p.o_sB + it.h * p.o_sH + (int64_t)min(tok, p.Lq - 1) * p.o_sT);
+      if (!wait(TF + e, (j / NT) & 1, kDevTimeoutLoad)) break;
+      float acc = 0.f;
+#pragma unroll
+      for (int c = 0; c < 16; ++c) {
+        const uint4 ov = __ldg(o + c);
+        const uint4 dv = *reinterpret_cast<const uint4*>(dos + (c >> 3) * BOX128 + (((c & 7) ^ (row & 7)) << 4));
+        const uint32_t oa[4] = {ov.x, ov.y, ov.z, ov.w}, da[4] = {dv.x, dv.y, dv.z, dv.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float o0, o1, d0, d1;
+          unpack_bf2(oa[k], o0, o1);
+          unpack_bf2(da[k], d0, d1);
+          acc = fmaf(o0, d0, acc);
+          acc = fmaf(o1, d1, acc);
+        }
+      }
+      if (tok >= p.Lq) acc = 0.f;  // a padding row (its P is 0, its delta has to be a number)
+      reinterpret_cast<float*>(smem1k + OFF_DELTA)[e * 128 + row] = acc;
+      p.delta[((int64_t)it.b * p.H + it.h) * p.Lpad + tok] = acc;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(DR + e));
+      ++j;
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
     // -------------------------------------------------- dS, and dQ of an item
@@ -294,18 +333,17 @@ __global__ void __launch_bounds__(xdq::THREADS, 1)
     const uint64_t sc2 = f2_pack(p.qk_scale, p.qk_scale);
     int u = 0, j = 0, items = 0;  // steps, items with keys, items
     uint32_t ph = 0;              // of this warpgroup's steps
-    // the row's log-sum-exp and delta, one item ahead
-    auto stat = [&](const QueryItems& it, const float* t) {
-      return it.live(p) ? __ldg(t + ((int64_t)it.b * p.H + it.h) * p.Lpad + 128 * it.m + row) : 0.f;
+    // the row's log-sum-exp, one item ahead
+    auto stat = [&](const QueryItems& it) {
+      return it.live(p) ? __ldg(p.lse + ((int64_t)it.b * p.H + it.h) * p.Lpad + 128 * it.m + row) : 0.f;
     };
     QueryItems it(p);
-    float lse_next = stat(it, p.lse), dlt_next = stat(it, p.delta);
+    float lse_next = stat(it);
     while (it.live(p) && ok) {
       const int m = it.m, h = it.h, b = it.b, len = it.len, cnt = it.cnt;
-      const float lse = lse_next, dlt = dlt_next;
+      const float lse = lse_next;
       it.next(p);
-      lse_next = stat(it, p.lse);
-      dlt_next = stat(it, p.delta);
+      lse_next = stat(it);
       if (cnt == 0) {
         // no keys: zeros (one warpgroup in turn; no step, nothing to wait for)
         const int tok = 128 * m + row;
@@ -318,6 +356,8 @@ __global__ void __launch_bounds__(xdq::THREADS, 1)
         ++items;
         continue;
       }
+      if (!wait(DR + j % NT, (j / NT) & 1, kDevTimeoutSoftmax)) break;
+      const float dlt = reinterpret_cast<const float*>(smem1k + OFF_DELTA)[(j % NT) * 128 + row];
       const uint64_t nl2 = f2_pack(-lse, -lse), nd2 = f2_pack(-dlt, -dlt);
       for (int i = 0; i < cnt; ++i, ++u) {
         if (u % NS != g) continue;

@@ -257,7 +257,9 @@ int launch_cross_attn(const CUtensorMap& tq, const CUtensorMap& tk, const CUtens
 struct CrossBwdParams {
   const int32_t* kv_lens;
   const float* lse;    // [B*H, Lpad]
-  const float* delta;  // [B*H, Lpad]
+  float* delta;        // [B*H, Lpad], written by the dq kernel
+  const __nv_bfloat16* o;  // the forward's output
+  int64_t o_sB, o_sH, o_sT;
   __nv_bfloat16* dq;
   __nv_bfloat16* dk;
   __nv_bfloat16* dv;
