@@ -144,7 +144,7 @@ static int check_cross_sizes(int B, int H, int Hkv, int Lq, int Lk, const char* 
   ROLA_CHECK(B > 0 && H > 0 && Hkv > 0 && Lq > 0 && Lk > 0, "%s: bad sizes", what);
   ROLA_CHECK(H % Hkv == 0, "%s: the query heads must be a multiple of the key heads", what);
   ROLA_CHECK(Lq < (1 << 30) && Lk < (1 << 30), "%s: sequence too long", what);
-  ROLA_CHECK((int64_t)B * H * ((Lq + 63) / 64) < (1ll << 31) && (int64_t)B * H * ((Lk + 127) / 128) * 12 < (1ll << 31),
+  ROLA_CHECK((int64_t)B * H * ((Lq + 63) / 64) < (1ll << 31) && (int64_t)B * H * ((Lk + 127) / 128) * 8 < (1ll << 31),
              "%s: too many tiles", what);
   return ROLA_OK;
 }
@@ -204,15 +204,13 @@ int rola_b200_cross_attn(const void* q, int64_t q_sB, int64_t q_sH, int64_t q_sT
 
 struct CrossBwdLayout {
   size_t delta, part, total;
-  int nsplit;
+  int runs;
 };
 static CrossBwdLayout cross_bwd_layout(int B, int H, int Hkv, int Lq, int Lk) {
   CrossBwdLayout f{};
-  f.nsplit = cross_bwd_splits(B, H, Hkv, Lq, Lk);
-  f.delta = 0;
+  f.runs = cross_bwd_runs(B, H, Hkv, Lq, Lk);
   f.part = align256((size_t)B * H * (128 * (((size_t)Lq + 127) / 128)) * 4);
-  f.total = f.part;
-  if (f.nsplit > 1) f.total += 2 * (size_t)f.nsplit * B * Hkv * (128 * (((size_t)Lk + 127) / 128)) * 128 * 4;
+  f.total = f.part + (size_t)2 * f.runs * 2 * 128 * 128 * 4;
   return f;
 }
 
@@ -256,7 +254,7 @@ int rola_b200_cross_attn_bwd(const void* q, int64_t q_sB, int64_t q_sH, int64_t 
   p.dq = BFm(dq), p.dq_sB = dq_sB, p.dq_sH = dq_sH, p.dq_sT = dq_sT;
   p.dk = BFm(dk), p.dv = BFm(dv), p.dkv_sB = dkv_sB, p.dkv_sH = dkv_sH, p.dkv_sT = dkv_sT;
   p.B = B, p.H = H, p.Hkv = Hkv, p.G = H / Hkv, p.Lq = Lq, p.Lk = Lk;
-  p.NQT = (Lq + 127) / 128, p.NKT = (Lk + 127) / 128, p.Lpad = 128 * p.NQT, p.nsplit = f.nsplit;
+  p.NQT = (Lq + 127) / 128, p.NKT = (Lk + 127) / 128, p.Lpad = 128 * p.NQT, p.runs = f.runs;
   p.qk_scale = (float)(0.08838834764831845 * 1.4426950408889634);
   p.o = BF(out), p.o_sB = o_sB, p.o_sH = o_sH, p.o_sT = o_sT;
   return cuda_status(launch_cross_attn_bwd(tq, tk, tv, tdo, tdq, p, S(stream)), what);

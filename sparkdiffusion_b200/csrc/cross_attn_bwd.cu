@@ -10,8 +10,8 @@
 // P and dS are rounded to bf16 where they feed a product; sums are fp32 in
 // tensor memory.  dK and dV of a key head sum over its G query heads: the key
 // tile stays and the steps walk the rows of all of them.  An encoder's states
-// are few key tiles and many query rows, so the rows of one key tile are cut
-// into slices (one CTA each) that leave fp32 partials, added in slice order.
+// are few key tiles and many query rows, so a tile's rows are dealt to several
+// CTAs, whose fp32 partials are added in a fixed order.
 // Keys past len[b] contribute nothing whatever they hold: their scores are
 // dropped by selection, their K rows cleared before dS K.
 #include "common.cuh"
@@ -441,56 +441,96 @@ __global__ void __launch_bounds__(xdq::THREADS, 1)
 }
 
 // ---------------------------------------------------------------------------
-// dk, dv: one CTA per (128-row key tile, b, key head, slice of the query rows);
-// steps of 64 query rows, both softmax warpgroups on every step (32 columns each)
+// dk, dv: the steps (64 query rows against a 128-row key tile) of all key tiles
+// that hold a valid key, one tile after the other, are dealt to the CTAs in equal
+// runs.  A CTA's run is a few segments, each within one tile; a tile within one
+// run is stored as it is, the others' segments leave fp32 partials that
+// cross_bwd_join_kernel adds in order (an encoder's states are few tiles: 160 at
+// 512 states and 40 heads; 12 slices of each as CTAs of their own took 0.64 ms
+// with the join, of it 0.1 in their ends and last round).
+//   warp 0   TMA producer: K and V of the tile, the ring of (Q, dO, lse, delta)
+//   warp 1   issues S^T = K Q^T and dP^T = V dO^T of a step, then dV += P^T dO and
+//            dK += dS^T Q of the step before: in one warp's order the columns of a step
+//            are overwritten without a wait (a second issuing warp, which has to wait
+//            for that, measured 10 % slower: there are two steps in flight, not three);
+//            owner of the tensor memory
+//   warps 4-11  P^T and dS^T: both warpgroups on every step, 32 columns each
 // ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(bwd::THREADS, 1)
+namespace xkv {
+constexpr int THREADS = 384;
+constexpr int NR = 4;                                        // ring entries
+constexpr int ENTRY = 2 * bwd::HALF + 1024;                  // + 64 lse + 64 delta
+constexpr int OFF_K = 0, OFF_V = bwd::TILE, OFF_RING = 2 * bwd::TILE;
+constexpr int OFF_BAR = OFF_RING + NR * ENTRY;
+constexpr int SMEM = OFF_BAR + 256;
+enum : int {
+  TF = 0,            // K and V of a segment loaded
+  RF, RE = RF + NR,  // ring
+  SF = RE + NR,      // S^T and dP^T of a step in TMEM
+  DS = SF + 2,       // P^T and dS^T of a step in TMEM, 8 warp arrivals
+  AF = DS + 2,       // dV and dK of a segment final
+  AE,                // dV and dK of a segment read, 8 arrivals
+  DRAIN, COUNT
+};
+static_assert(8 * COUNT + 16 <= 256 && SMEM <= 227 * 1024, "shared memory");
+}  // namespace xkv
+
+// Key tiles (b, key head, J), J * 128 < len[b], in that order
+struct KvTiles {
+  int b = 0;
+  int64_t base = 0;  // tiles before batch b
+  int len = 0, n = 0;  // of batch b
+  __device__ __forceinline__ explicit KvTiles(const CrossBwdParams& p) { at(p); }
+  __device__ __forceinline__ void at(const CrossBwdParams& p) {
+    len = kv_len(p.kv_lens, b, p.Lk);
+    n = (len + 127) >> 7;
+  }
+  // tile t (not before an earlier call's)
+  __device__ __forceinline__ void find(const CrossBwdParams& p, int64_t t, int& hk, int& J) {
+    while (t >= base + (int64_t)n * p.Hkv && b + 1 < p.B) {
+      base += (int64_t)n * p.Hkv;
+      ++b;
+      at(p);
+    }
+    const int r = (int)(t - base);
+    hk = r / max(n, 1);
+    J = r - hk * n;
+  }
+};
+// valid key tiles of batches [0, end), by all threads of the CTA (s: a shared word)
+__device__ __forceinline__ int64_t kv_tiles_before(const CrossBwdParams& p, int end, unsigned long long* s) {
+  if (p.kv_lens == nullptr) return (int64_t)end * p.Hkv * p.NKT;
+  __syncthreads();
+  if (threadIdx.x == 0) *s = 0ull;
+  __syncthreads();
+  unsigned long long v = 0;
+  for (int b = threadIdx.x; b < end; b += blockDim.x) v += (unsigned)((kv_len(p.kv_lens, b, p.Lk) + 127) >> 7);
+  if (v) atomicAdd(s, v);  // whole numbers: the order does not matter
+  __syncthreads();
+  return (int64_t)*s * p.Hkv;
+}
+
+__global__ void __launch_bounds__(xkv::THREADS, 1)
     cross_bwd_dkdv_tcgen05(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk,
                            const __grid_constant__ CUtensorMap tv, const __grid_constant__ CUtensorMap tdo,
                            const CrossBwdParams p) {
-  using namespace bwd;
+  using namespace xkv;
+  constexpr int TILE = bwd::TILE, HALF = bwd::HALF, BOX = bwd::BOX, BOX128 = bwd::BOX128;
   extern __shared__ __align__(1024) uint8_t smem1k[];
   const uint32_t base = smem_u32(smem1k);
-  const uint32_t bars = base + KV_OFF_BAR;
-  auto bar = [&](int i) { return bars + 8u * i; };
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem1k + KV_OFF_BAR + 8 * G_COUNT);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem1k + KV_OFF_BAR + 8 * G_COUNT + 8);
+  auto bar = [&](int i) { return base + OFF_BAR + 8u * i; };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem1k + OFF_BAR + 8 * COUNT);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem1k + OFF_BAR + 8 * COUNT + 8);
+  // broadcast values are warp-uniform to the compiler too (uniform registers for the MMAs)
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // slices of one key tile are neighbours
-  const int split = (int)(blockIdx.x % p.nsplit);
-  const int64_t rest = blockIdx.x / p.nsplit;
-  const int J = (int)(rest % p.NKT), bk = (int)(rest / p.NKT), b = bk / p.Hkv, hk = bk % p.Hkv;
-  const int len = kv_len(p.kv_lens, b, p.Lk);
-  if (128 * J >= len) {  // no valid key (uniform over the CTA)
-    if (p.nsplit == 1 && threadIdx.x < 256) {
-      const int tok = 128 * J + (threadIdx.x >> 1);
-      if (tok < p.Lk) {
-        const int64_t off = b * p.dkv_sB + hk * p.dkv_sH + tok * p.dkv_sT + 64 * (threadIdx.x & 1);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          reinterpret_cast<uint4*>(p.dk + off)[c] = make_uint4(0u, 0u, 0u, 0u);
-          reinterpret_cast<uint4*>(p.dv + off)[c] = make_uint4(0u, 0u, 0u, 0u);
-        }
-      }
-    }
-    return;
-  }
-  const int NH = (p.Lq + 63) / 64;  // steps per query head
-  const int64_t T = (int64_t)p.G * NH;
-  const int first = (int)(T * split / p.nsplit), n = (int)(T * (split + 1) / p.nsplit) - first;
+  const int64_t tiles = kv_tiles_before(p, p.B, reinterpret_cast<unsigned long long*>(smem1k));
+  const int NH = (p.Lq + 63) / 64, T = p.G * NH;  // steps per query head, per tile
+  const int64_t x0 = tiles * T * blockIdx.x / gridDim.x, x1 = tiles * T * (blockIdx.x + 1) / gridDim.x;
+  __syncthreads();
 
   if (threadIdx.x == 0) {
-    mbar_init(bar(G_TILE), 1);
-    for (int s = 0; s < KV_STAGES; ++s) {
-      mbar_init(bar(G_FULL0 + s), 1);
-      mbar_init(bar(G_EMPTY0 + s), 1);
-    }
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(bar(G_SF0 + t), 1);
-      mbar_init(bar(G_DS0 + t), 8);
-    }
-    mbar_init(bar(G_ACC), 1);
+    for (int i = 0; i < COUNT; ++i) mbar_init(bar(i), (i >= DS && i < AF) || i == AE ? 8 : 1);
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tq);
@@ -505,160 +545,201 @@ __global__ void __launch_bounds__(bwd::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  constexpr uint32_t hi = sdesc_hi(1024);
+  bool ok = true;
+  auto wait = [&](int i, uint32_t parity, int code) {
+    if (ok) ok = __all_sync(0xffffffffu, mbar_spin(bar(i), parity, abort_flag, code));
+    tc_fence_after();
+    return ok;
+  };
+  auto steps_of = [&](int64_t x) {  // steps of the segment that starts at x
+    const int64_t s0 = x % T;
+    return (int)min((int64_t)T - s0, x1 - x);
+  };
 
   if (warp == 0) {
     if (lane == 0) {
-      // ------------------------------------------------------------ TMA
-      mbar_expect_tx(bar(G_TILE), 2 * TILE);
-      load_tile(base + KV_OFF_K, &tk, bar(G_TILE), 128 * J, hk, b);
-      load_tile(base + KV_OFF_V, &tv, bar(G_TILE), 128 * J, hk, b);
-      for (int i = 0; i < n; ++i) {
-        const int s = i % KV_STAGES;
-        if (!mbar_wait(bar(G_EMPTY0 + s), ((i / KV_STAGES) & 1) ^ 1, abort_flag, kDevTimeoutMma)) break;
-        const uint32_t dst = base + KV_OFF_RING + s * KV_ENTRY;
-        mbar_expect_tx(bar(G_FULL0 + s), 2 * HALF + 512);
-        const int h = hk * p.G + (first + i) / NH, r0 = 64 * ((first + i) % NH);
-        const int64_t row = ((int64_t)b * p.H + h) * p.Lpad + r0;
-        load_half(dst, &tq, bar(G_FULL0 + s), r0, h, b);
-        load_half(dst + HALF, &tdo, bar(G_FULL0 + s), r0, h, b);
-        bulk_load(dst + 2 * HALF, p.lse + row, 256, bar(G_FULL0 + s));
-        bulk_load(dst + 2 * HALF + 256, p.delta + row, 256, bar(G_FULL0 + s));
+      // -------------------------------------------------------------- TMA
+      KvTiles kt(p);
+      int seg = 0, r = 0;
+      for (int64_t x = x0; x < x1 && ok; ++seg) {
+        const int n = steps_of(x), first = (int)(x % T);
+        int hk, J;
+        kt.find(p, x / T, hk, J);
+        // the previous segment's products have read its K and V
+        if (seg > 0 && !(ok = mbar_spin(bar(AF), (seg - 1) & 1, abort_flag, kDevTimeoutMma))) break;
+        mbar_expect_tx(bar(TF), 2 * TILE);
+        load_tile(base + OFF_K, &tk, bar(TF), 128 * J, hk, kt.b);
+        load_tile(base + OFF_V, &tv, bar(TF), 128 * J, hk, kt.b);
+        int g = first / NH, h64 = first - g * NH;
+        for (int i = 0; i < n; ++i, ++r) {
+          const int e = r % NR;
+          if (!(ok = mbar_spin(bar(RE + e), ((r / NR) & 1) ^ 1, abort_flag, kDevTimeoutMma))) break;
+          const uint32_t dst = base + OFF_RING + e * ENTRY;
+          const int h = hk * p.G + g, r0 = 64 * h64;
+          const int64_t row = ((int64_t)kt.b * p.H + h) * p.Lpad + r0;
+          mbar_expect_tx(bar(RF + e), 2 * HALF + 512);
+          load_half(dst, &tq, bar(RF + e), r0, h, kt.b);
+          load_half(dst + HALF, &tdo, bar(RF + e), r0, h, kt.b);
+          bulk_load(dst + 2 * HALF, p.lse + row, 256, bar(RF + e));
+          bulk_load(dst + 2 * HALF + 256, p.delta + row, 256, bar(RF + e));
+          if (++h64 == NH) h64 = 0, ++g;
+        }
+        x += n;
       }
+      // no copy may still target shared memory when the CTA exits; the waits
+      // ignore the abort flag and share one limit
       const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
-      bool drained = mbar_wait_until(bar(G_TILE), 0, deadline);
-      for (int i = max(0, n - KV_STAGES); i < n && drained; ++i)
-        drained = mbar_wait_until(bar(G_FULL0 + i % KV_STAGES), (i / KV_STAGES) & 1, deadline);
+      bool drained = true;
+      if (seg > 0) drained = mbar_wait_until(bar(TF), (seg - 1) & 1, deadline);
+      for (int n = max(0, r - NR); n < r && drained; ++n)
+        drained = mbar_wait_until(bar(RF + n % NR), (n / NR) & 1, deadline);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA
     if (elect_one()) {
-      const uint32_t id_s = idesc_bf16_f32(128, 64, false, false);
-      const uint32_t id_a = idesc_bf16_f32(128, 128, false, true);
-      bool ok = mbar_wait(bar(G_TILE), 0, abort_flag, kDevTimeoutLoad);
-      auto issue_acc = [&](int i) {
-        if (!mbar_wait(bar(G_DS0 + (i & 1)), (i >> 1) & 1, abort_flag, kDevTimeoutSoftmax)) {
-          ok = false;
-          return;
-        }
+      constexpr uint32_t id_s = idesc_bf16_f32(128, 64, false, false), id_a = idesc_bf16_f32(128, 128, false, true);
+      const uint32_t dk = sdesc_lo(base + OFF_K, 16), dv = sdesc_lo(base + OFF_V, 16);
+      int r = 0, seg = 0;
+      // dV and dK of step `at` (the i-th of its segment)
+      auto issue_acc = [&](int at, bool first, bool last) {
+        const int e = at % NR, g = at & 1;
+        if (!(ok = mbar_spin(bar(DS + g), (at >> 1) & 1, abort_flag, kDevTimeoutSoftmax))) return;
         tc_fence_after();
-        const uint32_t sq = base + KV_OFF_RING + (i % KV_STAGES) * KV_ENTRY, sdo = sq + HALF;
-        const uint32_t tb = tmem + 128 * (i & 1);
+        const uint32_t dq = sdesc_lo(base + OFF_RING + e * ENTRY, BOX), ddo = sdesc_lo(base + OFF_RING + e * ENTRY + HALF, BOX);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {  // dV += P^T dO, dK += dS^T Q; queries 16 kk.. of warpgroup kk / 2
+        for (int kk = 0; kk < 4; ++kk) {  // queries 16 kk .. of warpgroup kk / 2
           const uint32_t a = 32 * (kk >> 1) + 8 * (kk & 1);
-          mma_bf16_ts(tmem + 256, tb + a, sdesc_sw128(sdo + kk * 2048, BOX, 1024), id_a, (i > 0 || kk > 0) ? 1u : 0u);
-          mma_bf16_ts(tmem + 384, tb + 64 + a, sdesc_sw128(sq + kk * 2048, BOX, 1024), id_a,
-                      (i > 0 || kk > 0) ? 1u : 0u);
+          mma_bf16_ts_lo(tmem + 256, tmem + 128 * g + a, ddo + ((kk * 2048) >> 4), hi, id_a, (!first || kk > 0) ? 1u : 0u);
+          mma_bf16_ts_lo(tmem + 384, tmem + 128 * g + 64 + a, dq + ((kk * 2048) >> 4), hi, id_a,
+                         (!first || kk > 0) ? 1u : 0u);
         }
-        mma_commit(bar(G_EMPTY0 + i % KV_STAGES));
+        mma_commit(bar(RE + e));
+        if (last) mma_commit(bar(AF));
       };
-      for (int i = 0; i < n && ok; ++i) {
-        const int s = i % KV_STAGES;
-        if (!mbar_wait(bar(G_FULL0 + s), (i / KV_STAGES) & 1, abort_flag, kDevTimeoutLoad)) {
-          ok = false;
-          break;
+      for (int64_t x = x0; x < x1 && ok; ++seg) {
+        const int n = steps_of(x);
+        if (!(ok = mbar_spin(bar(TF), seg & 1, abort_flag, kDevTimeoutLoad))) break;
+        for (int i = 0; i < n && ok; ++i, ++r) {
+          const int e = r % NR, g = r & 1;
+          if (!(ok = mbar_spin(bar(RF + e), (r / NR) & 1, abort_flag, kDevTimeoutLoad))) break;
+          tc_fence_after();
+          const uint32_t dq = sdesc_lo(base + OFF_RING + e * ENTRY, 16), ddo = sdesc_lo(base + OFF_RING + e * ENTRY + HALF, 16);
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint32_t ka = ((kk >> 2) * BOX128 + (kk & 3) * 32) >> 4, kb = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
+            mma_bf16_ss_lo(tmem + 128 * g, dk + ka, hi, dq + kb, hi, id_s, kk > 0 ? 1u : 0u);
+          }
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint32_t ka = ((kk >> 2) * BOX128 + (kk & 3) * 32) >> 4, kb = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
+            mma_bf16_ss_lo(tmem + 128 * g + 64, dv + ka, hi, ddo + kb, hi, id_s, kk > 0 ? 1u : 0u);
+          }
+          mma_commit(bar(SF + g));
+          if (i == 0) {
+            // the previous segment's dV and dK have been read
+            if (!(ok = mbar_spin(bar(AE), (seg & 1) ^ 1, abort_flag, kDevTimeoutSoftmax))) break;
+          } else {
+            issue_acc(r - 1, i == 1, false);
+          }
         }
-        tc_fence_after();
-        const uint32_t sq = base + KV_OFF_RING + s * KV_ENTRY, sdo = sq + HALF;
-        const uint32_t tb = tmem + 128 * (i & 1);
-        mma_step_ss(tb, base + KV_OFF_K, sq, id_s);        // S^T  = K Q^T
-        mma_step_ss(tb + 64, base + KV_OFF_V, sdo, id_s);  // dP^T = V dO^T
-        mma_commit(bar(G_SF0 + (i & 1)));
-        if (i > 0) issue_acc(i - 1);
+        if (ok) issue_acc(r - 1, n == 1, true);
+        x += n;
       }
-      if (ok && n > 0) issue_acc(n - 1);
-      mma_commit(bar(G_ACC));
       // every MMA issued has completed before TMEM is freed, also on the abort path
-      mbar_wait_until(bar(G_ACC), 0, globaltimer_ns() + kWaitLimitNs);
+      mma_commit(bar(DRAIN));
+      mbar_wait_until(bar(DRAIN), 0, globaltimer_ns() + kWaitLimitNs);
     }
+    __syncwarp();
   } else if (warp >= 4) {
-    // ---------- P^T, dS^T of query columns [32 wg, 32 wg + 32) of every step, then the dK/dV epilogue
-    const int wg = (warp - 4) >> 2;
-    const int q = warp & 3;
-    const int r = q * 32 + lane;  // key row of the tile = TMEM lane
-    const int tok = 128 * J + r;
-    const bool sel = tok < len;
+    // ---------- P^T, dS^T of query columns [32 wg, 32 wg + 32) of every step, then dV and dK of the segment
+    const int wg = (warp - 4) >> 2, q = warp & 3;
+    const int row = q * 32 + lane;  // key row of the tile = TMEM lane
     const uint32_t lane_off = (uint32_t)(q * 32) << 16;
     const uint64_t sc2 = f2_pack(p.qk_scale, p.qk_scale);
-    bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      const int s = i % KV_STAGES;
-      const uint32_t tS = tmem + lane_off + 128 * (i & 1) + 32 * wg, tdP = tS + 64;
-      bool got = mbar_wait(bar(G_SF0 + (i & 1)), (i >> 1) & 1, abort_flag, kDevTimeoutMma);
-      // the step's lse / delta (bulk copies) are visible once its load barrier completed
-      got = got && mbar_wait(bar(G_FULL0 + s), (i / KV_STAGES) & 1, abort_flag, kDevTimeoutLoad);
-      if (!__all_sync(0xffffffffu, got)) {
-        ok = false;
-        break;
+    KvTiles kt(p);
+    int r = 0, seg = 0;
+    for (int64_t x = x0; x < x1 && ok; ++seg) {
+      const int n = steps_of(x);
+      const bool begins = x % T == 0, ends = (x + n) % T == 0;
+      int hk, J;
+      kt.find(p, x / T, hk, J);
+      const int tok = 128 * J + row, b = kt.b;
+      const bool sel = tok < kt.len;
+      for (int i = 0; i < n; ++i, ++r) {
+        const int e = r % NR, g = r & 1;
+        const uint32_t tS = tmem + lane_off + 128 * g + 32 * wg, tdP = tS + 64;
+        // the step's lse and delta (bulk copies) are visible once its load barrier completed
+        if (!wait(RF + e, (r / NR) & 1, kDevTimeoutLoad) || !wait(SF + g, (r >> 1) & 1, kDevTimeoutMma)) break;
+        const float* lse_s = reinterpret_cast<const float*>(smem1k + OFF_RING + e * ENTRY + 2 * HALF) + 32 * wg;
+        const float* dlt_s = lse_s + 64;
+        uint32_t sv[32], dv[32];
+        tmem_ld32(tS, sv);
+        tmem_ld32(tdP, dv);
+        tmem_ld_wait();
+        uint32_t wp[16], wd[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float2 l2 = *reinterpret_cast<const float2*>(lse_s + 2 * k);
+          const float2 d2 = *reinterpret_cast<const float2*>(dlt_s + 2 * k);
+          float y0, y1, p0, p1, d0, d1;
+          f2_unpack(fma_f32x2(f2_pack(__uint_as_float(sv[2 * k]), __uint_as_float(sv[2 * k + 1])), sc2,
+                              f2_pack(-l2.x, -l2.y)),
+                    y0, y1);
+          p0 = ex2_approx(y0), p1 = ex2_approx(y1);
+          f2_unpack(mul_f32x2(f2_pack(p0, p1), add_f32x2(f2_pack(__uint_as_float(dv[2 * k]), __uint_as_float(dv[2 * k + 1])),
+                                                         f2_pack(-d2.x, -d2.y))),
+                    d0, d1);
+          const uint32_t pp = pack_bf2(p0, p1), pd = pack_bf2(d0, d1);
+          // by selection: a key row past len[b] may hold anything
+          wp[k] = sel ? pp : 0u;
+          wd[k] = sel ? pd : 0u;
+        }
+        tmem_st16(tS, wp);   // packed P^T over the first 16 of this warpgroup's S^T columns
+        tmem_st16(tdP, wd);  // packed dS^T over the first 16 of its dP^T columns
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(DS + g));
       }
-      tc_fence_after();
-      const float* lse_s = reinterpret_cast<const float*>(smem1k + KV_OFF_RING + s * KV_ENTRY + 2 * HALF) + 32 * wg;
-      const float* dlt_s = lse_s + 64;
-      uint32_t sv[32], dv[32];
-      tmem_ld32(tS, sv);
-      tmem_ld32(tdP, dv);
-      tmem_ld_wait();
-      uint32_t wp[16], wd[16];
+      if (!wait(AF, seg & 1, kDevTimeoutMma)) break;
+      // dV, then dK (scaled by D^-1/2): columns [64 wg, 64 wg + 64)
+      const bool whole = begins && ends;
+      float* part = p.part + ((int64_t)(2 * blockIdx.x + (begins ? 1 : 0)) * 2 * 128 + row) * 128 + 64 * wg;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float2 l2 = *reinterpret_cast<const float2*>(lse_s + 2 * e);
-        const float2 d2 = *reinterpret_cast<const float2*>(dlt_s + 2 * e);
-        float x0, x1;
-        f2_unpack(fma_f32x2(f2_pack(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), sc2,
-                            f2_pack(-l2.x, -l2.y)),
-                  x0, x1);
-        const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
-        const uint32_t pp = pack_bf2(p0, p1);
-        const uint32_t pd = pack_bf2(p0 * (__uint_as_float(dv[2 * e]) - d2.x), p1 * (__uint_as_float(dv[2 * e + 1]) - d2.y));
-        wp[e] = sel ? pp : 0u;
-        wd[e] = sel ? pd : 0u;
-      }
-      tmem_st16(tS, wp);   // packed P^T over the first 16 of this warpgroup's S^T columns
-      tmem_st16(tdP, wd);  // packed dS^T over the first 16 of its dP^T columns
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(G_DS0 + (i & 1)));
-    }
-    if (ok && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(bar(G_ACC), 0, abort_flag, kDevTimeoutMma));
-    tc_fence_after();
-    if (ok) {
+      for (int c = 0; c < 4; ++c) {
+        const int which = c >> 1, col = 32 * (c & 1);
+        uint32_t v[32];
+        __syncwarp();  // the stores below diverge, the load is warp-collective
+        tmem_ld32(tmem + 256 + 128 * which + lane_off + 64 * wg + col, v);
+        tmem_ld_wait();
+        if (c == 3) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(AE));
+        }
+        if (!whole) {
+          float4* dst = reinterpret_cast<float4*>(part + which * 128 * 128 + col);
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {  // dV, then dK (scaled by D^-1/2)
-        const float sc = which ? kSmScale : 1.0f;
+          for (int k = 0; k < 8; ++k)
+            dst[k] = make_float4(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1]), __uint_as_float(v[4 * k + 2]),
+                                 __uint_as_float(v[4 * k + 3]));
+        } else if (tok < p.Lk) {
+          const float sc = which ? bwd::kSmScale : 1.0f;
+          uint4* dst = reinterpret_cast<uint4*>((which ? p.dk : p.dv) + b * p.dkv_sB + hk * p.dkv_sH + tok * p.dkv_sT +
+                                                64 * wg + col);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t v[32];
-          __syncwarp();  // the stores below diverge, the load is warp-collective
-          if (n > 0) {
-            tmem_ld32(tmem + 256 + 128 * which + lane_off + 64 * wg + 32 * c, v);
-            tmem_ld_wait();
-          } else {
+          for (int k = 0; k < 4; ++k) {
+            uint32_t w4[4];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) v[e] = 0u;
-          }
-          if (p.nsplit > 1) {
-            const int64_t row = (((int64_t)which * p.nsplit + split) * p.B * p.Hkv + bk) * (128ll * p.NKT) + tok;
-            float4* dst = reinterpret_cast<float4*>(p.part + row * 128 + 64 * wg + 32 * c);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              dst[e] = make_float4(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1]),
-                                   __uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3]));
-          } else if (tok < p.Lk) {
-            uint4* dst = reinterpret_cast<uint4*>((which ? p.dk : p.dv) + b * p.dkv_sB + hk * p.dkv_sH + tok * p.dkv_sT +
-                                                  64 * wg + 32 * c);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t w4[4];
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                w4[j] = pack_bf2(__uint_as_float(v[8 * e + 2 * j]) * sc, __uint_as_float(v[8 * e + 2 * j + 1]) * sc);
-              dst[e] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
-            }
+            for (int m = 0; m < 4; ++m)
+              w4[m] = pack_bf2(__uint_as_float(v[8 * k + 2 * m]) * sc, __uint_as_float(v[8 * k + 2 * m + 1]) * sc);
+            dst[k] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
           }
         }
       }
+      x += n;
     }
   }
   tc_fence_before();
@@ -670,69 +751,74 @@ __global__ void __launch_bounds__(bwd::THREADS, 1)
   }
 }
 
-// dk, dv = sum over the slices in order (0 past len[b]); one thread per 4 columns of a key
-__global__ void __launch_bounds__(256) cross_bwd_join_kernel(const CrossBwdParams p) {
-  const int64_t g = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int c = (int)(g & 31);
-  int64_t r = g >> 5;
-  const int tok = (int)(r % p.Lk);
-  r /= p.Lk;
-  const int64_t BHk = (int64_t)p.B * p.Hkv;
-  const int64_t bk = r % BHk;
-  const int which = (int)(r / BHk);
-  if (which >= 2) return;
-  const int b = (int)(bk / p.Hkv), hk = (int)(bk % p.Hkv);
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (tok < kv_len(p.kv_lens, b, p.Lk)) {
-    const int64_t step = BHk * 128ll * p.NKT * 128;
-    const float* src = p.part + ((which * p.nsplit * BHk + bk) * (128ll * p.NKT) + tok) * 128 + 4 * c;
-    for (int s = 0; s < p.nsplit; ++s) {
-      const float4 v = *reinterpret_cast<const float4*>(src + s * step);
-      a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
-    }
+// One CTA per 16 rows of a key tile: the sum of its segments' partials in order (a
+// tile within one run has been stored already), zeros where no key of the tile is valid
+__global__ void __launch_bounds__(256) cross_bwd_join_kernel(const CrossBwdParams p, int runs) {
+  __shared__ unsigned long long s_sum;
+  const int rows16 = (int)(blockIdx.x & 7), tile = (int)(blockIdx.x >> 3);
+  const int J = tile % p.NKT, bk = tile / p.NKT, b = bk / p.Hkv, hk = bk - b * p.Hkv;
+  const int len = kv_len(p.kv_lens, b, p.Lk);
+  const int64_t before = kv_tiles_before(p, b, &s_sum);
+  const int64_t tiles = kv_tiles_before(p, p.B, &s_sum);
+  const bool any = 128 * J < len;
+  const int T = p.G * ((p.Lq + 63) / 64);
+  // run c covers the steps [S c / runs, S (c + 1) / runs)
+  const int64_t S = tiles * T, t0 = (before + (int64_t)hk * ((len + 127) >> 7) + J) * T, t1 = t0 + T;
+  auto run_start = [&](int64_t c) { return S * c / runs; };
+  int64_t c0 = 0, c1 = 0;
+  if (any) {
+    c0 = t0 * runs / S;  // within one of the run of t0
+    while (c0 > 0 && run_start(c0) > t0) --c0;
+    while (run_start(c0 + 1) <= t0) ++c0;
+    c1 = c0;
+    while (run_start(c1 + 1) < t1) ++c1;
+    if (c0 == c1) return;  // one run: stored
   }
-  const float sc = which ? bwd::kSmScale : 1.0f;
-  *reinterpret_cast<uint2*>((which ? p.dk : p.dv) + b * p.dkv_sB + hk * p.dkv_sH + tok * p.dkv_sT + 4 * c) =
-      make_uint2(pack_bf2(a.x * sc, a.y * sc), pack_bf2(a.z * sc, a.w * sc));
+  // 32 threads a row, 4 columns each
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int i = threadIdx.x + 256 * k;
+    const int which = i >> 9, row = 16 * rows16 + ((i >> 5) & 15), col = 4 * (i & 31), tok = 128 * J + row;
+    if (tok >= p.Lk) continue;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (any) {
+      for (int64_t c = c0; c <= c1; ++c) {
+        const int64_t start = run_start(c);
+        if (start == run_start(c + 1)) continue;  // an empty run
+        const int64_t slot = 2 * c + (start <= t0 ? 1 : 0);
+        const float4 v = *reinterpret_cast<const float4*>(p.part + ((slot * 2 + which) * 128 + row) * 128 + col);
+        a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+      }
+    }
+    const float sc = which ? bwd::kSmScale : 1.0f;
+    *reinterpret_cast<uint2*>((which ? p.dk : p.dv) + b * p.dkv_sB + hk * p.dkv_sH + tok * p.dkv_sT + col) =
+        make_uint2(pack_bf2(a.x * sc, a.y * sc), pack_bf2(a.z * sc, a.w * sc));
+  }
 }
 
-// Slices of the query rows per key tile: the count (at most 12) whose waves of
-// CTAs waste least, with 16 steps of 64 rows or more in each
-int cross_bwd_splits(int B, int H, int Hkv, int Lq, int Lk) {
-  const int64_t tiles = (int64_t)B * Hkv * ((Lk + 127) / 128);
-  const int64_t steps = (int64_t)(H / Hkv) * ((Lq + 63) / 64);
+// CTAs of the dk/dv kernel: one per SM, with 8 steps or more each (fewer do not
+// pay for a segment's ends)
+int cross_bwd_runs(int B, int H, int Hkv, int Lq, int Lk) {
+  const int64_t steps = (int64_t)B * Hkv * ((Lk + 127) / 128) * (H / Hkv) * ((Lq + 63) / 64);
+  const int64_t runs = (steps + 7) / 8;
   const int sms = device_sms();
-  int best = 1;
-  double cost = 1e30;
-  for (int s = 1; s <= 12 && (s == 1 || steps / s >= 16); ++s) {
-    const double waves = (double)((tiles * s + sms - 1) / sms) / s;
-    if (waves < cost * 0.97) {
-      cost = waves;
-      best = s;
-    }
-  }
-  return best;
+  return (int)(runs < sms ? runs : sms);
 }
 
 int launch_cross_attn_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
                           const CUtensorMap& tdq, const CrossBwdParams& p, cudaStream_t s) {
-  using namespace bwd;
   static KernelReady ready_dq, ready_dkdv;
   int rc = kernel_ready(ready_dq, cross_bwd_dq_tcgen05, xdq::SMEM, xdq::LAUNCH_REGS);
-  if (rc == 0) rc = kernel_ready(ready_dkdv, cross_bwd_dkdv_tcgen05, KV_SMEM);
+  if (rc == 0) rc = kernel_ready(ready_dkdv, cross_bwd_dkdv_tcgen05, xkv::SMEM);
   if (rc != 0) return rc;
   cudaError_t e;
   const int64_t items = (int64_t)p.NQT * p.B * p.H;
   const int sms = device_sms();
   cross_bwd_dq_tcgen05<<<(unsigned)(items < sms ? items : sms), xdq::THREADS, xdq::SMEM, s>>>(tq, tk, tv, tdo, tdq, p);
   if ((e = cudaGetLastError()) != cudaSuccess) return (int)e;
-  cross_bwd_dkdv_tcgen05<<<(unsigned)((int64_t)p.NKT * p.B * p.Hkv * p.nsplit), THREADS, KV_SMEM, s>>>(tq, tk, tv, tdo,
-                                                                                                  p);
+  cross_bwd_dkdv_tcgen05<<<p.runs, xkv::THREADS, xkv::SMEM, s>>>(tq, tk, tv, tdo, p);
   if ((e = cudaGetLastError()) != cudaSuccess) return (int)e;
-  if (p.nsplit > 1) {
-    const int64_t threads = 2ll * p.B * p.Hkv * p.Lk * 32;
-    cross_bwd_join_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, s>>>(p);
-  }
+  cross_bwd_join_kernel<<<(unsigned)((int64_t)p.NKT * p.B * p.Hkv * 8), 256, 0, s>>>(p, p.runs);
   return (int)cudaGetLastError();
 }
 

@@ -264,11 +264,11 @@ struct CrossBwdParams {
   __nv_bfloat16* dk;
   __nv_bfloat16* dv;
   int64_t dq_sB, dq_sH, dq_sT, dkv_sB, dkv_sH, dkv_sT;
-  float* part;         // nsplit > 1: [2 (dv, dk), nsplit, B*Hkv, 128 * NKT, 128]
-  int B, H, Hkv, G, Lq, Lk, Lpad, NQT, NKT, nsplit;
+  float* part;         // [2 * runs, 2 (dv, dk), 128, 128]
+  int B, H, Hkv, G, Lq, Lk, Lpad, NQT, NKT, runs;
   float qk_scale;
 };
-int cross_bwd_splits(int B, int H, int Hkv, int Lq, int Lk);
+int cross_bwd_runs(int B, int H, int Hkv, int Lq, int Lk);  // CTAs of the dk/dv kernel
 // 64-row boxes; tdq: the output dq
 int launch_cross_attn_bwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const CUtensorMap& tdo,
                           const CUtensorMap& tdq, const CrossBwdParams& p, cudaStream_t s);
