@@ -18,7 +18,12 @@ Ops (inputs and layouts as in ``ops``; outputs are new tensors):
 * ``block_select(pooled_q, pooled_k, topk) -> [B*H, NBq, topk]`` int32;
 * ``fused_sparse_attn(q, k, v, topk_ratio, blkq, blkk, num_heads) -> [B, H, L, D]``
   (fused_sparse_attn.py:151-215);
-* ``dense_attention(q, k, v, num_heads) -> [B, H, L, D]``.
+* ``dense_attention(q, k, v, num_heads) -> [B, H, L, D]``;
+* ``cross_attention(q, k, v, kv_lens?) -> [B, H, Lq, D]`` (a view of a token-major tensor);
+* ``add_rms_norm(x, residual, weight, eps) -> (y, h)`` and
+  ``add_rms_norm_e4m3(x, residual, weight, eps) -> (yq, scale, h)`` (a scale per 128 columns);
+* ``quantize_blocks_e4m3(x) -> (xq, scale)`` and
+  ``gemm_fp8_block(xq, x_scale, wq, w_scale, bias?) -> [M, N]`` bf16.
 """
 
 from __future__ import annotations
@@ -90,3 +95,64 @@ def dense_attention(q: Tensor, k: Tensor, v: Tensor, num_heads: int) -> Tensor:
 def _(q, k, v, num_heads):
     BH, L, D = q.shape
     return v.new_empty(BH // num_heads, num_heads, L, D)
+
+
+@torch.library.custom_op("rola_b200::cross_attention", mutates_args=())
+def cross_attention(q: Tensor, k: Tensor, v: Tensor, kv_lens: Optional[Tensor]) -> Tensor:
+    return ops.cross_attention(q, k, v, kv_lens)
+
+
+@cross_attention.register_fake
+def _(q, k, v, kv_lens):
+    B, H, Lq, D = q.shape
+    return q.new_empty_strided((B, H, Lq, D), (Lq * H * D, D, H * D, 1))
+
+
+@torch.library.custom_op("rola_b200::add_rms_norm", mutates_args=())
+def add_rms_norm(x: Tensor, residual: Tensor, weight: Tensor, eps: float) -> tuple[Tensor, Tensor]:
+    return ops.add_rms_norm(x, weight, eps, residual)
+
+
+@add_rms_norm.register_fake
+def _(x, residual, weight, eps):
+    return x.new_empty(x.shape, dtype=BF16), x.new_empty(x.shape, dtype=residual.dtype)
+
+
+def _scales_like(x: Tensor) -> Tensor:
+    """The layout ``ops`` gives block scales: rows (flattened) innermost."""
+    lead, nb = x.shape[:-1], (x.shape[-1] + ops.SCALE_BLOCK - 1) // ops.SCALE_BLOCK
+    strides, step = [], 1
+    for n in reversed(lead):
+        strides.insert(0, step)
+        step = step * n
+    return x.new_empty_strided((*lead, nb), (*strides, step), dtype=torch.float32)
+
+
+@torch.library.custom_op("rola_b200::add_rms_norm_e4m3", mutates_args=())
+def add_rms_norm_e4m3(x: Tensor, residual: Tensor, weight: Tensor, eps: float) -> tuple[Tensor, Tensor, Tensor]:
+    return ops.add_rms_norm_e4m3(x, weight, eps, residual)
+
+
+@add_rms_norm_e4m3.register_fake
+def _(x, residual, weight, eps):
+    return x.new_empty(x.shape, dtype=ops.E4M3), _scales_like(x), x.new_empty(x.shape, dtype=residual.dtype)
+
+
+@torch.library.custom_op("rola_b200::quantize_blocks_e4m3", mutates_args=())
+def quantize_blocks_e4m3(x: Tensor) -> tuple[Tensor, Tensor]:
+    return ops.quantize_blocks_e4m3(x)
+
+
+@quantize_blocks_e4m3.register_fake
+def _(x):
+    return x.new_empty(x.shape, dtype=ops.E4M3), _scales_like(x)
+
+
+@torch.library.custom_op("rola_b200::gemm_fp8_block", mutates_args=())
+def gemm_fp8_block(xq: Tensor, x_scale: Tensor, wq: Tensor, w_scale: Tensor, bias: Optional[Tensor]) -> Tensor:
+    return ops.gemm_fp8_block(xq, x_scale, wq, w_scale, bias)
+
+
+@gemm_fp8_block.register_fake
+def _(xq, x_scale, wq, w_scale, bias):
+    return xq.new_empty(xq.shape[0], wq.shape[0], dtype=BF16)

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import sublayer_oracle as orc
-from sparkdiffusion_b200 import _lib, ops, train
+from sparkdiffusion_b200 import _lib, ops, torch_ops, train  # noqa: F401  (torch_ops registers torch.ops.rola_b200.*)
 
 gpu = pytest.mark.gpu
 BF16, F32, E4M3 = torch.bfloat16, torch.float32, torch.float8_e4m3fn
@@ -51,6 +51,8 @@ ATTENTION = {
     # more items than SMs: CTAs walk several, with one and two query tiles, empty ones between
     "many_items": (5, 40, 40, 300, 200, (200, 0, 77, 1, 128)),
     "many_groups": (4, 40, 8, 130, 140, (140, 0, 139, 13)),
+    # items of one step, four a CTA: every role runs across their ends
+    "one_step_items": (1, 4, 4, 19000, 40, None),
     "clamped_lens": (3, 1, 1, 40, 50, (-3, 50, 99)),
 }
 
@@ -248,6 +250,102 @@ def test_cross_attention_long_offsets():
 
 
 @gpu
+def test_cross_attention_long_rows():
+    """Rows whose offsets pass 2^31 elements, against one state: o is v, and dv the sum of dO's rows."""
+    L = (1 << 24) + 70
+    q = torch.zeros(1, 1, L, 128, device="cuda", dtype=BF16)
+    assert q.numel() > 2 ** 31
+    q[:, :, -300:] = _randn(300, 128, seed=6).cuda()
+    q.requires_grad_(True)
+    k, v = (_randn(1, 1, 1, 128, seed=s).cuda().requires_grad_(True) for s in (7, 8))
+    do = torch.zeros_like(q)
+    do[:, :, -1] = _randn(128, seed=9).cuda()
+    o = train.cross_attention(q, k, v)
+    assert bool((o[:, :, -300:] == v).all()) and bool((o[:, :, ::4096] == v).all())
+    dq, dk, dv = torch.autograd.grad(o, (q, k, v), do)
+    _ok()
+    assert torch.equal(dv[0, 0, 0], do[0, 0, -1])
+    # dS = P (dP - delta): the same sum of 128 products twice, in fp32 in two orders
+    eps = 2 * 128 * 2.0 ** -24 * (do[0, 0, -1].float() * v[0, 0, 0].float()).abs().sum().item()
+    assert bool((dq[:, :, :-1] == 0).all())
+    assert bool((dq[0, 0, -1].float().abs() <= eps * k[0, 0, 0].float().abs() * 128 ** -0.5 * 1.01).all())
+    assert bool((dk[0, 0, 0].float().abs() <= eps * q[0, 0, -1].float().abs() * 128 ** -0.5 * 1.01).all())
+
+
+@gpu
+def test_norm_and_product_long_offsets():
+    """Rows whose offsets pass 2^31 elements: the bits of a call on the last rows alone."""
+    M, K = 140000, 16384
+    x = torch.zeros(M, K, device="cuda", dtype=BF16)
+    assert x.numel() > 2 ** 31
+    x[-3:] = _randn(3, K, seed=1).cuda()
+    w = _randn(K, seed=2).cuda()
+    y, h = ops.add_rms_norm(x, w, 1e-6, x)
+    y1, h1 = ops.add_rms_norm(x[-3:], w, 1e-6, x[-3:])
+    assert torch.equal(y[-3:], y1) and torch.equal(h[-3:], h1) and bool((y[:: M // 7] == 0).all())
+    rstd = torch.ones(M, device="cuda")
+    dx, _, _ = ops.add_rms_norm_bwd(h, w, rstd, x, None, BF16, None, need_dw=False)
+    assert torch.equal(dx[-3:], ops.add_rms_norm_bwd(h1, w, rstd[:3], x[-3:], None, BF16, None, need_dw=False)[0])
+    del y, h, dx
+    yq, s, _ = ops.add_rms_norm_e4m3(x, w)
+    y1, s1, _ = ops.add_rms_norm_e4m3(x[-3:], w)
+    assert torch.equal(yq[-3:].view(torch.uint8), y1.view(torch.uint8)) and torch.equal(s[-3:], s1)
+    del x, yq
+    (xq, xs), (wq, ws) = _quantized(200, 128, 1, 1), _quantized(32768, 128, 128, 2)
+    xq, xs, wq, ws = _cuda(xq, xs, wq, ws)
+    many = 70000
+    tall = torch.zeros(many + 200, 128, device="cuda", dtype=torch.uint8)
+    tall[many:] = xq.view(torch.uint8)
+    out = ops.gemm_fp8_block(tall.view(E4M3), torch.cat([xs.new_ones(many, 1), xs]), wq, ws)
+    assert out.numel() > 2 ** 31
+    assert torch.equal(out[-200:], ops.gemm_fp8_block(xq, xs, wq, ws)) and bool((out[: many: 997] == 0).all())
+    _ok()
+
+
+@gpu
+def test_norm_and_product_streams_and_graphs():
+    """Two calls at once on two streams, and two captured graphs replayed in turn with new inputs: the eager bits."""
+    xs = [_randn(257, 1536, seed=1 + i).cuda() for i in range(2)]
+    res = [_randn(257, 1536, seed=5 + i, dtype=F32).cuda() for i in range(2)]
+    w = (1 + 0.2 * _randn(1536, seed=3, dtype=F32)).cuda()
+    wq, ws = ops.quantize_tiles_e4m3(_randn(520, 1536, seed=4).cuda())
+    dy = _randn(257, 1536, seed=7).cuda()
+
+    def step(x, r):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, r)]
+        y, h = train.add_rms_norm(leaves[0], leaves[1], 1e-6, leaves[2])
+        yq, ys, _ = ops.add_rms_norm_e4m3(x, w, 1e-6, r)
+        few = [ops.gemm_fp8_block(yq[:n], ys[:n], wq, ws) for n in (1, 257)]
+        return (y.detach(), h.detach(), *few, *torch.autograd.grad((y, h), leaves, (dy, r)))
+
+    want = [step(x, r) for x, r in zip(xs, res)]
+    side = [torch.cuda.Stream() for _ in xs]
+    torch.cuda.synchronize()
+    got = []
+    for s, x, r in zip(side, xs, res):
+        with torch.cuda.stream(s):
+            got.append(step(x, r))
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(t, u) for t, u in zip(a, b))
+    graphs = []
+    for x, r in zip(xs, res):
+        buf, g = (x.clone(), r.clone()), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(*buf)
+        graphs.append((g, buf, out))
+    for turn in range(2):
+        for i, (g, buf, _) in enumerate(graphs):
+            buf[0].copy_(xs[(i + turn) % 2])
+            buf[1].copy_(res[(i + turn) % 2])
+            g.replay()
+        torch.cuda.synchronize()
+        for i, (_, _, out) in enumerate(graphs):
+            assert all(torch.equal(t, u) for t, u in zip(out, want[(i + turn) % 2]))
+    _ok()
+
+
+@gpu
 def test_cross_attention_no_rows_or_states():
     z = lambda *s: torch.zeros(*s, device="cuda", dtype=BF16)  # noqa: E731
     assert ops.cross_attention(z(2, 3, 0, 128), z(2, 3, 5, 128), z(2, 3, 5, 128)).shape == (2, 3, 0, 128)
@@ -257,6 +355,53 @@ def test_cross_attention_no_rows_or_states():
     assert bool((o == 0).all())
     dq, dk = torch.autograd.grad(o.sum(), (q, k))
     assert bool((dq == 0).all()) and dk.shape == k.shape
+
+
+@gpu
+@pytest.mark.parametrize("order", ["rising", "falling", "one_late_peak"])
+def test_cross_attention_running_maximum(order):
+    """Row maxima that grow by more than 2^8 from tile to tile (and within one), fall, or come with
+    one late key: the rescaling of O and l, in the forward and through its log-sum-exp in the backward."""
+    B, H, Lq, Lk = 1, 2, 150, 700
+    q, k, v, do = (_randn(B, H, n, 128, seed=80 + i, dtype=F32) for i, n in enumerate((Lq, Lk, Lk, Lq)))
+    u = torch.nn.functional.normalize(torch.ones(128), dim=0)
+    q = q * 0.3 + 8 * u
+    grow = torch.arange(Lk) / Lk * 40 if order == "rising" else torch.arange(Lk, 0, -1) / Lk * 40
+    if order == "one_late_peak":
+        grow = torch.where(torch.arange(Lk) == Lk - 3, 30.0, 0.0)
+    k = k * 0.3 + grow[:, None] * u  # scores up to about 8 * 40 / sqrt(128): 28, or 41 in powers of two
+    q, k, v, do = (t.to(BF16) for t in (q, k, v, do))
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    o = train.cross_attention(*leaves)
+    grads = torch.autograd.grad(o, leaves, do.cuda())
+    _ok()
+    ref, _, tol = orc.cross_attention_bound(q, k, v)
+    _within(o, ref, tol, "o")
+    bounds = orc.cross_attention_grads(q, k, v, do)
+    for name, g in zip(("dq", "dk", "dv"), grads):
+        _within(g, *bounds[name], name)
+
+
+@gpu
+def test_sublayer_operators_under_torch_compile():
+    """The custom operators' fake kernels agree with the real ones in shape, type and layout."""
+    q, k, v, _, lens = _attention_inputs("key_tail")
+    x, r, w, eps = _norm_inputs("heads_12")
+    (xq, xs), (wq, ws) = _quantized(40, 256, 1, 1), _quantized(64, 256, 128, 2)
+    t = torch.ops.rola_b200
+    for op, args in (
+        (t.cross_attention, (*_cuda(q, k, v), _lens_gpu(lens))),
+        (t.cross_attention, (*_cuda(q, k, v), None)),
+        (t.add_rms_norm, (*_cuda(x, r, w), eps)),
+        (t.add_rms_norm_e4m3, (*_cuda(x, r, w), eps)),
+        (t.add_rms_norm_e4m3, (*(c.view(257, 2, 768) for c in _cuda(x, r)), w.cuda()[:768], eps)),
+        (t.quantize_blocks_e4m3, _cuda(x)),
+        (t.gemm_fp8_block, (*_cuda(xq, xs, wq, ws), None)),
+    ):
+        # (the schema test computes on its inputs and outputs, which e4m3 does not support)
+        e4m3 = any(t.dtype is E4M3 for t in (args[0], *torch.utils._pytree.tree_leaves(op(*args))))
+        torch.library.opcheck(op.default, args, test_utils=("test_faketensor",) if e4m3 else ("test_schema", "test_faketensor"))
+    _ok()
 
 
 # --------------------------------------------------------------------- norm
@@ -421,6 +566,9 @@ PRODUCT = {
     "rows_300": (300, 1032, 1536, True),
     "tall": (2049, 24, 128, False),
     "many_tiles": (1500, 2600, 656, True),
+    # several tiles a CTA, of both widths
+    "persistent_narrow": (2000, 2600, 144, True),
+    "persistent_wide": (3500, 2560, 272, False),
 }
 
 
