@@ -127,7 +127,7 @@ int rola_b200_gemm_fp8_block(const void* xq, const float* x_scale, int64_t xs_sM
   {
     const uint64_t dims[2] = {(uint64_t)K, (uint64_t)N};
     const uint64_t strides[1] = {(uint64_t)K};
-    const uint32_t box[2] = {128, (uint32_t)gemm_block_w_rows((int)M, (int)N, (int)K)};
+    const uint32_t box[2] = {128, 128};
     ROLA_TRY(make_map(&tb, wq, 2, dims, strides, box, "gemm_fp8_block: wq", true));
   }
   GemmBlockParams p{};
@@ -238,6 +238,7 @@ int rola_b200_cross_attn_bwd(const void* q, int64_t q_sB, int64_t q_sH, int64_t 
                  aligned16(workspace),
              "%s: 16-byte aligned tensors required", what);
   const CrossBwdLayout f = cross_bwd_layout(B, H, Hkv, Lq, Lk);
+  ROLA_CHECK(kv_lens == nullptr || B <= 65536, "%s: at most 65536 sequences of their own lengths", what);
   ROLA_CHECK(workspace_bytes >= f.total, "%s: workspace of %zu bytes < %zu", what, workspace_bytes, f.total);
   CUtensorMap tq, tk, tv, tdo, tdq;
   ROLA_TRY(make_head_map(&tq, q, 128, q_sB, q_sH, q_sT, Lq, H, B, "cross_attn_bwd: q", 64));

@@ -139,11 +139,13 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 // The same in few instructions, for warps whose waits are on the path of every
 // step: bounded by attempts (each is at least a shared-memory round trip and may
 // suspend the thread, so 2^20 of them last tens of milliseconds or longer; a
-// legitimate wait lasts microseconds).
-__device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity, volatile int* abort_flag, int err_code) {
+// legitimate wait lasts microseconds).  A wait for the end of a longer piece of
+// work, `tiles` tiles of a few microseconds each, is given as many attempts more.
+__device__ __forceinline__ bool mbar_spin(uint32_t bar, uint32_t parity, volatile int* abort_flag, int err_code,
+                                          uint32_t tiles = 0) {
   for (uint32_t n = 0; !mbar_try_wait(bar, parity); ++n) {
     if ((n & 1023u) == 1023u && *abort_flag) return false;
-    if (n >= (1u << 20)) {
+    if (n >= (1u << 20) + 256u * tiles) {
       *abort_flag = 1;
       set_device_error(err_code);
       return false;

@@ -196,10 +196,10 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
       if (lane == 0) {
         // -------------------------------------------- TMA: Q and K; the output
         int q = 0, k = 0;  // tiles loaded
-        int om[NQ], oh[NQ], ob[NQ];  // the items whose Q tiles are loaded
+        int om[NQ] = {}, oh[NQ] = {}, ob[NQ] = {};  // the items whose Q tiles are loaded
         // output of the item in Q tile e, the n-th of that tile
         auto store_out = [&](int e, int n) {
-          if (!mbar_spin(bar(QE + e), n & 1, abort_flag, kDevTimeoutSoftmax)) return false;
+          if (!mbar_spin(bar(QE + e), n & 1, abort_flag, kDevTimeoutSoftmax, 2 * (uint32_t)(p.Lk >> 7))) return false;
           if (p.nsplit == 1) {
             tma_store_4d(&to, base + OFF_Q + e * TILE, 0, om[e] * 128, oh[e], ob[e]);
             tma_store_4d(&to, base + OFF_Q + e * TILE + BOX, 64, om[e] * 128, oh[e], ob[e]);

@@ -1,7 +1,11 @@
 // Backward of the attention to another sequence's states (cross_attn.cu), on
 // tcgen05, without atomics.  From the forward's base-2 log-sum-exp:
 //
-//   delta[i] = sum_d dO[i, d] O[i, d]   (by the way, in the dq kernel, which has dO)
+//   delta[i] = sum_d dO[i, d] O[i, d]   (by the way, in the dq kernel, which has dO;
+//              O is the rounded output.  Over 64 keys or fewer, where dP and delta
+//              nearly cancel and that rounding would be the largest error of dQ and dK
+//              (2 keys: 0.0037 of their norm, without it 0.0024), it is sum_j P dP,
+//              the same number)
 //   P  = exp2(q.k D^-1/2 log2(e) - lse[i])             (recomputed, fp32; 0 past len[b])
 //   dP = dO V^T,  dS = P (dP - delta[i])
 //   dQ = D^-1/2 dS K                    query-stationary   (cross_bwd_dq_tcgen05)
@@ -153,9 +157,9 @@ __global__ void __launch_bounds__(xdq::THREADS, 1)
       if (lane == 0) {
         // ------------------------------------------ TMA: Q, dO; dQ of the items
         int q = 0;
-        int om[NT], oh[NT], ob[NT];
+        int om[NT] = {}, oh[NT] = {}, ob[NT] = {};
         auto store_out = [&](int e, int n) {
-          if (!mbar_spin(bar(TE + e), n & 1, abort_flag, kDevTimeoutSoftmax)) return false;
+          if (!mbar_spin(bar(TE + e), n & 1, abort_flag, kDevTimeoutSoftmax, 2 * (uint32_t)(p.Lk >> 6))) return false;
           const uint32_t src = base + OFF_T + e * 2 * TILE;
 #pragma unroll
           for (int c = 0; c < 4; ++c)
@@ -301,25 +305,29 @@ __global__ void __launch_bounds__(xdq::THREADS, 1)
       const int e = j % NT, tok = 128 * it.m + row;
       const uint8_t* dos = smem1k + OFF_T + e * 2 * TILE + TILE + row * 128;
       const uint4* o = reinterpret_cast<const uint4*>(p.o + it.b * p.o_sB + it.h * p.o_sH + (int64_t)min(tok, p.Lq - 1) * p.o_sT);
-      if (!wait(TF + e, (j / NT) & 1, kDevTimeoutLoad)) break;
-      float acc = 0.f;
+      // (loaded once the item before the previous one has left its tile: an item's time)
+      ok = __all_sync(0xffffffffu, mbar_spin(bar(TF + e), (j / NT) & 1, abort_flag, kDevTimeoutLoad, 2 * (uint32_t)(p.Lk >> 6)));
+      if (!ok) break;
+      if (it.cnt > 1) {
+        float acc = 0.f;
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const uint4 ov = __ldg(o + c);
-        const uint4 dv = *reinterpret_cast<const uint4*>(dos + (c >> 3) * BOX128 + (((c & 7) ^ (row & 7)) << 4));
-        const uint32_t oa[4] = {ov.x, ov.y, ov.z, ov.w}, da[4] = {dv.x, dv.y, dv.z, dv.w};
+        for (int c = 0; c < 16; ++c) {
+          const uint4 ov = __ldg(o + c);
+          const uint4 dv = *reinterpret_cast<const uint4*>(dos + (c >> 3) * BOX128 + (((c & 7) ^ (row & 7)) << 4));
+          const uint32_t oa[4] = {ov.x, ov.y, ov.z, ov.w}, da[4] = {dv.x, dv.y, dv.z, dv.w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float o0, o1, d0, d1;
-          unpack_bf2(oa[k], o0, o1);
-          unpack_bf2(da[k], d0, d1);
-          acc = fmaf(o0, d0, acc);
-          acc = fmaf(o1, d1, acc);
+          for (int k = 0; k < 4; ++k) {
+            float o0, o1, d0, d1;
+            unpack_bf2(oa[k], o0, o1);
+            unpack_bf2(da[k], d0, d1);
+            acc = fmaf(o0, d0, acc);
+            acc = fmaf(o1, d1, acc);
+          }
         }
+        if (tok >= p.Lq) acc = 0.f;  // a padding row (its P is 0, its delta has to be a number)
+        reinterpret_cast<float*>(smem1k + OFF_DELTA)[e * 128 + row] = acc;
+        p.delta[((int64_t)it.b * p.H + it.h) * p.Lpad + tok] = acc;
       }
-      if (tok >= p.Lq) acc = 0.f;  // a padding row (its P is 0, its delta has to be a number)
-      reinterpret_cast<float*>(smem1k + OFF_DELTA)[e * 128 + row] = acc;
-      p.delta[((int64_t)it.b * p.H + it.h) * p.Lpad + tok] = acc;
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(DR + e));
       ++j;
@@ -356,12 +364,37 @@ __global__ void __launch_bounds__(xdq::THREADS, 1)
         ++items;
         continue;
       }
-      if (!wait(DR + j % NT, (j / NT) & 1, kDevTimeoutSoftmax)) break;
-      const float dlt = reinterpret_cast<const float*>(smem1k + OFF_DELTA)[(j % NT) * 128 + row];
-      const uint64_t nl2 = f2_pack(-lse, -lse), nd2 = f2_pack(-dlt, -dlt);
+      const uint64_t nl2 = f2_pack(-lse, -lse);
+      uint64_t nd2 = 0ull;
+      bool have_delta = false;
       for (int i = 0; i < cnt; ++i, ++u) {
         if (u % NS != g) continue;
         if (!wait(SF + g, ph, kDevTimeoutMma)) break;
+        if (!have_delta) {
+          // only with a step of the item at hand: a warpgroup without one may find the
+          // barrier two phases on, which parity cannot tell from not yet
+          float dlt = 0.f;
+          if (cnt == 1) {
+            // every key of the row is here: delta as sum_j P dP, from fp32 alone
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              uint32_t sv[32], dv[32];
+              tmem_ld32(tS + 32 * c, sv);
+              tmem_ld32(tdP + 32 * c, dv);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (32 * c + e < len)
+                  dlt = fmaf(ex2_approx(fmaf(__uint_as_float(sv[e]), p.qk_scale, -lse)), __uint_as_float(dv[e]), dlt);
+            }
+            p.delta[((int64_t)b * p.H + h) * p.Lpad + 128 * m + row] = dlt;
+          } else {
+            if (!wait(DR + j % NT, (j / NT) & 1, kDevTimeoutSoftmax)) break;
+            dlt = reinterpret_cast<const float*>(smem1k + OFF_DELTA)[(j % NT) * 128 + row];
+          }
+          nd2 = f2_pack(-dlt, -dlt);
+          have_delta = true;
+        }
         const int valid = len - 64 * i;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {

@@ -399,8 +399,6 @@ static int launch_gemm_block_few_rows(const GemmBlockParams& p, cudaStream_t s) 
   return (int)cudaGetLastError();
 }
 
-int gemm_block_w_rows(int, int, int) { return 128; }
-
 // The wider tile unless its last wave of CTAs is so empty that the narrower one,
 // at 0.57 of its time a tile (measured), finishes first
 int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, cudaStream_t s) {

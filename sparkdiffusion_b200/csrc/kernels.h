@@ -224,8 +224,6 @@ struct GemmBlockParams {
   int64_t xs_sM, xs_sK, ws_ld;
   int M, N, K;
 };
-// rows of the W box the launch for these sizes loads (the map of W is made with it)
-int gemm_block_w_rows(int M, int N, int K);
 int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, cudaStream_t s);
 
 // cross_attn.cu -----------------------------------------------------------

@@ -724,6 +724,16 @@ def _call_on(dev: int, name: str, *args) -> None:
         _lib.check(rc, name)
 
 
+def _workspace_on(dev: int, name: str, *sizes: int) -> tuple[torch.Tensor | None, int]:
+    """The workspace that ``name`` asks for on device ``dev`` (it depends on the number of SMs), and its bytes."""
+    if torch._C._cuda_getDevice() == dev:
+        nb = getattr(_lib.lib(), name)(*sizes)
+    else:
+        with torch.cuda.device(dev):
+            nb = getattr(_lib.lib(), name)(*sizes)
+    return (torch.empty(nb, device=torch.device("cuda", dev), dtype=torch.uint8) if nb else None), nb
+
+
 def _empty_as(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """A new dense tensor of ``t``'s shape."""
     return torch.empty_like(t, dtype=dtype, memory_format=torch.contiguous_format)
@@ -849,8 +859,7 @@ def add_rms_norm_bwd(h: torch.Tensor, weight: torch.Tensor, rstd: torch.Tensor, 
     dres = None if res_dtype is None else dx if res_dtype == x_dtype else torch.empty_like(dx, dtype=res_dtype)
     dw = None if not need_dw else torch.empty_like(w) if M else torch.zeros_like(w)
     if M:
-        nb = _lib.lib().rola_b200_add_rms_norm_bwd_workspace(M, K) if need_dw else 0
-        ws = h.new_empty(nb, dtype=torch.uint8) if nb else None
+        ws, nb = _workspace_on(dev, "rola_b200_add_rms_norm_bwd_workspace", M, K) if need_dw else (None, 0)
         _call_on(dev, "rola_b200_add_rms_norm_bwd", hp, hf, h_ld, w.data_ptr(), wf, rstd.data_ptr(), yp, dy_ld, dp, df,
                  dh_ld, M, K, dx.data_ptr(), int(x_dtype is torch.float32), None if dres is dx else _ptr(dres),
                  int(res_dtype is torch.float32), _ptr(dw), _ptr(ws), nb)
@@ -987,8 +996,7 @@ def cross_attention_fwd_lse(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k
     if Lk == 0:
         return o.zero_(), None if lse is None else lse.fill_(float("inf"))
     (q, qa), (k, ka), (v, va) = _head_args(q), _head_args(k), _head_args(v)
-    nb = _lib.lib().rola_b200_cross_attn_workspace(*sizes)
-    ws = q.new_empty(nb, dtype=torch.uint8) if nb else None
+    ws, nb = _workspace_on(dev, "rola_b200_cross_attn_workspace", *sizes)
     _call_on(dev, "rola_b200_cross_attn", *qa, *ka, *va, _ptr(lens), *sizes, o.data_ptr(), Lq * H * HEAD_DIM, HEAD_DIM,
              H * HEAD_DIM, _ptr(lse), _ptr(ws), nb)
     return o, lse
@@ -1033,10 +1041,9 @@ def _cross_bwd(dev: int, sizes: tuple, q, k, v, o, do, lse, lens):
         return dq.zero_(), dk.zero_(), dv.zero_()
     (q, qa), (k, ka), (v, va), (o, oa) = _head_args(q), _head_args(k), _head_args(v), _head_args(o)
     do, da = _head_args(do if do.dtype is BF16 else do.to(BF16))
-    nb = _lib.lib().rola_b200_cross_attn_bwd_workspace(*sizes)
-    if nb == 0:
+    ws, nb = _workspace_on(dev, "rola_b200_cross_attn_bwd_workspace", *sizes)
+    if ws is None:
         raise ValueError("cross_attention_bwd: bad sizes")
-    ws = q.new_empty(nb, dtype=torch.uint8)
     _call_on(dev, "rola_b200_cross_attn_bwd", *qa, *ka, *va, *oa, *da, _ptr(lens), lse.data_ptr(), *sizes,
              dq.data_ptr(), Lq * H * HEAD_DIM, HEAD_DIM, H * HEAD_DIM, dk.data_ptr(), dv.data_ptr(),
              Lk * Hkv * HEAD_DIM, HEAD_DIM, Hkv * HEAD_DIM, ws.data_ptr(), nb)
