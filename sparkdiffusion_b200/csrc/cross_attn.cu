@@ -44,26 +44,27 @@ constexpr int REGS_LOAD = 56, REGS_SOFTMAX = 152;
 static_assert(128 * (REGS_LOAD + 3 * REGS_SOFTMAX) <= THREADS * LAUNCH_REGS, "register split");
 constexpr int BOX = 16384;        // [128 rows x 64 bf16], 128-byte swizzle
 constexpr int TILE = 2 * BOX;     // 128 rows x 128 columns
-constexpr int NQ = 2, NK = 2, NV = 3, NS = 3;
+constexpr int NQ = 2, NK = 2, NV = 3, NS = 2, NG = 3;  // S and P tiles; softmax warpgroups
 constexpr int OFF_Q = 0;
 constexpr int OFF_K = NQ * TILE, OFF_V = OFF_K + NK * TILE;
 constexpr int OFF_M = OFF_V + NV * TILE;  // [2][128] running maxima after even / odd units
 constexpr int OFF_L = OFF_M + 1024;         // [2][128] running sums
 constexpr int OFF_BAR = OFF_L + 1024;
 constexpr int SMEM = OFF_BAR + 512;
-constexpr int O_COL = 128 * NS;   // S of unit u at column 128 (u % 3), its P in the upper 64 of those; O behind them
+constexpr int O_COL = 128 * NS, P_COL = O_COL + 128;  // S of unit u at column 128 (u % 2); O; P at 64 (u % 2) behind it
 constexpr float RESCALE = 8.0f;   // log2 growth of the maximum that triggers a rescale of O
 enum : int {
   QF = 0, QE = QF + NQ,  // QE: the item's output is in its Q tile, 4 warp arrivals
   KF = QE + NQ, KE = KF + NK, VF = KE + NK, VE = VF + NV,
-  SF = VE + NV,      // S of a unit in TMEM: SF + u % 3
-  PB = SF + NS,      // P of keys [64, 128) in TMEM, 4 warp arrivals
+  SF = VE + NV,      // S of a unit in TMEM: SF + u % 3. As MR and LR below one barrier per warpgroup that waits:
+                     // one per tile could be two phases behind for it, which parity cannot tell from done
+  SR = SF + NG,      // S of a unit read, 4 warp arrivals: SR + u % 2, as PB, PA and PV
+  PB = SR + NS,      // P of keys [64, 128) in TMEM, 4 warp arrivals
   PA = PB + NS,      // P of keys [0, 64)
-  PV = PA + NS,      // P V of a unit done (its S columns are free, O holds it)
-  MR = PV + NS,      // m after unit u published: MR + u % 3, 4 arrivals (a single barrier would not do: the unit
-                     // that waits may find it two phases behind, which parity cannot tell from done)
-  LR = MR + NS,      // l after unit u published, 4 arrivals
-  OE = LR + NS,      // O read by the item's epilogue (phase: item), 4 arrivals
+  PV = PA + NS,      // P V of a unit done (its P columns are free, O holds it)
+  MR = PV + NS,      // m after unit u published: MR + u % 3, 4 arrivals
+  LR = MR + NG,      // l after unit u published, 4 arrivals
+  OE = LR + NG,      // O read by the item's epilogue (phase: item), 4 arrivals
   DRAIN_S = OE + 1,
   DRAIN_P,
   COUNT
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < COUNT; ++i) mbar_init(bar(i), (i >= QE && i < KF) || (i >= PB && i < PV) || (i >= MR && i < DRAIN_S) ? 4 : 1);
+    for (int i = 0; i < COUNT; ++i) mbar_init(bar(i), (i >= QE && i < KF) || (i >= SR && i < PV) || (i >= MR && i < DRAIN_S) ? 4 : 1);
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tq);
@@ -260,15 +261,15 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
     } else if (warp == 1) {
       // ------------------------------------------------------- MMA: S = Q K^T
       constexpr uint32_t id_qk = idesc_bf16_f32(128, 128, false, false);
-      int eq = 0, ek = 0, g = 0;
-      uint32_t q_ph = 0, k_ph = 0, g_ph = 1;  // g_ph: the buffer's previous unit is done (passes at first)
+      int eq = 0, ek = 0, g = 0, u3 = 0;
+      uint32_t q_ph = 0, k_ph = 0, g_ph = 1;  // g_ph: the buffer's previous unit is read (passes at first)
       for (CrossItems it(p); it.live(p) && ok; it.next(p)) {
         const int cnt = __shfl_sync(0xffffffffu, it.cnt, 0);
         if (cnt == 0) continue;
         if (!wait(QF + eq, q_ph, kDevTimeoutLoad)) break;
         const uint32_t dq = sdesc_lo(base + OFF_Q + eq * TILE, 16);
         for (int i = 0; i < cnt; ++i) {
-          if (!wait(KF + ek, k_ph, kDevTimeoutLoad) || !wait(PV + g, g_ph, kDevTimeoutMma)) break;
+          if (!wait(KF + ek, k_ph, kDevTimeoutLoad) || !wait(SR + g, g_ph, kDevTimeoutSoftmax)) break;
           if (elect_one()) {
             const uint32_t dk = sdesc_lo(base + OFF_K + ek * TILE, 16);
 #pragma unroll
@@ -276,10 +277,11 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
               const uint32_t off = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
               mma_bf16_ss_lo(tmem + 128 * g, dq + off, hi, dk + off, hi, id_qk, kk > 0 ? 1u : 0u);
             }
-            mma_commit(bar(SF + g));
+            mma_commit(bar(SF + u3));
             mma_commit(bar(KE + ek));
           }
           __syncwarp();
+          if (++u3 == NG) u3 = 0;
           if (++ek == NK) {
             ek = 0;
             k_ph ^= 1u;
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
           if (tail < 128 && i + 1 == cnt) clear_rows(smem1k + OFF_V + ev * TILE, tail, lane);
           // O of the previous item has been read
           if (i == 0 && !wait(OE, o_ph, kDevTimeoutSoftmax)) break;
-          const uint32_t dv = sdesc_lo(base + OFF_V + ev * TILE, BOX), tp = tmem + 128 * g + 64;
+          const uint32_t dv = sdesc_lo(base + OFF_V + ev * TILE, BOX), tp = tmem + P_COL + 64 * g;
 #pragma unroll
           for (int half = 1; half >= 0; --half) {  // keys [64, 128) first, as the softmax hands them over
             if (!wait((half ? PB : PA) + g, g_ph, kDevTimeoutSoftmax)) break;
@@ -356,7 +358,7 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
     // ------------------------------------------------------- softmax and output
     const int g = (warp >> 2) - 1, q = warp & 3, row = q * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q * 32) << 16;
-    const uint32_t tS = tmem + 128 * g + lane_off, tO = tmem + O_COL + lane_off;
+    const uint32_t tO = tmem + O_COL + lane_off;
     float* s_m = reinterpret_cast<float*>(smem1k + OFF_M) + row;
     float* s_l = reinterpret_cast<float*>(smem1k + OFF_L) + row;
     const float scale = p.qk_scale;
@@ -387,53 +389,53 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
         continue;
       }
       for (int i = 0; i < it.cnt && ok; ++i, ++u) {
-        if (u % NS != g) continue;
+        if (u % NG != g) continue;
+        const int s = u % NS;
         const uint32_t ph = (u / NS) & 1;
-        if (!wait(SF + g, ph, kDevTimeoutMma)) break;
+        const uint32_t tS = tmem + 128 * s + lane_off, tP = tmem + P_COL + 64 * s + lane_off;
+        if (!wait(SF + g, (u / NG) & 1, kDevTimeoutMma)) break;
         tc_fence_after();
-        // maximum of the row; the upper 64 scores stay in registers (P takes their
-        // place in TMEM), the lower 64 are read again for the exponentials
+        // maximum of the row, 32 columns at a time; the last two chunks stay in registers,
+        // the first two are read again for the exponentials.  The loops over chunks stay
+        // loops: unrolled, three warpgroups' places in the code overran the instruction
+        // cache (28 % of their time)
         const int valid = it.len - (it.i0 + i) * 128;
-        uint32_t hi[64];
-        float mx;
-        {
-          uint32_t lo[64];
-          tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&lo[0]));
-          tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&lo[32]));
-          tmem_ld_wait();
-          if (valid < 64) {
+        uint32_t v[2][32];
+        if (valid < 128) {  // scores past the last key: -inf, in tensor memory
+#pragma unroll 1
+          for (int c = valid; c < 128;) {
+            if (c & 15) {
+              tmem_st1(tS + c++, 0xff800000u);
+            } else {
+              uint32_t w[16];
 #pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (c >= valid) lo[c] = __float_as_uint(-INFINITY);
+              for (int e = 0; e < 16; ++e) w[e] = 0xff800000u;
+              tmem_st16(tS + c, w);
+              c += 16;
+            }
           }
-          float m4[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            m4[k] = __uint_as_float(lo[k]);
-#pragma unroll
-            for (int e = 0; e < 7; ++e)
-              m4[k] = max3f(m4[k], __uint_as_float(lo[k + 4 + 8 * e]), __uint_as_float(lo[k + 8 + 8 * e]));
-            m4[k] = fmaxf(m4[k], __uint_as_float(lo[k + 60]));
-          }
-          tmem_ld32(tS + 64, *reinterpret_cast<uint32_t(*)[32]>(&hi[0]));
-          tmem_ld32(tS + 96, *reinterpret_cast<uint32_t(*)[32]>(&hi[32]));
-          tmem_ld_wait();
-          if (valid < 128) {
-#pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (64 + c >= valid) hi[c] = __float_as_uint(-INFINITY);
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              m4[k] = max3f(m4[k], __uint_as_float(hi[k + 8 * e]), __uint_as_float(hi[k + 4 + 8 * e]));
-          }
-          mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+          tmem_st_wait();
         }
+        float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        auto fold = [&](const uint32_t(&x)[32]) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              m4[k] = max3f(m4[k], __uint_as_float(x[k + 8 * e]), __uint_as_float(x[k + 4 + 8 * e]));
+        };
+#pragma unroll 1
+        for (int c = 0; c < 4; c += 2) {
+          tmem_ld32(tS + 32 * c, v[0]);
+          tmem_ld32(tS + 32 * c + 32, v[1]);
+          tmem_ld_wait();
+          fold(v[0]);
+          fold(v[1]);
+        }
+        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         // m after this unit, from the unit before (published in unit order)
         float m = fmaxf(mx * scale, -FLT_MAX), alpha = 1.f;  // finite, should every score be -inf
-        if (u > 0 && !wait(MR + (u + NS - 1) % NS, ((u - 1) / NS) & 1, kDevTimeoutSoftmax)) break;
+        if (u > 0 && !wait(MR + (u - 1) % NG, ((u - 1) / NG) & 1, kDevTimeoutSoftmax)) break;
         if (i > 0) {
           const float m_prev = s_m[128 * ((u & 1) ^ 1)];
           if (m - m_prev > RESCALE) {
@@ -445,12 +447,16 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
         s_m[128 * (u & 1)] = m;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(MR + g));
+        // the P tile's previous unit is done (S was read after that unit's own such wait,
+        // so the barrier is one phase behind at most)
+        if (!wait(PV + s, ph ^ 1u, kDevTimeoutMma)) break;
+        tc_fence_after();
         if (__any_sync(0xffffffffu, alpha != 1.f)) {
-          // O of the units before, once the last of them is in
-          if (!wait(PV + (u + NS - 1) % NS, ((u - 1) / NS) & 1, kDevTimeoutMma)) break;
+          // O of the units before, once the last of them is in (the one before that is, by the wait above)
+          if (!wait(PV + (s ^ 1), ((u - 1) / NS) & 1, kDevTimeoutMma)) break;
           tc_fence_after();
           const uint64_t a2 = f2_pack(alpha, alpha);
-#pragma unroll
+#pragma unroll 1
           for (int c = 0; c < 4; ++c) {
             uint32_t ov[32];
             tmem_ld32(tO + 32 * c, ov);
@@ -468,47 +474,44 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
         }
         const uint64_t sc2 = f2_pack(scale, scale), nm2 = f2_pack(-m, -m);
         uint64_t rs2[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-        // P of 32 keys, packed bf16, over 16 columns of the upper half of S
-        auto exp32 = [&](const uint32_t* v, int c) {
+        // P of 32 keys, packed bf16
+        auto exp32 = [&](const uint32_t(&x)[32], int c) {
           uint32_t pw[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             float x0, x1;
-            f2_unpack(fma_f32x2(f2_pack(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), sc2, nm2), x0, x1);
+            f2_unpack(fma_f32x2(f2_pack(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1])), sc2, nm2), x0, x1);
             const float p0 = ex2_approx(x0), p1 = ex2_approx(x1);
             rs2[e & 1] = add_f32x2(rs2[e & 1], f2_pack(p0, p1));
             pw[e] = pack_bf2(p0, p1);
           }
-          tmem_st16(tS + 64 + 16 * c, pw);
+          tmem_st16(tP + 16 * c, pw);
         };
         auto publish = [&](int b) {
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(b + g));
+          if (lane == 0) mbar_arrive(bar(b + s));
         };
-        exp32(hi, 2);
-        exp32(hi + 32, 3);
-        {
-          uint32_t lo[64];
-          tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&lo[0]));
-          tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&lo[32]));
-          publish(PB);
-          tmem_ld_wait();
-          if (valid < 64) {
-#pragma unroll
-            for (int c = 0; c < 64; ++c)
-              if (c >= valid) lo[c] = __float_as_uint(-INFINITY);
+#pragma unroll 1
+        for (int c = 2; c >= 0; c -= 2) {
+          exp32(v[1], c + 1);
+          if (c == 2) tmem_ld32(tS + 32, v[1]);
+          exp32(v[0], c);
+          if (c == 2) tmem_ld32(tS, v[0]);
+          publish(c == 2 ? PB : PA);
+          if (c == 2) {
+            tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(SR + s));
           }
-          exp32(lo, 0);
-          exp32(lo + 32, 1);
-          publish(PA);
         }
         float ra, rb, rc, rd;
         f2_unpack(rs2[0], ra, rb);
         f2_unpack(rs2[1], rc, rd);
         float l = (ra + rc) + (rb + rd);
-        if (u > 0 && !wait(LR + (u + NS - 1) % NS, ((u - 1) / NS) & 1, kDevTimeoutSoftmax)) break;
+        if (u > 0 && !wait(LR + (u - 1) % NG, ((u - 1) / NG) & 1, kDevTimeoutSoftmax)) break;
         if (i > 0) l = fmaf(s_l[128 * ((u & 1) ^ 1)], alpha, l);
         s_l[128 * (u & 1)] = l;
         __syncwarp();
@@ -519,13 +522,13 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
         int h, tok;
         const bool live = it.row(p, row, h, tok);
         const float inv_l = 1.0f / l, lse = m + log2f(l);
-        if (!wait(PV + g, ph, kDevTimeoutMma)) break;
+        if (!wait(PV + s, ph, kDevTimeoutMma)) break;
         tc_fence_after();
         const int64_t prow = (((int64_t)it.split * p.B + it.b) * p.H + h) * p.Lq + tok;
         // the row of the item's Q tile, whose last product is done: 16-byte chunk c of a
         // box at c ^ (row & 7), the maps' swizzle
         uint8_t* stage = smem1k + OFF_Q + (j % NQ) * TILE + row * 128;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           uint32_t v[64];
           __syncwarp();  // the stores of a slice's partial diverge, the load is warp-collective
