@@ -44,27 +44,28 @@ constexpr int REGS_LOAD = 56, REGS_SOFTMAX = 152;
 static_assert(128 * (REGS_LOAD + 3 * REGS_SOFTMAX) <= THREADS * LAUNCH_REGS, "register split");
 constexpr int BOX = 16384;        // [128 rows x 64 bf16], 128-byte swizzle
 constexpr int TILE = 2 * BOX;     // 128 rows x 128 columns
-constexpr int NQ = 2, NK = 2, NV = 3, NS = 2, NG = 3;  // S and P tiles; softmax warpgroups
+constexpr int NQ = 2, NK = 2, NV = 3, NS = 3;
 constexpr int OFF_Q = 0;
 constexpr int OFF_K = NQ * TILE, OFF_V = OFF_K + NK * TILE;
 constexpr int OFF_M = OFF_V + NV * TILE;  // [2][128] running maxima after even / odd units
 constexpr int OFF_L = OFF_M + 1024;         // [2][128] running sums
 constexpr int OFF_BAR = OFF_L + 1024;
 constexpr int SMEM = OFF_BAR + 512;
-constexpr int O_COL = 128 * NS, P_COL = O_COL + 128;  // S of unit u at column 128 (u % 2); O; P at 64 (u % 2) behind it
+constexpr int O_COL = 128 * NS;   // S of unit u at column 128 (u % 3), its P in the upper 64 of those; O behind them
 constexpr float RESCALE = 8.0f;   // log2 growth of the maximum that triggers a rescale of O
 enum : int {
-  QF = 0, QE = QF + NQ,  // QE: the item's output is in its Q tile, 4 warp arrivals
+  QF = 0, QE = QF + NQ,
   KF = QE + NQ, KE = KF + NK, VF = KE + NK, VE = VF + NV,
-  SF = VE + NV,      // S of a unit in TMEM: SF + u % 3. As MR and LR below one barrier per warpgroup that waits:
-                     // one per tile could be two phases behind for it, which parity cannot tell from done
-  SR = SF + NG,      // S of a unit read, 4 warp arrivals: SR + u % 2, as PB, PA and PV
-  PB = SR + NS,      // P of keys [64, 128) in TMEM, 4 warp arrivals
+  SF = VE + NV,      // S of a unit in TMEM: SF + u % 3, as those below
+  PB = SF + NS,      // P of keys [64, 128) in TMEM, 4 warp arrivals
   PA = PB + NS,      // P of keys [0, 64)
-  PV = PA + NS,      // P V of a unit done (its P columns are free, O holds it)
-  MR = PV + NS,      // m after unit u published: MR + u % 3, 4 arrivals
-  LR = MR + NG,      // l after unit u published, 4 arrivals
-  OE = LR + NG,      // O read by the item's epilogue (phase: item), 4 arrivals
+  OV = PA + NS,      // output of an item in the V tile of its last unit, 4 arrivals: OV + u % 3
+  OQ = OV + NV,      // output of an item in its Q tile, 4 arrivals
+  PV = OQ + NQ,      // P V of a unit done (its S columns are free, O holds it)
+  MR = PV + NS,      // m after unit u published, 4 arrivals (a single barrier would not do: the unit that waits
+                     // may find it two phases behind, which parity cannot tell from done)
+  LR = MR + NS,      // l after unit u published, 4 arrivals
+  OE = LR + NS,      // O read by the item's epilogue (phase: item), 4 arrivals
   DRAIN_S = OE + 1,
   DRAIN_P,
   COUNT
@@ -72,6 +73,12 @@ enum : int {
 static_assert(8 * COUNT + 16 <= 512, "barrier region");
 static_assert(SMEM <= 227 * 1024, "shared memory");
 }  // namespace xattn
+
+// Where an item's output waits for its TMA store.  A Q tile that holds one is loaded
+// late, which an item of one or two units cannot hide from the S products three units
+// on; a V tile is held up by the store, which costs the others 3 % (32760 x 128 / 256 /
+// 512, 40 heads, us: in Q tiles 182 / 217 / 327, in V tiles 154 / 207 / 341).
+__device__ __forceinline__ bool out_in_q(int units) { return units >= 3; }
 
 // valid keys of batch b
 __device__ __forceinline__ int kv_len(const int32_t* lens, int b, int Lk) {
@@ -166,7 +173,7 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < COUNT; ++i) mbar_init(bar(i), (i >= QE && i < KF) || (i >= SR && i < PV) || (i >= MR && i < DRAIN_S) ? 4 : 1);
+    for (int i = 0; i < COUNT; ++i) mbar_init(bar(i), (i >= PB && i < PV) || (i >= MR && i < DRAIN_S) ? 4 : 1);
     *abort_flag = 0;
     fence_barrier_init();
     prefetch_tmap(&tq);
@@ -193,33 +200,42 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
       tc_fence_after();
       return ok;
     };
+    // An item's output waits in one of its tiles until that is loaded again: the tiles
+    // of one ring that hold one
+    struct Outputs {
+      uint32_t held = 0, phase = 0;  // bits: tile f holds the output of an item; phase of its barrier
+      int m[NV] = {}, h[NV] = {}, b[NV] = {};
+      __device__ __forceinline__ void expect(int f, const CrossItems& it, const CrossAttnParams& p) {
+        held |= 1u << f;
+        m[f] = it.m * 128, h[f] = p.pack ? it.h * p.G : it.h, b[f] = it.b;
+      }
+    };
+    auto store_out = [&](Outputs& o, int f, uint32_t tile, int staged) {
+      if (!((o.held >> f) & 1)) return true;
+      if (!mbar_spin(bar(staged), (o.phase >> f) & 1, abort_flag, kDevTimeoutSoftmax)) return false;
+      o.held ^= 1u << f;
+      o.phase ^= 1u << f;
+      tma_store_4d(&to, tile, 0, o.m[f], o.h[f], o.b[f]);
+      tma_store_4d(&to, tile + BOX, 64, o.m[f], o.h[f], o.b[f]);
+      tma_store_commit();
+      tma_store_wait_read();
+      return true;
+    };
     if (warp == 0) {
       if (lane == 0) {
-        // -------------------------------------------- TMA: Q and K; the output
+        // -------------------------------------------- TMA: Q and K; outputs in Q tiles
         int q = 0, k = 0;  // tiles loaded
-        int om[NQ] = {}, oh[NQ] = {}, ob[NQ] = {};  // the items whose Q tiles are loaded
-        // output of the item in Q tile e, the n-th of that tile
-        auto store_out = [&](int e, int n) {
-          if (!mbar_spin(bar(QE + e), n & 1, abort_flag, kDevTimeoutSoftmax, 2 * (uint32_t)(p.Lk >> 7))) return false;
-          if (p.nsplit == 1) {
-            tma_store_4d(&to, base + OFF_Q + e * TILE, 0, om[e] * 128, oh[e], ob[e]);
-            tma_store_4d(&to, base + OFF_Q + e * TILE + BOX, 64, om[e] * 128, oh[e], ob[e]);
-            tma_store_commit();
-            tma_store_wait_read();
-          }
-          return true;
-        };
+        Outputs outs;
         for (CrossItems it(p); it.live(p) && ok; it.next(p)) {
           if (it.cnt == 0) continue;
           const int e = q % NQ;
-          if (q >= NQ && !(ok = store_out(e, q / NQ - 1))) break;
+          if (!(ok = mbar_spin(bar(QE + e), ((q / NQ) & 1) ^ 1, abort_flag, kDevTimeoutMma))) break;
+          if (!(ok = store_out(outs, e, base + OFF_Q + e * TILE, OQ + e))) break;
+          if (p.nsplit == 1 && out_in_q(it.cnt)) outs.expect(e, it, p);
           mbar_expect_tx(bar(QF + e), p.q_bytes);
           const int hq = p.pack ? it.h * p.G : it.h, hk = p.pack ? it.h : it.h / p.G;
           tma_load_4d(base + OFF_Q + e * TILE, &tq, bar(QF + e), 0, it.m * 128, hq, it.b);
           tma_load_4d(base + OFF_Q + e * TILE + BOX, &tq, bar(QF + e), 64, it.m * 128, hq, it.b);
-          om[e] = it.m;
-          oh[e] = hq;
-          ob[e] = it.b;
           ++q;
           for (int i = it.i0; i < it.i0 + it.cnt; ++i, ++k) {
             const int f = k % NK;
@@ -229,7 +245,8 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
             tma_load_4d(base + OFF_K + f * TILE + BOX, &tk, bar(KF + f), 64, i * 128, hk, it.b);
           }
         }
-        for (int n = max(0, q - NQ); n < q && ok; ++n) ok = store_out(n % NQ, n / NQ);
+        for (int n = max(0, q - NQ); n < q && ok; ++n)
+          ok = store_out(outs, n % NQ, base + OFF_Q + n % NQ * TILE, OQ + n % NQ);
         // no copy may still target shared memory when the CTA exits; the waits
         // ignore the abort flag and share one limit
         const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
@@ -241,18 +258,23 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
       }
     } else if (warp == 3) {
       if (lane == 0) {
-        // ------------------------------------------------------------ TMA: V
+        // ------------------------------------------------ TMA: V; outputs in V tiles
         int k = 0;
+        Outputs outs;
         for (CrossItems it(p); it.live(p) && ok; it.next(p)) {
           const int hk = p.pack ? it.h : it.h / p.G;
           for (int i = it.i0; i < it.i0 + it.cnt; ++i, ++k) {
             const int f = k % NV;
             if (!(ok = mbar_spin(bar(VE + f), ((k / NV) & 1) ^ 1, abort_flag, kDevTimeoutMma))) break;
+            if (!(ok = store_out(outs, f, base + OFF_V + f * TILE, OV + f))) break;
             mbar_expect_tx(bar(VF + f), TILE);
             tma_load_4d(base + OFF_V + f * TILE, &tv, bar(VF + f), 0, i * 128, hk, it.b);
             tma_load_4d(base + OFF_V + f * TILE + BOX, &tv, bar(VF + f), 64, i * 128, hk, it.b);
+            if (p.nsplit == 1 && i + 1 == it.i0 + it.cnt && !out_in_q(it.cnt)) outs.expect(f, it, p);
           }
         }
+        for (int n = max(0, k - NV); n < k && ok; ++n)
+          ok = store_out(outs, n % NV, base + OFF_V + n % NV * TILE, OV + n % NV);
         const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
         bool drained = true;
         for (int n = max(0, k - NV); n < k && drained; ++n)
@@ -261,15 +283,15 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
     } else if (warp == 1) {
       // ------------------------------------------------------- MMA: S = Q K^T
       constexpr uint32_t id_qk = idesc_bf16_f32(128, 128, false, false);
-      int eq = 0, ek = 0, g = 0, u3 = 0;
-      uint32_t q_ph = 0, k_ph = 0, g_ph = 1;  // g_ph: the buffer's previous unit is read (passes at first)
+      int eq = 0, ek = 0, g = 0;
+      uint32_t q_ph = 0, k_ph = 0, g_ph = 1;  // g_ph: the buffer's previous unit is done (passes at first)
       for (CrossItems it(p); it.live(p) && ok; it.next(p)) {
         const int cnt = __shfl_sync(0xffffffffu, it.cnt, 0);
         if (cnt == 0) continue;
         if (!wait(QF + eq, q_ph, kDevTimeoutLoad)) break;
         const uint32_t dq = sdesc_lo(base + OFF_Q + eq * TILE, 16);
         for (int i = 0; i < cnt; ++i) {
-          if (!wait(KF + ek, k_ph, kDevTimeoutLoad) || !wait(SR + g, g_ph, kDevTimeoutSoftmax)) break;
+          if (!wait(KF + ek, k_ph, kDevTimeoutLoad) || !wait(PV + g, g_ph, kDevTimeoutMma)) break;
           if (elect_one()) {
             const uint32_t dk = sdesc_lo(base + OFF_K + ek * TILE, 16);
 #pragma unroll
@@ -277,11 +299,11 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
               const uint32_t off = ((kk >> 2) * BOX + (kk & 3) * 32) >> 4;
               mma_bf16_ss_lo(tmem + 128 * g, dq + off, hi, dk + off, hi, id_qk, kk > 0 ? 1u : 0u);
             }
-            mma_commit(bar(SF + u3));
+            mma_commit(bar(SF + g));
             mma_commit(bar(KE + ek));
+            if (i + 1 == cnt) mma_commit(bar(QE + eq));
           }
           __syncwarp();
-          if (++u3 == NG) u3 = 0;
           if (++ek == NK) {
             ek = 0;
             k_ph ^= 1u;
@@ -318,7 +340,7 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
           if (tail < 128 && i + 1 == cnt) clear_rows(smem1k + OFF_V + ev * TILE, tail, lane);
           // O of the previous item has been read
           if (i == 0 && !wait(OE, o_ph, kDevTimeoutSoftmax)) break;
-          const uint32_t dv = sdesc_lo(base + OFF_V + ev * TILE, BOX), tp = tmem + P_COL + 64 * g;
+          const uint32_t dv = sdesc_lo(base + OFF_V + ev * TILE, BOX), tp = tmem + 128 * g + 64;
 #pragma unroll
           for (int half = 1; half >= 0; --half) {  // keys [64, 128) first, as the softmax hands them over
             if (!wait((half ? PB : PA) + g, g_ph, kDevTimeoutSoftmax)) break;
@@ -358,7 +380,7 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
     // ------------------------------------------------------- softmax and output
     const int g = (warp >> 2) - 1, q = warp & 3, row = q * 32 + lane;
     const uint32_t lane_off = (uint32_t)(q * 32) << 16;
-    const uint32_t tO = tmem + O_COL + lane_off;
+    const uint32_t tS = tmem + 128 * g + lane_off, tP = tS + 64, tO = tmem + O_COL + lane_off;
     float* s_m = reinterpret_cast<float*>(smem1k + OFF_M) + row;
     float* s_l = reinterpret_cast<float*>(smem1k + OFF_L) + row;
     const float scale = p.qk_scale;
@@ -389,11 +411,9 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
         continue;
       }
       for (int i = 0; i < it.cnt && ok; ++i, ++u) {
-        if (u % NG != g) continue;
-        const int s = u % NS;
+        if (u % NS != g) continue;
         const uint32_t ph = (u / NS) & 1;
-        const uint32_t tS = tmem + 128 * s + lane_off, tP = tmem + P_COL + 64 * s + lane_off;
-        if (!wait(SF + g, (u / NG) & 1, kDevTimeoutMma)) break;
+        if (!wait(SF + g, ph, kDevTimeoutMma)) break;
         tc_fence_after();
         // maximum of the row, 32 columns at a time; the last two chunks stay in registers,
         // the first two are read again for the exponentials.  The loops over chunks stay
@@ -435,7 +455,7 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
         const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
         // m after this unit, from the unit before (published in unit order)
         float m = fmaxf(mx * scale, -FLT_MAX), alpha = 1.f;  // finite, should every score be -inf
-        if (u > 0 && !wait(MR + (u - 1) % NG, ((u - 1) / NG) & 1, kDevTimeoutSoftmax)) break;
+        if (u > 0 && !wait(MR + (u - 1) % NS, ((u - 1) / NS) & 1, kDevTimeoutSoftmax)) break;
         if (i > 0) {
           const float m_prev = s_m[128 * ((u & 1) ^ 1)];
           if (m - m_prev > RESCALE) {
@@ -447,13 +467,9 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
         s_m[128 * (u & 1)] = m;
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(MR + g));
-        // the P tile's previous unit is done (S was read after that unit's own such wait,
-        // so the barrier is one phase behind at most)
-        if (!wait(PV + s, ph ^ 1u, kDevTimeoutMma)) break;
-        tc_fence_after();
         if (__any_sync(0xffffffffu, alpha != 1.f)) {
-          // O of the units before, once the last of them is in (the one before that is, by the wait above)
-          if (!wait(PV + (s ^ 1), ((u - 1) / NS) & 1, kDevTimeoutMma)) break;
+          // O of the units before, once the last of them is in
+          if (!wait(PV + (u - 1) % NS, ((u - 1) / NS) & 1, kDevTimeoutMma)) break;
           tc_fence_after();
           const uint64_t a2 = f2_pack(alpha, alpha);
 #pragma unroll 1
@@ -491,7 +507,7 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(b + s));
+          if (lane == 0) mbar_arrive(bar(b + g));
         };
 #pragma unroll 1
         for (int c = 2; c >= 0; c -= 2) {
@@ -500,18 +516,13 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
           exp32(v[0], c);
           if (c == 2) tmem_ld32(tS, v[0]);
           publish(c == 2 ? PB : PA);
-          if (c == 2) {
-            tmem_ld_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(SR + s));
-          }
+          if (c == 2) tmem_ld_wait();
         }
         float ra, rb, rc, rd;
         f2_unpack(rs2[0], ra, rb);
         f2_unpack(rs2[1], rc, rd);
         float l = (ra + rc) + (rb + rd);
-        if (u > 0 && !wait(LR + (u - 1) % NG, ((u - 1) / NG) & 1, kDevTimeoutSoftmax)) break;
+        if (u > 0 && !wait(LR + (u - 1) % NS, ((u - 1) / NS) & 1, kDevTimeoutSoftmax)) break;
         if (i > 0) l = fmaf(s_l[128 * ((u & 1) ^ 1)], alpha, l);
         s_l[128 * (u & 1)] = l;
         __syncwarp();
@@ -522,12 +533,13 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
         int h, tok;
         const bool live = it.row(p, row, h, tok);
         const float inv_l = 1.0f / l, lse = m + log2f(l);
-        if (!wait(PV + s, ph, kDevTimeoutMma)) break;
+        if (!wait(PV + g, ph, kDevTimeoutMma)) break;
         tc_fence_after();
         const int64_t prow = (((int64_t)it.split * p.B + it.b) * p.H + h) * p.Lq + tok;
-        // the row of the item's Q tile, whose last product is done: 16-byte chunk c of a
-        // box at c ^ (row & 7), the maps' swizzle
-        uint8_t* stage = smem1k + OFF_Q + (j % NQ) * TILE + row * 128;
+        // the row of the item's Q tile or the unit's V tile, whose products are done: 16-byte
+        // chunk c of a box at c ^ (row & 7), the maps' swizzle
+        const bool in_q = out_in_q(it.cnt);
+        uint8_t* stage = smem1k + (in_q ? OFF_Q + (j % NQ) * TILE : OFF_V + (u % NV) * TILE) + row * 128;
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
           uint32_t v[64];
@@ -558,9 +570,11 @@ __global__ void __launch_bounds__(xattn::THREADS, 1)
                                   __uint_as_float(v[4 * e + 2]) * inv_l, __uint_as_float(v[4 * e + 3]) * inv_l);
           }
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar(QE + j % NQ));
+        if (p.nsplit == 1) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(in_q ? OQ + j % NQ : OV + u % NV));
+        }
         if (p.nsplit > 1) {
           if (live) p.part_lse[prow] = lse;
         } else if (p.lse && (live || !p.pack)) {
