@@ -57,9 +57,12 @@ __device__ __forceinline__ void store_row(const uint64_t (&acc)[n], const __nv_b
 // streams (column halves) of two, and a warpgroup of the epilogue each (128 sums
 // a thread; the registers of the producer's warpgroup go to them by setmaxnreg);
 // BN = 128 one stream of four that both warpgroups share, 64 columns each.
-// Measured at 32760 x 15360 x 5120 (TFLOP/s): BN = 256 1780, with neither
-// hand-off nor epilogue 2860 (operands from L2), hand-offs alone 2270; SM pairs
-// (256 x 256 tiles, whose hand-offs cross SMs) 1340 with the hand-offs alone.
+// Measured at 32760 x 15360 x 5120 (TFLOP/s): BN = 256 1939 alone (2657 us; 0.58 of
+// twice the bf16 peak), 1650 in a long run under the power limit; with neither
+// hand-off nor epilogue 2860 (operands from L2), hand-offs alone 2270, which is what
+// bounds it: every 128 columns x 128 k of products, 64 x 4 clocks of the tensor core,
+// pass through a barrier each way.  SM pairs (256 x 256 tiles, whose hand-offs cross
+// SMs) 1340 with the hand-offs alone.
 // A warp of its own copies the scales of the next kScales blocks into shared
 // memory (4-byte cp.async, so any strides): loaded by the epilogue itself, even
 // four blocks ahead, they held it to one L2 access per block (1260 TFLOP/s).
@@ -400,7 +403,10 @@ static int launch_gemm_block_few_rows(const GemmBlockParams& p, cudaStream_t s) 
 }
 
 // The wider tile unless its last wave of CTAs is so empty that the narrower one,
-// at 0.57 of its time a tile (measured), finishes first
+// at about 0.6 of its time a tile, finishes first (M x N x K, us, wide | narrow, waves
+// in brackets: 512 x 5120 x 5120 28.2 (1) | 32.8 (2), 1001 x 5120 x 5120 50.0 (2) |
+// 46.0 (3), 4096 x 5120 x 5120 120 (5) | 130 (9), 32760 x 15360 x 5120 2650 | 3040;
+// one wave of each, 128 x 5120 x 5120, 27.5 | 19.5)
 int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, cudaStream_t s) {
   // Up to 8 rows the weight's bytes decide (M = 8, us, few rows | tiles: N x K =
   // 15360 x 5120 18.9 | 19.5, 5120 x 5120 9.1 | 17, 1536 x 1536 3.7 | 7.8); from 9
@@ -411,7 +417,7 @@ int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBl
   const int sms = device_sms();
   const int64_t num_m = (p.M + 127) / 128;
   const int64_t wide = (num_m * ((p.N + 255) / 256) + sms - 1) / sms, narrow = (num_m * ((p.N + 127) / 128) + sms - 1) / sms;
-  return narrow * 57 < wide * 100 ? launch_gemm_block_bn<128>(ta, tb, p, sms, s)
+  return narrow * 60 < wide * 100 ? launch_gemm_block_bn<128>(ta, tb, p, sms, s)
                                   : launch_gemm_block_bn<256>(ta, tb, p, sms, s);
 }
 

@@ -1,6 +1,6 @@
 """Host-side ops of the B200 RoLa attention forward.
 
-Two layers of API:
+Three layers of API:
 
 * ``rola_attention_core`` / ``rola_attention_from_qkv``: the fused B200 path
   used by the drop-in layer.  Activations stay token-major ``[B, L, H*D]``
@@ -9,7 +9,10 @@ Two layers of API:
 * reference-named functions mirroring ``sparkdiffusion.ops.fused_kernel``
   (``fused_qkv_gemm_rope``, ``mean_pool``, ``fused_sparse_attn``) with the
   reference's argument meaning, layouts and ``ValueError``s, so callers and
-  tests written against the reference read the same.
+  tests written against the reference read the same;
+* the operators of the cross-attention sublayer that follows in a block: norm with
+  the residual's addition, e4m3 quantisation and product with a scale per block
+  of 128, attention to states of another length (``add_rms_norm`` and below).
 
 Every function launches librola_b200 kernels on the current CUDA stream and
 raises if the library is missing or the tensors are not on a CUDA device:

@@ -12,6 +12,11 @@ B200 selection kernels and the attention's forward (with the row
 log-sum-exp) and backward on the tcgen05 kernels (``BlockSparseAttention``);
 the eager parts stay eager PyTorch, as in the reference.  There is no
 fallback: the attention raises without the CUDA library.
+
+``add_rms_norm`` and ``cross_attention`` are the differentiable operators of the
+block's next sublayer.  A backward of any of these functions may be captured
+into a CUDA graph as long as no eager autograd graph of the same leaf tensors is
+alive (PyTorch would order the captured backward after the eager graph's stream).
 """
 
 from __future__ import annotations

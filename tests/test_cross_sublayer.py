@@ -564,6 +564,8 @@ PRODUCT = {
     "rows_33": (33, 520, 400, False),
     "tile_tails": (129, 136, 272, True),
     "rows_300": (300, 1032, 1536, True),
+    "rows_16_narrow": (16, 1536, 1536, False),
+    "rows_16_wide": (16, 9000, 400, True),
     "tall": (2049, 24, 128, False),
     "many_tiles": (1500, 2600, 656, True),
     # several tiles a CTA, of both widths
