@@ -38,7 +38,11 @@ __device__ __forceinline__ void clear_half_rows(uint8_t* half, int valid, int la
 // A step is a chain, (S, dP) -> dS -> dQ, three in flight across the items' ends
 // (S and dP of a step take 128 columns of tensor memory, dQ 128), as the units of
 // cross_attn_tcgen05; one CTA per item spent more time on its ends than on the 8
-// steps of 512 keys (1.06 ms at 32760 x 512, 40 heads).
+// steps of 512 keys (1.06 ms at 32760 x 512, 40 heads; now 0.53: 965 TFLOP/s, 0.58 of
+// the matrix peak).  The three chains bound it, 4150 clocks each: 3 x 256 of products,
+// about 2000 of the softmax warpgroup, the hand-offs between them.  Tried and slower:
+// S ahead of the dQ of the step before in its columns (0.64), dQ read by warpgroup 4
+// (0.57), rings of 3 K and 3 V tiles (0.6).
 //   warp 0   TMA producer of Q and dO (2 x 64 KB); it also stores an item's dQ,
 //            left in the item's Q tile, before that is loaded again
 //   warp 3   TMA producer of K (4 x 16 KB) and V (2 x 16 KB)
@@ -478,9 +482,11 @@ __global__ void __launch_bounds__(xdq::THREADS, 1)
 // that hold a valid key, one tile after the other, are dealt to the CTAs in equal
 // runs.  A CTA's run is a few segments, each within one tile; a tile within one
 // run is stored as it is, the others' segments leave fp32 partials that
-// cross_bwd_join_kernel adds in order (an encoder's states are few tiles: 160 at
-// 512 states and 40 heads; 12 slices of each as CTAs of their own took 0.64 ms
-// with the join, of it 0.1 in their ends and last round).
+// cross_bwd_join_kernel adds in order.  (An encoder's states are few tiles: 160 at
+// 512 states and 40 heads.  12 slices of each as CTAs of their own took 0.64 ms with
+// the join, of it 0.1 in their ends and last round.)  Measured there: 0.56 ms and
+// 0.013 for the join, 1220 TFLOP/s, 0.73 of the matrix peak; two steps in flight,
+// which is all that tensor memory holds beside dV and dK, bound it.
 //   warp 0   TMA producer: K and V of the tile, the ring of (Q, dO, lse, delta)
 //   warp 1   issues S^T = K Q^T and dP^T = V dO^T of a step, then dV += P^T dO and
 //            dK += dS^T Q of the step before: in one warp's order the columns of a step
