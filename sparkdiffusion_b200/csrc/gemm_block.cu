@@ -8,6 +8,8 @@
 // K = 32), and the running sum is kept in fp32 registers: the epilogue warps
 // read every block's accumulator and add it times xs * ws.  Both sums are fp32;
 // the result is rounded once, to bf16.
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -63,6 +65,8 @@ __device__ __forceinline__ void store_row(const uint64_t (&acc)[n], const __nv_b
 // bounds it: every 128 columns x 128 k of products, 64 x 4 clocks of the tensor core,
 // pass through a barrier each way.  SM pairs (256 x 256 tiles, whose hand-offs cross
 // SMs) 1340 with the hand-offs alone.
+// Few tiles (kSplit): the CTAs of a cluster share a 128 x 128 tile, each takes a run
+// of its K blocks; the sums meet in shared memory and are added in the CTAs' order.
 // A warp of its own copies the scales of the next kScales blocks into shared
 // memory (4-byte cp.async, so any strides): loaded by the epilogue itself, even
 // four blocks ahead, they held it to one L2 access per block (1260 TFLOP/s).
@@ -74,6 +78,7 @@ constexpr int EPI_WARPS = 8, THREADS = 128 + 32 * EPI_WARPS;
 constexpr int LAUNCH_REGS = 168, REGS_LOAD = 56, REGS_EPI = 224;  // 65536 / 384, in steps of 8
 static_assert(128 * REGS_LOAD + 32 * EPI_WARPS * REGS_EPI <= THREADS * LAUNCH_REGS, "register split");
 constexpr int kScales = 8;                    // blocks whose scales are on their way
+constexpr int SUM_LD = 132;                   // kSplit: floats of a row of sums (+ 4: rows shift by four banks)
 template <int BN>
 struct Cfg {
   static constexpr int A_BYTES = BM * BK, B_BYTES = BN * BK, STAGE = A_BYTES + B_BYTES;
@@ -95,7 +100,11 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-template <int BN>
+__device__ __forceinline__ void ld_cluster(uint32_t a, float4& v) {
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+}
+
+template <int BN, bool kSplit>
 __global__ void __launch_bounds__(gemmb::THREADS, 1)
     gemm_block_tcgen05(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
                             const GemmBlockParams p) {
@@ -120,10 +129,14 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int num_m = (p.M + BM - 1) / BM, num_n = (p.N + BN - 1) / BN;
   const int num_tiles = num_m * num_n;
-  const int nk = (p.K + BK - 1) / BK;
-  const int my_tiles = blockIdx.x < num_tiles ? (num_tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;
+  const int all_k = (p.K + BK - 1) / BK;
+  // this CTA's K blocks [kb0, kb0 + nk) and tiles
+  const int rank = kSplit ? (int)cluster_ctarank() : 0, ks = kSplit ? p.ks : 1;
+  const int kb0 = kSplit ? all_k * rank / ks : 0;
+  const int nk = kSplit ? all_k * (rank + 1) / ks - kb0 : all_k;
+  const int my_tiles = kSplit ? 1 : blockIdx.x < num_tiles ? (num_tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;
   auto tile_coords = [&](int lt, int& m0, int& n0) {
-    const int tile = blockIdx.x + lt * gridDim.x;
+    const int tile = kSplit ? blockIdx.x / ks : blockIdx.x + lt * gridDim.x;
     const int per_group = GROUP_M * num_n;
     const int g = tile / per_group, r = tile % per_group;
     const int gm = min(GROUP_M, num_m - g * GROUP_M);
@@ -176,10 +189,10 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
           }
           const uint32_t sa = base + s * C::STAGE;
           mbar_expect_tx(full(s), C::STAGE);
-          tma_load_2d(sa, &ta, full(s), kb * BK, m0);
+          tma_load_2d(sa, &ta, full(s), (kb0 + kb) * BK, m0);
 #pragma unroll
           for (int h = 0; h < C::STREAMS; ++h)
-            tma_load_2d(sa + C::A_BYTES + h * 128 * BK, &tb, full(s), kb * BK, n0 + 128 * h);
+            tma_load_2d(sa + C::A_BYTES + h * 128 * BK, &tb, full(s), (kb0 + kb) * BK, n0 + 128 * h);
         }
       }
       // no load is still writing shared memory when the CTA exits
@@ -222,7 +235,7 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
     for (int lt = 0; lt < my_tiles && ok; ++lt) {
       int m0, n0;
       tile_coords(lt, m0, n0);
-      const float* ws = p.ws + (int64_t)min((n0 >> 7) + lane % C::STREAMS, (p.N - 1) >> 7) * p.ws_ld;
+      const float* ws = p.ws + (int64_t)min((n0 >> 7) + lane % C::STREAMS, (p.N - 1) >> 7) * p.ws_ld + kb0;
       for (int kb = 0; kb < nk; ++kb, ++it) {
         const int c = it % kScales;
         ok = __all_sync(0xffffffffu, mbar_spin(sc_empty(c), ((it / kScales) & 1) ^ 1, abort_flag, kDevTimeoutSoftmax));
@@ -231,7 +244,7 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int64_t m = min(m0 + 32 * i + lane, p.M - 1);
-          cp_async4(dst + 4 * (32 * i + lane), p.xs + m * p.xs_sM + kb * p.xs_sK);
+          cp_async4(dst + 4 * (32 * i + lane), p.xs + m * p.xs_sM + (kb0 + kb) * p.xs_sK);
         }
         if (lane < C::STREAMS) cp_async4(dst + 4 * (128 + lane), ws + kb);
         cp_async_arrive(sc_full(c));
@@ -291,7 +304,20 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
           scaled_add(acc[i], v[i & 1], s2);
         }
       }
-      if (ok && m < p.M) {
+      if (kSplit) {
+        // every load has landed and every product is done (the last block's was), so the
+        // stages hold nothing any more: this CTA's sums take their place
+        float4* dst = reinterpret_cast<float4*>(gbase + row * SUM_LD * 4 + C::CW * 4 * group);
+#pragma unroll
+        for (int c = 0; c < C::CW / 32; ++c)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float4 f;
+            f2_unpack(acc[c][2 * i], f.x, f.y);
+            f2_unpack(acc[c][2 * i + 1], f.z, f.w);
+            if (ok) dst[8 * c + i] = f;
+          }
+      } else if (ok && m < p.M) {
         __nv_bfloat16* out = p.out + m * p.N;
 #pragma unroll
         for (int c = 0; c < C::CW / 32; ++c) store_row(acc[c], p.bias, out, col + 32 * c, p.N);
@@ -305,6 +331,29 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (kSplit) {
+    cluster_sync_all();  // every CTA's sums are in its shared memory
+    int m0, n0;
+    tile_coords(0, m0, n0);
+    // rows [128 rank / ks, 128 (rank + 1) / ks): 16 threads a row, 8 columns each
+    const int col = 8 * (threadIdx.x & 15);
+    for (int row = 128 * rank / ks + (threadIdx.x >> 4); row < 128 * (rank + 1) / ks; row += THREADS / 16) {
+      if (m0 + row >= p.M) break;
+      float f[8] = {};
+      for (int r = 0; r < ks; ++r) {
+        const uint32_t src = mapa_shared(base + (row * SUM_LD + col) * 4, r);
+        float4 a, b;
+        ld_cluster(src, a);
+        ld_cluster(src + 16, b);
+        f[0] += a.x, f[1] += a.y, f[2] += a.z, f[3] += a.w;
+        f[4] += b.x, f[5] += b.y, f[6] += b.z, f[7] += b.w;
+      }
+      const uint64_t acc[4] = {f2_pack(f[0], f[1]), f2_pack(f[2], f[3]), f2_pack(f[4], f[5]), f2_pack(f[6], f[7])};
+      store_row(acc, p.bias, p.out + (int64_t)(m0 + row) * p.N, n0 + col, p.N);
+    }
+    __syncwarp();
+    cluster_sync_all();  // no CTA leaves while another reads its sums
+  }
 }
 
 template <int BN>
@@ -312,11 +361,34 @@ static int launch_gemm_block_bn(const CUtensorMap& ta, const CUtensorMap& tb, co
                                 cudaStream_t s) {
   using C = gemmb::Cfg<BN>;
   static KernelReady ready;
-  const int rc = kernel_ready(ready, gemm_block_tcgen05<BN>, C::SMEM, gemmb::LAUNCH_REGS);
+  const int rc = kernel_ready(ready, gemm_block_tcgen05<BN, false>, C::SMEM, gemmb::LAUNCH_REGS);
   if (rc != 0) return rc;
   const int64_t tiles = (int64_t)((p.M + 127) / 128) * ((p.N + BN - 1) / BN);
-  gemm_block_tcgen05<BN><<<(unsigned)(tiles < sms ? tiles : sms), gemmb::THREADS, C::SMEM, s>>>(ta, tb, p);
+  gemm_block_tcgen05<BN, false><<<(unsigned)(tiles < sms ? tiles : sms), gemmb::THREADS, C::SMEM, s>>>(ta, tb, p);
   return (int)cudaGetLastError();
+}
+
+// ks CTAs a tile of 128 x 128
+static int launch_gemm_block_split(const CUtensorMap& ta, const CUtensorMap& tb, GemmBlockParams p, int tiles, int ks,
+                                   cudaStream_t s) {
+  using C = gemmb::Cfg<128>;
+  static_assert(128 * gemmb::SUM_LD * 4 <= C::OFF_SC, "the sums take the stages' place");
+  static KernelReady ready;
+  const int rc = kernel_ready(ready, gemm_block_tcgen05<128, true>, C::SMEM, gemmb::LAUNCH_REGS);
+  if (rc != 0) return rc;
+  p.ks = ks;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = (unsigned)ks;
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(tiles * ks));
+  cfg.blockDim = dim3(gemmb::THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = s;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, gemm_block_tcgen05<128, true>, ta, tb, p);
 }
 
 // ---------------------------------------------------------------------------
@@ -409,14 +481,21 @@ static int launch_gemm_block_few_rows(const GemmBlockParams& p, cudaStream_t s) 
 // one wave of each, 128 x 5120 x 5120, 27.5 | 19.5)
 int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, cudaStream_t s) {
   // Up to 8 rows the weight's bytes decide (M = 8, us, few rows | tiles: N x K =
-  // 15360 x 5120 18.9 | 19.5, 5120 x 5120 9.1 | 17, 1536 x 1536 3.7 | 7.8); from 9
-  // to 16 the second token tile costs, and only narrow outputs gain (M = 16: 29 |
-  // 19.5, 15.5 | 17, 4.0 | 7.8).
+  // 15360 x 5120 18.9 | 19.5, 5120 x 5120 9.1 | 13.2, 1536 x 1536 3.7 | 7.8); from 9
+  // to 16 the second token tile costs, and only small weights gain (M = 16: 29 |
+  // 19.5, 15.5 | 13.2, 4.0 | 7.8).
   if (p.M <= 8) return launch_gemm_block_few_rows<1>(p, s);
-  if (p.M <= 16 && p.N <= 8192) return launch_gemm_block_few_rows<2>(p, s);
+  if (p.M <= 16 && (int64_t)p.N * p.K <= (16 << 20)) return launch_gemm_block_few_rows<2>(p, s);
   const int sms = device_sms();
   const int64_t num_m = (p.M + 127) / 128;
   const int64_t wide = (num_m * ((p.N + 255) / 256) + sms - 1) / sms, narrow = (num_m * ((p.N + 127) / 128) + sms - 1) / sms;
+  const int64_t tiles = num_m * ((p.N + 127) / 128), nk = (p.K + 127) / 128;
+  // Few tiles: their K blocks are cut over the CTAs of a cluster while most SMs can take
+  // one (clusters do not fill every group of SMs) and 8 blocks are left to each (us,
+  // whole | cut: 128 x 5120 x 5120 17.3 | 13.2 by 3, 128 x 1536 x 8960 25.4 | 14.0 by 4;
+  // 4 blocks each, 128 x 1536 x 1536 9.0 | 9.6)
+  const int64_t most = std::min<int64_t>(4, std::min(sms * 7 / 8 / tiles, nk / 8));
+  if (most > 1) return launch_gemm_block_split(ta, tb, p, (int)tiles, (int)most, s);
   return narrow * 60 < wide * 100 ? launch_gemm_block_bn<128>(ta, tb, p, sms, s)
                                   : launch_gemm_block_bn<256>(ta, tb, p, sms, s);
 }

@@ -223,6 +223,7 @@ struct GemmBlockParams {
   __nv_bfloat16* out;         // [M, N]
   int64_t xs_sM, xs_sK, ws_ld;
   int M, N, K;
+  int ks;  // CTAs that share a tile's K blocks (few tiles)
 };
 int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, cudaStream_t s);
 

@@ -568,6 +568,10 @@ PRODUCT = {
     "rows_16_wide": (16, 9000, 400, True),
     "tall": (2049, 24, 128, False),
     "many_tiles": (1500, 2600, 656, True),
+    # a tile shared by 2, 3 and 4 CTAs, even and uneven runs of K blocks
+    "shared_by_2": (130, 3800, 2064, True),
+    "shared_by_3": (100, 5000, 3088, False),
+    "shared_by_4": (200, 1000, 4112, True),
     # several tiles a CTA, of both widths
     "persistent_narrow": (2000, 2600, 144, True),
     "persistent_wide": (3500, 2560, 272, False),
