@@ -42,6 +42,10 @@ ATTENTION = {
     "few_rows_split": (1, 2, 2, 130, 3000, None),
     "packed_128_rows": (1, 8, 1, 16, 700, (641,)),
     "unpacked_136_rows": (1, 8, 1, 17, 700, (641,)),
+    # runs that end in the midst of items, of one and two query tiles; empty and short sequences between
+    "ragged_tokens": (6, 8, 2, 1, 3000, (0, 3000, 1, 129, 2999, 640)),
+    "ragged_rows": (3, 4, 4, 200, 2100, (2100, 0, 300)),
+    "fewer_tiles_than_runs": (4, 3, 3, 2, 4000, (5, 0, 130, 0)),
     "row_tail": (1, 2, 2, 129, 64, None),
     "key_tail": (2, 2, 1, 127, 257, (257, 129)),
     "empty_rows": (3, 2, 2, 70, 129, (0, 128, 129)),
