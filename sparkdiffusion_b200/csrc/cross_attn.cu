@@ -18,16 +18,23 @@
 // own, and they run across the items' ends: an encoder's states are few keys (512:
 // four units), and the S products of the next item are issued while this one
 // finishes.  m and l pass from unit to unit through shared memory, in order.
-//   warp 0        TMA producer of Q (2 x 32 KB) and K tiles (2 x 32 KB); it also stores
-//                 an item's output, left in the item's Q tile, before the tile is loaded
-//                 again (rows stored by the lanes themselves held their warps 2500 clocks)
+//   warp 0        TMA producer of Q (2 x 32 KB) and K tiles (2 x 32 KB)
 //   warp 3        TMA producer of V tiles (3 x 32 KB)
+//                 Both also store the outputs that wait in their tiles (out_in_q;
+//                 rows stored by the lanes themselves held their warps 2500 clocks)
 //   warp 1        issues S; owner of the tensor memory
 //   warp 2        issues P V.  It also clears the V rows past len[b] (their P is 0,
 //                 but 0 * NaN is not).  One warp for both products was the limit:
 //                 2150 clocks a unit to issue what takes the tensor core 1024
 //   warpgroup g = 1, 2, 3: the units u with u % 3 == g - 1; thread = row = TMEM lane.
 //                 The unit that ends an item scales its O by 1/l and leaves it in bf16.
+// Measured alone: 32760 rows x 512 keys, 40 heads 322 us (1068 TFLOP/s, 0.64 of the
+// matrix peak), 32760 x 8192, 4 heads 413 us (1330, 0.79); in a long run the power
+// limit takes 10 to 15 % of the clock.  With many keys a unit takes 1600 clocks, of
+// which its products need 1041 and its exponentials 1024: neither is full, the three
+// chains are what bounds it; an item's end costs some 1400 clocks more.  Tried and
+// slower: two S and two P tiles apart (the next S starts once its tile is read, but
+// only two wait), half units for four warpgroups, a warpgroup of its own for the outputs.
 // Few rows: the keys of an item are cut into slices, each leaves O/l in fp32 and
 // its log-sum-exp, and combine_kernel joins them.  When the G query heads of a
 // key head have 128 rows or fewer together, they form one tile (one read of K/V
