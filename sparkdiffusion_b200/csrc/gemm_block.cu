@@ -127,8 +127,7 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gbase + C::OFF_BAR + 328);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int num_m = (p.M + BM - 1) / BM, num_n = (p.N + BN - 1) / BN;
-  const int num_tiles = num_m * num_n;
+  const int num_tiles = p.tiles;
   const int all_k = (p.K + BK - 1) / BK;
   // this CTA's K blocks [kb0, kb0 + nk) and tiles
   const int rank = kSplit ? (int)cluster_ctarank() : 0, ks = kSplit ? p.ks : 1;
@@ -136,12 +135,17 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
   const int nk = kSplit ? all_k * (rank + 1) / ks - kb0 : all_k;
   const int my_tiles = kSplit ? 1 : blockIdx.x < num_tiles ? (num_tiles - 1 - blockIdx.x) / gridDim.x + 1 : 0;
   auto tile_coords = [&](int lt, int& m0, int& n0) {
-    const int tile = kSplit ? blockIdx.x / ks : blockIdx.x + lt * gridDim.x;
+    int tile = kSplit ? blockIdx.x / ks : blockIdx.x + lt * gridDim.x, half = 0, width = BN;
+    if (BN == 128 && p.tile0 >= 0) {  // the halves of the wide tiles from tile0 on
+      half = tile & 1, width = 256;
+      tile = p.tile0 + (tile >> 1);
+    }
+    const int num_m = (p.M + BM - 1) / BM, num_n = (p.N + width - 1) / width;
     const int per_group = GROUP_M * num_n;
     const int g = tile / per_group, r = tile % per_group;
     const int gm = min(GROUP_M, num_m - g * GROUP_M);
     m0 = (g * GROUP_M + r % gm) * BM;
-    n0 = (r / gm) * BN;
+    n0 = (r / gm) * width + 128 * half;
   };
 
   if (threadIdx.x == 0) {
@@ -356,6 +360,7 @@ __global__ void __launch_bounds__(gemmb::THREADS, 1)
   }
 }
 
+// p.tiles tiles of 128 x BN
 template <int BN>
 static int launch_gemm_block_bn(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, int sms,
                                 cudaStream_t s) {
@@ -363,32 +368,44 @@ static int launch_gemm_block_bn(const CUtensorMap& ta, const CUtensorMap& tb, co
   static KernelReady ready;
   const int rc = kernel_ready(ready, gemm_block_tcgen05<BN, false>, C::SMEM, gemmb::LAUNCH_REGS);
   if (rc != 0) return rc;
-  const int64_t tiles = (int64_t)((p.M + 127) / 128) * ((p.N + BN - 1) / BN);
-  gemm_block_tcgen05<BN, false><<<(unsigned)(tiles < sms ? tiles : sms), gemmb::THREADS, C::SMEM, s>>>(ta, tb, p);
+  gemm_block_tcgen05<BN, false><<<p.tiles < sms ? p.tiles : sms, gemmb::THREADS, C::SMEM, s>>>(ta, tb, p);
   return (int)cudaGetLastError();
 }
 
-// ks CTAs a tile of 128 x 128
-static int launch_gemm_block_split(const CUtensorMap& ta, const CUtensorMap& tb, GemmBlockParams p, int tiles, int ks,
+// p.tiles tiles of 128 x 128, p.ks CTAs each
+static int launch_gemm_block_split(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p,
                                    cudaStream_t s) {
   using C = gemmb::Cfg<128>;
   static_assert(128 * gemmb::SUM_LD * 4 <= C::OFF_SC, "the sums take the stages' place");
   static KernelReady ready;
   const int rc = kernel_ready(ready, gemm_block_tcgen05<128, true>, C::SMEM, gemmb::LAUNCH_REGS);
   if (rc != 0) return rc;
-  p.ks = ks;
   cudaLaunchAttribute cluster;
   cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = (unsigned)ks;
+  cluster.val.clusterDim.x = (unsigned)p.ks;
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(tiles * ks));
+  cfg.gridDim = dim3((unsigned)(p.tiles * p.ks));
   cfg.blockDim = dim3(gemmb::THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = s;
   cfg.attrs = &cluster;
   cfg.numAttrs = 1;
   return (int)cudaLaunchKernelEx(&cfg, gemm_block_tcgen05<128, true>, ta, tb, p);
+}
+
+// p.tiles tiles of 128 x 128.  Few: their K blocks are cut over the CTAs of a cluster
+// while most SMs can take one (clusters do not fill every group of SMs) and 8 blocks
+// are left to each (us, whole | cut: 128 x 5120 x 5120 17.3 | 13.2 by 3, 128 x 1536 x
+// 8960 25.4 | 14.0 by 4; 4 blocks each, 128 x 1536 x 1536 9.0 | 9.6)
+static int gemm_block_cut(int64_t tiles, int K, int64_t sms) {
+  const int64_t most = std::min<int64_t>(4, std::min(sms * 7 / 8 / tiles, (int64_t)((K + 127) / 128 / 8)));
+  return most > 1 ? (int)most : 1;
+}
+static int launch_gemm_block_narrow(const CUtensorMap& ta, const CUtensorMap& tb, GemmBlockParams p, int sms,
+                                    cudaStream_t s) {
+  p.ks = gemm_block_cut(p.tiles, p.K, sms);
+  return p.ks > 1 ? launch_gemm_block_split(ta, tb, p, s) : launch_gemm_block_bn<128>(ta, tb, p, sms, s);
 }
 
 // ---------------------------------------------------------------------------
@@ -474,30 +491,38 @@ static int launch_gemm_block_few_rows(const GemmBlockParams& p, cudaStream_t s) 
   return (int)cudaGetLastError();
 }
 
-// The wider tile unless its last wave of CTAs is so empty that the narrower one,
-// at about 0.6 of its time a tile, finishes first (M x N x K, us, wide | narrow, waves
-// in brackets: 512 x 5120 x 5120 28.2 (1) | 32.8 (2), 1001 x 5120 x 5120 50.0 (2) |
-// 46.0 (3), 4096 x 5120 x 5120 120 (5) | 130 (9), 32760 x 15360 x 5120 2650 | 3040;
-// one wave of each, 128 x 5120 x 5120, 27.5 | 19.5)
-int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, cudaStream_t s) {
+int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, GemmBlockParams p, cudaStream_t s) {
   // Up to 8 rows the weight's bytes decide (M = 8, us, few rows | tiles: N x K =
   // 15360 x 5120 18.9 | 19.5, 5120 x 5120 9.1 | 13.2, 1536 x 1536 3.7 | 7.8); from 9
   // to 16 the second token tile costs, and only small weights gain (M = 16: 29 |
   // 19.5, 15.5 | 13.2, 4.0 | 7.8).
   if (p.M <= 8) return launch_gemm_block_few_rows<1>(p, s);
   if (p.M <= 16 && (int64_t)p.N * p.K <= (16 << 20)) return launch_gemm_block_few_rows<2>(p, s);
-  const int sms = device_sms();
-  const int64_t num_m = (p.M + 127) / 128;
-  const int64_t wide = (num_m * ((p.N + 255) / 256) + sms - 1) / sms, narrow = (num_m * ((p.N + 127) / 128) + sms - 1) / sms;
-  const int64_t tiles = num_m * ((p.N + 127) / 128), nk = (p.K + 127) / 128;
-  // Few tiles: their K blocks are cut over the CTAs of a cluster while most SMs can take
-  // one (clusters do not fill every group of SMs) and 8 blocks are left to each (us,
-  // whole | cut: 128 x 5120 x 5120 17.3 | 13.2 by 3, 128 x 1536 x 8960 25.4 | 14.0 by 4;
-  // 4 blocks each, 128 x 1536 x 1536 9.0 | 9.6)
-  const int64_t most = std::min<int64_t>(4, std::min(sms * 7 / 8 / tiles, nk / 8));
-  if (most > 1) return launch_gemm_block_split(ta, tb, p, (int)tiles, (int)most, s);
-  return narrow * 60 < wide * 100 ? launch_gemm_block_bn<128>(ta, tb, p, sms, s)
-                                  : launch_gemm_block_bn<256>(ta, tb, p, sms, s);
+  // Rounds of tiles over the SMs, in hundredths of a wide tile's time (a narrow one takes
+  // about 0.6 of it, cut ones their part and 0.2; a second launch 0.1): wide tiles, narrow
+  // ones, or whole rounds of wide tiles and the rest as narrow ones (M x N x K, us, the
+  // three: 512 x 5120 x 5120 28.2 | 32.8 | -, 1001 x 5120 x 5120 50.0 | 46.0 | 39.8,
+  // 2048 x 5120 x
+  // 5120 72.5 | - | 64.4, 4096 x 5120 x 5120 120 | 130 | 118, 32760 x 15360 x 5120 2650 | 3040 | -)
+  const int64_t sms = device_sms(), num_m = (p.M + 127) / 128;
+  const int64_t wide = num_m * ((p.N + 255) / 256), narrow = num_m * ((p.N + 127) / 128);
+  const int64_t full = wide / sms * sms, rest = wide - full;
+  auto narrow_cost = [&](int64_t tiles) {
+    const int ks = gemm_block_cut(tiles, p.K, sms);
+    return ks > 1 ? 60 / ks + 20 : 60 * ((tiles + sms - 1) / sms);
+  };
+  const int64_t cost_wide = 100 * ((wide + sms - 1) / sms), cost_narrow = narrow_cost(narrow);
+  const int64_t cost_both = full > 0 && rest > 0 ? 100 * (full / sms) + 10 + narrow_cost(2 * rest) : cost_wide;
+  p.tile0 = -1;
+  if (cost_narrow < cost_wide && cost_narrow <= cost_both) {
+    p.tiles = (int)narrow;
+    return launch_gemm_block_narrow(ta, tb, p, (int)sms, s);
+  }
+  p.tiles = (int)(cost_both < cost_wide ? full : wide);
+  const int rc = launch_gemm_block_bn<256>(ta, tb, p, (int)sms, s);
+  if (rc != 0 || p.tiles == wide) return rc;
+  p.tile0 = (int)full, p.tiles = (int)(2 * rest);
+  return launch_gemm_block_narrow(ta, tb, p, (int)sms, s);
 }
 
 }  // namespace rola

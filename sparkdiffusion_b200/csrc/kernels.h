@@ -223,9 +223,10 @@ struct GemmBlockParams {
   __nv_bfloat16* out;         // [M, N]
   int64_t xs_sM, xs_sK, ws_ld;
   int M, N, K;
-  int ks;  // CTAs that share a tile's K blocks (few tiles)
+  int tiles, tile0;  // of this launch; its tiles are the halves of the 256-column tiles from tile0 on, if >= 0
+  int ks;            // CTAs that share a tile's K blocks (few tiles)
 };
-int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, const GemmBlockParams& p, cudaStream_t s);
+int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, GemmBlockParams p, cudaStream_t s);
 
 // cross_attn.cu -----------------------------------------------------------
 struct CrossAttnPlan {

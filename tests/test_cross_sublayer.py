@@ -572,6 +572,10 @@ PRODUCT = {
     "rows_16_wide": (16, 9000, 400, True),
     "tall": (2049, 24, 128, False),
     "many_tiles": (1500, 2600, 656, True),
+    # rounds of narrow tiles; whole rounds of wide tiles and the rest as narrow ones, shared by CTAs or not
+    "narrow_rounds": (12524, 384, 144, True),
+    "rest_shared": (1300, 3904, 2064, True),
+    "rest_not_shared": (4990, 5000, 400, False),
     # a tile shared by 2, 3 and 4 CTAs, even and uneven runs of K blocks
     "shared_by_2": (130, 3800, 2064, True),
     "shared_by_3": (100, 5000, 3088, False),
