@@ -441,7 +441,8 @@ int rola_b200_cross_attn(const void* q, int64_t q_sB, int64_t q_sH, int64_t q_sT
 /* Its backward: dq [B, H, Lq, 128], dk and dv [B, Hkv, Lk, 128] (shared
  * strides; summed over the query heads of a key head; 0 past kv_lens[b]) from
  * the forward's out and lse and from dout.  No atomics: the same inputs give the
- * same bits.  workspace: rola_b200_cross_attn_bwd_workspace bytes. */
+ * same bits.  workspace: rola_b200_cross_attn_bwd_workspace bytes.  With kv_lens
+ * at most 65536 sequences. */
 size_t rola_b200_cross_attn_bwd_workspace(int B, int H, int Hkv, int Lq, int Lk);
 int rola_b200_cross_attn_bwd(const void* q, int64_t q_sB, int64_t q_sH, int64_t q_sT, const void* k, int64_t k_sB,
                              int64_t k_sH, int64_t k_sT, const void* v, int64_t v_sB, int64_t v_sH, int64_t v_sT,

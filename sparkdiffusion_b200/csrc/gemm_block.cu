@@ -501,9 +501,9 @@ int launch_gemm_block(const CUtensorMap& ta, const CUtensorMap& tb, GemmBlockPar
   // Rounds of tiles over the SMs, in hundredths of a wide tile's time (a narrow one takes
   // about 0.6 of it, cut ones their part and 0.2; a second launch 0.1): wide tiles, narrow
   // ones, or whole rounds of wide tiles and the rest as narrow ones (M x N x K, us, the
-  // three: 512 x 5120 x 5120 28.2 | 32.8 | -, 1001 x 5120 x 5120 50.0 | 46.0 | 39.8,
-  // 2048 x 5120 x
-  // 5120 72.5 | - | 64.4, 4096 x 5120 x 5120 120 | 130 | 118, 32760 x 15360 x 5120 2650 | 3040 | -)
+  // three: 512 x 5120 x 5120 28.2 | 32.8 | -, 1001 x 5120 x 5120 50.0 | 46.0 | 39.8, 2048 x
+  // 5120 x 5120 72.5 | - | 64.4, 4096 x 5120 x 5120 120 | 130 | 118, 32760 x 15360 x 5120
+  // 2650 | 3040 | -)
   const int64_t sms = device_sms(), num_m = (p.M + 127) / 128;
   const int64_t wide = num_m * ((p.N + 255) / 256), narrow = num_m * ((p.N + 127) / 128);
   const int64_t full = wide / sms * sms, rest = wide - full;

@@ -610,6 +610,33 @@ def test_gemm_fp8_block(case):
 
 
 @gpu
+@pytest.mark.parametrize("case", ["shared_by_4", "rest_shared"])
+def test_gemm_fp8_block_shared_tiles_on_streams_and_in_a_graph(case):
+    """Tiles whose K blocks several CTAs share: two calls at once, and captured and replayed with new operands."""
+    M, N, K, _ = PRODUCT[case]
+    ops1, ops2 = (_cuda(*_quantized(M, K, 1, 10 + i), *_quantized(N, K, 128, 20 + i)) for i in range(2))
+    want = [ops.gemm_fp8_block(*o) for o in (ops1, ops2)]
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = []
+    for s, o in zip(side, (ops1, ops2)):
+        with torch.cuda.stream(s):
+            got.append([ops.gemm_fp8_block(*o) for _ in range(4)][-1])
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    buf, g = [t.clone() for t in ops1], torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.gemm_fp8_block(*buf)
+    for o, w in ((ops1, want[0]), (ops2, want[1])):
+        for b, t in zip(buf, o):
+            b.copy_(t)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, w)
+    _ok()
+
+
+@gpu
 def test_gemm_fp8_block_nan_stays_in_its_row():
     (xq, xs), (wq, ws) = _quantized(200, 256, 1, 1), _quantized(64, 256, 128, 2)
     xs[5, 1] = float("nan")
