@@ -375,8 +375,12 @@ __global__ void __launch_bounds__(xdq::THREADS, 1)
         if (u % NS != g) continue;
         if (!wait(SF + g, ph, kDevTimeoutMma)) break;
         if (!have_delta) {
-          // only with a step of the item at hand: a warpgroup without one may find the
-          // barrier two phases on, which parity cannot tell from not yet
+          // Only with a step of the item at hand: a warpgroup without one may find the
+          // barrier two phases on, which parity cannot tell from not yet.  Items of one step
+          // wait too, although they make delta themselves: the item's TE, and with it the
+          // reload of its tiles, comes behind this wait, which keeps the delta warps within
+          // NT items (nothing else does; they too know phases by parity)
+          if (!wait(DR + j % NT, (j / NT) & 1, kDevTimeoutSoftmax)) break;
           float dlt = 0.f;
           if (cnt == 1) {
             // every key of the row is here: delta as sum_j P dP, from fp32 alone
@@ -393,7 +397,6 @@ __global__ void __launch_bounds__(xdq::THREADS, 1)
             }
             p.delta[((int64_t)b * p.H + h) * p.Lpad + 128 * m + row] = dlt;
           } else {
-            if (!wait(DR + j % NT, (j / NT) & 1, kDevTimeoutSoftmax)) break;
             dlt = reinterpret_cast<const float*>(smem1k + OFF_DELTA)[(j % NT) * 128 + row];
           }
           nd2 = f2_pack(-dlt, -dlt);

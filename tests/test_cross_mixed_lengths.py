@@ -1,0 +1,38 @@
+"""Attention to another sequence's states over batches in which sequences of one
+64-key step, of several and without keys follow one another in a CTA's items."""
+
+import pytest
+import torch
+
+from oracle import sublayer_oracle as orc
+from sparkdiffusion_b200 import _lib, train
+
+BF16 = torch.bfloat16
+MIXED = {
+    # H, Hkv, Lq, Lk, lens: more items than SMs, so that every CTA meets several lengths
+    "short_and_long": (8, 8, 300, 400, (1, 400, 64, 65, 2, 399, 63, 129) * 2),
+    "short_between_empty": (4, 4, 260, 330, (64, 0, 330, 0, 3, 128, 0, 7, 200, 64, 1, 330) * 2),
+    "shared_heads": (10, 2, 130, 200, (10, 200, 64, 66, 33, 1, 150, 2, 64, 64)),
+    "short_only": (6, 3, 500, 64, (64, 1, 17, 2, 63, 30, 64, 5)),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", sorted(MIXED))
+def test_gradients_over_mixed_lengths(case):
+    H, Hkv, Lq, Lk, lens = MIXED[case]
+    B = len(lens)
+    g = torch.Generator().manual_seed(5)
+    q, do = (torch.randn(B, H, Lq, 128, generator=g).to(BF16) for _ in range(2))
+    k, v = (torch.randn(B, Hkv, Lk, 128, generator=g).to(BF16) for _ in range(2))
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    o = train.cross_attention(*leaves, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    runs = [torch.autograd.grad(o, leaves, do.cuda(), retain_graph=True) for _ in range(8)]
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+    ref = orc.cross_attention_grads(q, k, v, do, lens)
+    for i, name in enumerate(("dq", "dk", "dv")):
+        r, tol = ref[name]
+        worst = ((runs[0][i].cpu().double() - r).abs() / (tol + 1e-30)).max().item()
+        assert worst <= 1.0, f"{name}: {worst:.3f} of the bound"
+        assert all(torch.equal(run[i], runs[0][i]) for run in runs), f"{name}: two runs differ"
