@@ -36,3 +36,29 @@ def test_gradients_over_mixed_lengths(case):
         worst = ((runs[0][i].cpu().double() - r).abs() / (tol + 1e-30)).max().item()
         assert worst <= 1.0, f"{name}: {worst:.3f} of the bound"
         assert all(torch.equal(run[i], runs[0][i]) for run in runs), f"{name}: two runs differ"
+
+
+@pytest.mark.gpu
+def test_a_million_sequences():
+    """Of one token and two states each: the bits of a call on each 65536 of them."""
+    B, part = (1 << 20) + 7, 1 << 16
+    g = torch.Generator("cuda").manual_seed(6)
+    q, do = (torch.randn(B, 1, 1, 128, device="cuda", generator=g).to(BF16) for _ in range(2))
+    k, v = (torch.randn(B, 1, 2, 128, device="cuda", generator=g).to(BF16) for _ in range(2))
+
+    def step(at):
+        leaves = [t[at].detach().requires_grad_(True) for t in (q, k, v)]
+        o = train.cross_attention(*leaves)
+        return (o.detach(), *torch.autograd.grad(o, leaves, do[at]))
+
+    got = step(slice(None))
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0
+    for b in range(0, B, part):
+        for name, a, w in zip(("o", "dq", "dk", "dv"), got, step(slice(b, b + part))):
+            assert torch.equal(a[b:b + part], w), (name, b)
+    last = slice(B - 50, B)
+    ref = orc.cross_attention_grads(*(t[last].cpu() for t in (q, k, v, do)))
+    for name, a in zip(("dq", "dk", "dv"), got[1:]):
+        r, tol = ref[name]
+        assert bool(((a[last].cpu().double() - r).abs() <= tol + 1e-30).all()), name
