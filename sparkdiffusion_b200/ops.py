@@ -698,6 +698,7 @@ def sparse_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: t
 # product, attention to an encoder's states
 # ---------------------------------------------------------------------------
 SCALE_BLOCK = 128  # values that share a scale
+MAX_BWD_LENS = 65536  # sequences of their own lengths in one cross_attention_bwd
 E4M3 = torch.float8_e4m3fn
 
 
@@ -1022,7 +1023,7 @@ def cross_attention_bwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, o: to
                         ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Gradients ``(dq, dk, dv)`` (bf16) of ``cross_attention`` given its ``o``,
     ``lse`` and ``do = dL/do``; dk and dv sum over the query heads of a key head.
-    The same inputs give the same bits."""
+    With ``kv_lens`` at most 65536 sequences.  The same inputs give the same bits."""
     what = "cross_attention_bwd"
     dev, sizes, lens = _cross_args(what, q, k, v, kv_lens)
     B, H, Hkv, Lq, Lk = sizes

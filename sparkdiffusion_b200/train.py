@@ -250,7 +250,12 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                     kv_lens: torch.Tensor | None = None) -> torch.Tensor:
     """Differentiable attention of ``q [B, H, Lq, 128]`` to the states ``k, v
     [B, Hkv, Lk, 128]`` (``ops.cross_attention``), in the input dtype; beside
-    ``dense_attention``, which takes one length."""
+    ``dense_attention``, which takes one length.  With ``kv_lens`` at most 65536
+    sequences where a gradient is asked for (the backward kernels' limit)."""
+    if (kv_lens is not None and q.shape[0] > ops.MAX_BWD_LENS and torch.is_grad_enabled()
+            and any(t.requires_grad for t in (q, k, v))):
+        raise ValueError(f"cross_attention: {q.shape[0]} sequences of their own lengths, the backward takes at most "
+                         f"{ops.MAX_BWD_LENS}")
     if not q.is_cuda:
         raise RuntimeError("the B200 training path runs on CUDA tensors only")
     dt, bf16 = q.dtype, torch.bfloat16

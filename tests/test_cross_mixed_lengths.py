@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from oracle import sublayer_oracle as orc
-from sparkdiffusion_b200 import _lib, train
+from sparkdiffusion_b200 import _lib, ops, train
 
 BF16 = torch.bfloat16
 MIXED = {
@@ -62,3 +62,30 @@ def test_a_million_sequences():
     for name, a in zip(("dq", "dk", "dv"), got[1:]):
         r, tol = ref[name]
         assert bool(((a[last].cpu().double() - r).abs() <= tol + 1e-30).all()), name
+
+
+def _ragged(B, device="cpu"):
+    t = [torch.zeros(B, 1, 1, 128, device=device, dtype=BF16, requires_grad=True) for _ in range(3)]
+    return t, torch.ones(B, device=device, dtype=torch.int32)
+
+
+def test_too_many_lengths_are_refused_before_the_forward():
+    """What the backward cannot take is refused when the gradient is asked for, not after the forward."""
+    t, lens = _ragged(ops.MAX_BWD_LENS + 1)
+    with pytest.raises(ValueError, match="65536"):
+        train.cross_attention(*t, lens)
+    with pytest.raises(RuntimeError, match="CUDA"):  # no gradient asked for: on to the next check
+        train.cross_attention(*(x.detach() for x in t), lens)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        train.cross_attention(*t)
+
+
+@pytest.mark.gpu
+def test_as_many_lengths_as_the_backward_takes():
+    t, lens = _ragged(ops.MAX_BWD_LENS, "cuda")
+    dq, dk, dv = torch.autograd.grad(train.cross_attention(*t, lens).sum(), t)
+    assert bool((dv == 1).all()) and bool((dq == 0).all()) and bool((dk == 0).all())
+    many, lens = _ragged(ops.MAX_BWD_LENS + 1, "cuda")
+    with torch.no_grad():
+        assert bool((train.cross_attention(*many, lens) == 0).all())
+    assert _lib.device_status() == 0
