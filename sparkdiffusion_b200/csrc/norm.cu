@@ -213,6 +213,18 @@ __global__ void __launch_bounds__(128) add_rms_norm_warp_kernel(const AddRmsNorm
   }
 }
 
+// End of a ring's CTA of `rows` rows, whose thread 0 has seen the first `seen` arrive.
+// Fewer than all only after a wait that ran out (which has set the device error; what
+// was computed from there on is undefined): the copies on their way land before shared
+// memory goes.
+__device__ __forceinline__ void ring_drain(const uint64_t* bars, int ring, int rows, int seen) {
+  if (threadIdx.x != 0 || seen == rows) return;
+  const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
+  const int fetched = min(rows, seen + ring);
+  for (int n = seen; n < fetched; ++n)
+    if (!mbar_wait_until(smem_u32(&bars[n % ring]), (n / ring) & 1, deadline)) return;
+}
+
 // Longer rows: a CTA each, the next rows on their way.  Thread 0 fetches whole
 // rows of x and res by bulk copies into a ring of kRing shared-memory stages (fewer where rows are too long);
 // the barrier of the row's reduction also says that its stage is free.
@@ -237,11 +249,10 @@ __global__ void __launch_bounds__(512) add_rms_norm_ring_kernel(const AddRmsNorm
       if (blockIdx.x + (int64_t)s * gridDim.x < p.M) fetch(blockIdx.x + (int64_t)s * gridDim.x, s);
   }
   __syncthreads();
-  int n = 0;
-  bool ok = true;
+  int n = 0, seen = 0;  // rows; of them arrived (fewer once a wait has run out)
   for (int64_t m = blockIdx.x; m < p.M; m += gridDim.x, ++n) {
     const int s = n % p.ring;
-    if (ok) ok = mbar_wait_until(smem_u32(&s_bar[s]), (n / p.ring) & 1, globaltimer_ns() + kWaitLimitNs);
+    if (seen == n) seen += mbar_wait_until(smem_u32(&s_bar[s]), (n / p.ring) & 1, globaltimer_ns() + kWaitLimitNs);
     const uint8_t* xs = smem_ring + s * stage;
     float v[NV][8];
 #pragma unroll
@@ -256,9 +267,10 @@ __global__ void __launch_bounds__(512) add_rms_norm_ring_kernel(const AddRmsNorm
     }
     norm_row<NV, false, kOut>(p, m, v, s_red[n & 1], [&] {
       const int64_t next = m + (int64_t)p.ring * gridDim.x;
-      if (threadIdx.x == 0 && next < p.M) fetch(next, s);
+      if (threadIdx.x == 0 && seen > n && next < p.M) fetch(next, s);
     });
   }
+  ring_drain(s_bar, p.ring, n, seen);
 }
 
 // Backward.  With u = h r (the unit rows), g = dy w:
@@ -353,17 +365,17 @@ __global__ void __launch_bounds__(512) add_rms_norm_bwd_ring_kernel(const AddRms
   }
   __syncthreads();
   float dw[NV][8] = {};
-  int n = 0;
-  bool ok = true;
+  int n = 0, seen = 0;  // rows; of them arrived (fewer once a wait has run out)
   for (int64_t m = blockIdx.x; m < p.M; m += gridDim.x, ++n) {
     const int s = n % p.ring;
-    if (ok) ok = mbar_wait_until(smem_u32(&s_bar[s]), (n / p.ring) & 1, globaltimer_ns() + kWaitLimitNs);
+    if (seen == n) seen += mbar_wait_until(smem_u32(&s_bar[s]), (n / p.ring) & 1, globaltimer_ns() + kWaitLimitNs);
     const uint8_t* hs = smem_ring + s * stage;
     norm_bwd_row<NV, false>(p, m, hs, 0, hs + hb, 0, db ? hs + hb + yb : nullptr, 0, dw, s_red[n & 1], [&] {
       const int64_t next = m + (int64_t)p.ring * gridDim.x;
-      if (threadIdx.x == 0 && next < p.M) fetch(next, s);
+      if (threadIdx.x == 0 && seen > n && next < p.M) fetch(next, s);
     });
   }
+  ring_drain(s_bar, p.ring, n, seen);
   store_dw_part<NV>(p, blockIdx.x, threadIdx.x, blockDim.x, dw);
 }
 
