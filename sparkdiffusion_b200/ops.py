@@ -914,7 +914,9 @@ def gemm_fp8_block(xq: torch.Tensor, x_scale: torch.Tensor, wq: torch.Tensor, w_
     w_scale[n // 128, kb] * (xq . wq^T) + bias)`` on e4m3 operands ``xq [M, K]``,
     ``wq [N, K]`` (``add_rms_norm_e4m3`` or ``quantize_blocks_e4m3``, and
     ``quantize_tiles_e4m3``), fp32 sums.  Beside ``qkv_gemm_fp8``, whose scales
-    are one per row.  N % 8 == 0, K % 16 == 0."""
+    are one per row.  N % 8 == 0, K % 16 == 0.  A row's bits do not depend on the
+    other rows' values, but on their number: M chooses among kernels that add the
+    K blocks in different orders."""
     what = "gemm_fp8_block"
     dev = _device_of(what, xq, x_scale, wq, w_scale, bias)
     if xq.dtype is not E4M3 or wq.dtype is not E4M3:
