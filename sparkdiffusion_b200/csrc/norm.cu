@@ -18,10 +18,10 @@
 // take a warp each (no barrier), longer ones a CTA, whose next rows are fetched by
 // bulk copies meanwhile (loads by the threads themselves left the memory idle
 // between a row's load and its barriers: 255 us instead of 206 in the first line).
-// Measured: 32760 x 5120, x bf16, res fp32, to e4m3: 206 us, 5.7 TB/s (0.88 of a
-// copy's rate); 32760 x 1536 bf16: 37 us, 5.4 TB/s; forward and backward of 32760 x
-// 5120 with its weight's gradient 771 us at 28 bytes an element, 6.1 TB/s (0.94);
-// 4 rows 3.1 us, a launch.
+// Measured: 32760 x 5120, x and res bf16, to e4m3: 206 us, 5.7 TB/s (0.88 of a copy's
+// rate); 16381 x 1536, x and res bf16, to bf16: 37 us, 5.4 TB/s; forward and backward
+// of 32760 x 5120, x bf16, res fp32, with the weight's gradient 771 us at 28 bytes an
+// element, 6.1 TB/s (0.94); 4 rows 3.2 us, a launch.
 #include <atomic>
 
 #include "common.cuh"
