@@ -158,8 +158,8 @@ def dq_kernel(items, one_step_waits=True):
 
     roles = {"query tiles": query_tiles(), "keys": keys(), "scores": scores(), "gradient": gradient()}
     roles.update({f"delta warp {w}": delta() for w in range(4)})
-    roles.update({f"softmax {g}": softmax(g) for g in range(3)})
-    return roles, {"DR": 4}
+    roles.update({f"softmax {g} warp {w}": softmax(g) for g in range(3) for w in range(4)})
+    return roles, dict.fromkeys(("DR", "DS", "OE", "TE"), 4)
 
 
 def dkdv_kernel(segments):
@@ -293,8 +293,8 @@ def forward_kernel(items, rescale):
                 yield arrive("OQ", j % 2) if in_q(cnt) else arrive("OV", u % 3)
 
     roles = {"query tiles": query_tiles(), "values": values(), "scores": scores(), "outputs": outputs()}
-    roles.update({f"softmax {g}": softmax(g) for g in range(3)})
-    return roles, {}
+    roles.update({f"softmax {g} warp {w}": softmax(g) for g in range(3) for w in range(4)})
+    return roles, dict.fromkeys(("PA", "PB", "MR", "LR", "OE", "OQ", "OV"), 4)
 
 
 # steps of the items of a CTA: of one step, of one and of several by turns (lengths of a batch), without keys
@@ -334,7 +334,7 @@ def test_dq_kernel_without_the_wait_of_one_step_items(items, found):
 def test_dq_kernel_without_the_wait_reads_an_older_delta():
     """The other side of the same missing wait: with a delta warp late between its item's load and its
     arrival, an item of several steps passes on the phase of the one-step item before it in its slot."""
-    with pytest.raises(Violation, match=r"softmax \d: phase 1 of \('DR', 0\) passed after 0 phases"):
+    with pytest.raises(Violation, match=r"softmax \d warp \d: phase 1 of \('DR', 0\) passed after 0 phases"):
         for seed in range(1000):
             roles, counts = dq_kernel([1, 1, 2], one_step_waits=False)
             replay(roles, counts, random.Random(seed), "delta warp 2", after=1)
